@@ -47,6 +47,24 @@ class Epilogue(C.Structure):
                 ("rms_weight", C.c_void_p), ("rms_eps", C.c_float), ("rms_out", C.c_void_p)]
 
 
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_NTK, ROPE_SCALE_YARN, ROPE_SCALE_WAVELENGTH = range(5)
+
+
+class RopeScaling(C.Structure):
+    """AccelHipRopeScaling."""
+
+    _fields_ = [("kind", C.c_int32), ("theta", C.c_double), ("factor", C.c_double), ("original_context", C.c_double),
+                ("fast", C.c_double), ("slow", C.c_double)]
+
+
+class CacheQ8(C.Structure):
+    """AccelHipCacheQ8."""
+
+    _fields_ = [("k", Buffer), ("v", Buffer), ("k_scale", Buffer), ("v_scale", Buffer), ("capacity", C.c_int64),
+                ("kv_heads", C.c_int64), ("head_dim", C.c_int64), ("block", C.c_int64)]
+
+
 WORK_FN = C.CFUNCTYPE(C.c_int, C.c_void_p)
 
 # name -> (restype, argtypes)
@@ -94,6 +112,13 @@ SIGNATURES = {
     "accel_hip_silu_mul": (C.c_int, [Buffer, Buffer, i64]),
     "accel_hip_residual_add": (C.c_int, [Buffer, Buffer, i64]),
     "accel_hip_sample_token": (C.c_int, [Buffer, Buffer, i64, i64, C.c_float, U32P, C.c_int32]),
+    "accel_hip_rope_frequencies": (C.c_int, [C.POINTER(RopeScaling), i64, Buffer, F32P]),
+    "accel_hip_rope_scaled": (C.c_int, [Buffer, Buffer, Buffer, Buffer, i64, i64, i64, i64, i64, C.c_int32, i64,
+                                        C.c_float]),
+    "accel_hip_append_cache_q8": (C.c_int, [Buffer, Buffer, C.POINTER(CacheQ8), i64, i64, i64]),
+    "accel_hip_read_cache_q8": (C.c_int, [C.POINTER(CacheQ8), i64, i64, Buffer, Buffer]),
+    "accel_hip_attention_q8": (C.c_int, [Buffer, C.POINTER(CacheQ8), Buffer, i64, i64, i64, i64, i64, i64]),
+    "accel_hip_attention_window": (C.c_int, [Buffer, Buffer, Buffer, Buffer, i64, i64, i64, i64, i64, i64, i64, i64]),
     "accel_hip_time_ms": (C.c_double, [WORK_FN, C.c_void_p, C.c_int32]),
     "accel_hip_event_record": (C.c_int, [C.c_int32]),
     "accel_hip_event_elapsed_ms": (C.c_double, [C.c_int32, C.c_int32]),

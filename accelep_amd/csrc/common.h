@@ -457,6 +457,44 @@ constexpr size_t kDecodeSplitMaxBytesPerHead = 64 * (2 + 64) * sizeof(float);
 // Scratch bytes LaunchAttention needs for these sizes (0 when none).
 size_t AttentionWorkBytes(int64_t seq, int64_t heads, int64_t max_position, int64_t head_dim);
 size_t AttentionFlashWorkBytes(int64_t head_dim);
+// ---- long contexts (rope_scaled.hip, cache_q8.hip, attention_q8.hip, attention_window.hip; the
+// entry points and their checks are in long_context.cc) ----
+struct RopeScaledArgs {
+  const float* states;
+  float* out;
+  const double* frequencies;   // [rotary / 2], radians per position
+  const int32_t* positions;    // [seq] or null
+  int64_t seq, row_stride, position;
+  int32_t heads, dim, rotary, layout;
+  float magnitude;
+};
+void LaunchRopeScaled(const RopeScaledArgs& a, hipStream_t stream);
+// One plane (keys or values) of AccelHipCacheQ8.
+struct Q8Plane {
+  int8_t* code;   // [capacity, kv_heads, dim]
+  float* scale;   // [blocks, kv_heads]
+};
+struct Q8Cache {
+  Q8Plane k, v;
+  int32_t kv_heads, dim;
+  int32_t block_shift;  // log2 of the tokens of a block
+};
+void LaunchAppendCacheQ8(const float* k, const float* v, const Q8Cache& cache, int64_t seq, int64_t position,
+                         int64_t row_stride, hipStream_t stream);
+// k_out or v_out may be null.
+void LaunchReadCacheQ8(const Q8Cache& cache, int64_t first, int64_t count, float* k_out, float* v_out,
+                       hipStream_t stream);
+// Which keys the row at position p sees: t <= p, and t > p - window or t < sinks (kNoWindow: all).
+constexpr int32_t kNoWindow = 0x7fffffff;
+struct AttendArgs {
+  const float* q;  // rows of heads * dim, q_stride apart
+  float* out;      // dense
+  int64_t q_stride;
+  int32_t seq, position, heads, kv_heads, dim;  // position + seq < 2^31 - 256
+  int32_t window, sinks;
+};
+void LaunchAttentionQ8(const AttendArgs& a, const Q8Cache& cache, hipStream_t stream);
+void LaunchAttentionWindow(const AttendArgs& a, const float* k, const float* v, hipStream_t stream);
 // rng_inout is a device word holding the xorshift32 state; index_dev offsets `chosen`.
 // greedy_work (at least GreedyWorkBytes(vocab) bytes, its first word zero and left zero by
 // each launch; launches sharing it must not overlap) lets a greedy pick run over many

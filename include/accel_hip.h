@@ -232,6 +232,77 @@ ACCEL_HIP_API int accel_hip_residual_add(AccelHipBuffer dest, AccelHipBuffer ext
 ACCEL_HIP_API int accel_hip_sample_token(AccelHipBuffer logits, AccelHipBuffer chosen_ids, int64_t chosen_index,
                                          int64_t vocab, float temperature, uint32_t* rng_state, int32_t top_k);
 
+/* ---- long contexts -----------------------------------------------------------------------
+ * No reference counterpart: beside Rope, AppendCache and Attention above, what a long context needs.
+ * These calls also take device memory of this GPU that another allocator made (a buffer with id 0); they
+ * run on the library's stream like every other call, so data written elsewhere has to be there first.
+ * Rows lie `row_stride` floats apart (0: dense). Exact products do not apply to them. */
+enum { ACCEL_HIP_ROPE_HALF = 0, ACCEL_HIP_ROPE_INTERLEAVED = 1 }; /* pair i: dims (i, i + r/2), or (2i, 2i + 1) */
+enum {
+  ACCEL_HIP_ROPE_SCALE_NONE = 0,
+  ACCEL_HIP_ROPE_SCALE_LINEAR = 1,    /* every frequency / factor */
+  ACCEL_HIP_ROPE_SCALE_NTK = 2,       /* theta * factor^(r / (r - 2)) in theta's place */
+  ACCEL_HIP_ROPE_SCALE_YARN = 3,      /* / factor below `slow` turns, as it is above `fast`, a ramp over the pairs between */
+  ACCEL_HIP_ROPE_SCALE_WAVELENGTH = 4 /* the same borders, a ramp over the turns between */
+};
+/* How a model's rotary frequencies theta^(-2i/r) are scaled. A pair's turns are those it makes over
+ * original_context positions; original_context, fast and slow are read by the last two kinds only
+ * (usual borders: fast 32 and slow 1, and fast 4 and slow 1), factor by all but the first. */
+typedef struct AccelHipRopeScaling {
+  int32_t kind; /* ACCEL_HIP_ROPE_SCALE_* */
+  double theta, factor, original_context, fast, slow;
+} AccelHipRopeScaling;
+/* Writes the rotary_dim / 2 frequencies (double, radians per position) of `scaling` into the device
+ * buffer, once per model: it synchronizes and is refused in a capture. *magnitude (may be NULL)
+ * receives what the rotated values are multiplied with: 0.1 ln(factor) + 1 for YaRN with a factor
+ * above 1, otherwise 1. */
+ACCEL_HIP_API int accel_hip_rope_frequencies(const AccelHipRopeScaling* scaling, int64_t rotary_dim,
+                                             AccelHipBuffer frequencies, float* magnitude);
+/* Rotates the first rotary_dim (even) dims of every head by the angle position_s * frequency_i and
+ * multiplies them with magnitude; the other dims come out as they are. states and out are rows of
+ * n_heads * head_dim floats (and row_stride apart both; what lies behind a row's heads is left alone):
+ * the query and key heads of a fused projection's rows turn in one call. out may be states itself, and
+ * may not overlap it otherwise. position_s is position + s, or position + positions[s] where positions
+ * (int32 [seq]) has data. Angles are formed in 64 bits: position_s counts up to 2^32. */
+ACCEL_HIP_API int accel_hip_rope_scaled(AccelHipBuffer states, AccelHipBuffer out, AccelHipBuffer frequencies,
+                                        AccelHipBuffer positions, int64_t seq, int64_t n_heads, int64_t head_dim,
+                                        int64_t row_stride, int64_t rotary_dim, int32_t layout, int64_t position,
+                                        float magnitude);
+/* A layer's KV cache in 8 bits: codes int8 [capacity, kv_heads, head_dim] and one fp32 scale for each
+ * block of `block` tokens and head, [ceil(capacity / block), kv_heads], for keys and values. A value is
+ * code * scale. block is a power of two up to 256, head_dim at most 256. */
+typedef struct AccelHipCacheQ8 {
+  AccelHipBuffer k, v, k_scale, v_scale;
+  int64_t capacity, kv_heads, head_dim, block;
+} AccelHipCacheQ8;
+/* AppendCache into the 8-bit cache: rows [position, position + seq) of k and v (fp32, kv_heads *
+ * head_dim a row). Each touched block and head gets the scale max|x| / 127 of its new rows, or keeps
+ * the scale it has where rows of the block before `position` need more; when it grows, those rows'
+ * codes become the nearest code of code * old / new. A code is the nearest integer to x / scale (the
+ * true quotient; ties to even). Rows of the block from position + seq on do not count any more. A
+ * NaN or an infinity makes its block's scale of that head NaN, and all that is read of it, until the
+ * block is written from its start. The planes must not overlap one another or k and v. */
+ACCEL_HIP_API int accel_hip_append_cache_q8(AccelHipBuffer k, AccelHipBuffer v, const AccelHipCacheQ8* cache,
+                                            int64_t seq, int64_t position, int64_t row_stride);
+/* Rows [first, first + count) of the 8-bit cache as fp32 [count, kv_heads, head_dim], code * scale
+ * rounded once. k_out or v_out without data leaves that plane out. */
+ACCEL_HIP_API int accel_hip_read_cache_q8(const AccelHipCacheQ8* cache, int64_t first, int64_t count,
+                                          AccelHipBuffer k_out, AccelHipBuffer v_out);
+/* Attention (as accel_hip_attention: causal, grouped heads, 1 / sqrt(head_dim)) over the 8-bit cache,
+ * whose rows up to position + seq are written. With window > 0 the row at p sees the keys t <= p with
+ * t > p - window or t < sinks; with window 0 every t <= p. q's rows are row_stride apart, out is dense
+ * and may not overlap q. Rounding: queries and softmax weights enter the products with 22 bits (a
+ * query relative to its row's largest value, a weight to the largest), sums are fp32. */
+ACCEL_HIP_API int accel_hip_attention_q8(AccelHipBuffer q, const AccelHipCacheQ8* cache, AccelHipBuffer out,
+                                         int64_t seq, int64_t position, int64_t heads, int64_t row_stride,
+                                         int64_t window, int64_t sinks);
+/* Attention over an fp32 cache k, v [>= position + seq, kv_heads, head_dim] with a sliding window: the
+ * row at p sees the keys t <= p with t > p - window or t < sinks (window 0: every t <= p). Keys that no
+ * row sees are not read. q's rows are row_stride apart, out is dense and may not overlap q. */
+ACCEL_HIP_API int accel_hip_attention_window(AccelHipBuffer q, AccelHipBuffer k, AccelHipBuffer v, AccelHipBuffer out,
+                                             int64_t seq, int64_t position, int64_t heads, int64_t kv_heads,
+                                             int64_t head_dim, int64_t row_stride, int64_t window, int64_t sinks);
+
 /* ---- timing ----------------------------------------------------------------------------- */
 /* Milliseconds between two HIP events recorded on the library's stream around `iters`
  * back-to-back calls of fn(user); returns < 0 on failure. Used by bench.py. */
