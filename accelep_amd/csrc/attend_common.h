@@ -1,0 +1,90 @@
+// What the attention kernels over the 8-bit cache and in a window share: which keys a block of query
+// rows reads and a row sees, queries and softmax weights as two f16 parts, codes as f16, and the join
+// of key ranges.
+#pragma once
+
+#include "device_common.h"
+
+namespace accel_hip {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Rows are pairs (query s, head g of a key head's group), row = s * group + g: a key head's rows share
+// its keys. The keys that rows [r0, r1) read, in steps of kStep keys: first those before `low` that
+// stay visible, then [low, high). Both parts begin at a multiple of kStep, so a step lies in one part,
+// and scale blocks of kStep tokens and more hold whole steps.
+template <int kStep>
+struct KeyRange {
+  int32_t low, high;          // high: one past the last row's own key
+  int32_t first_steps, steps;
+  int32_t p_first, p_last;    // the rows' positions
+  __device__ __forceinline__ KeyRange(const AttendArgs& a, int32_t r0, int32_t r1, int32_t group) {
+    p_first = a.position + r0 / group;
+    p_last = a.position + (r1 - 1) / group;
+    low = a.window == kNoWindow ? 0 : max(0, p_first - a.window + 1) / kStep * kStep;
+    high = p_last + 1;
+    first_steps = (min(a.sinks, low) + kStep - 1) / kStep;
+    steps = first_steps + (high - low + kStep - 1) / kStep;
+  }
+  __device__ __forceinline__ int32_t Key(int32_t step) const {
+    return step < first_steps ? step * kStep : low + (step - first_steps) * kStep;
+  }
+  // Every row sees every key of the step.
+  __device__ __forceinline__ bool Whole(const AttendArgs& a, int32_t t0) const {
+    const int32_t last = t0 + kStep - 1;
+    return last <= p_first && (t0 > p_last - a.window || last < a.sinks);
+  }
+};
+__device__ __forceinline__ bool Sees(const AttendArgs& a, int32_t p, int32_t t) {
+  return t <= p && (t > p - a.window || t < a.sinks);
+}
+
+__device__ __forceinline__ h2 PackRtz(float x, float y) {
+  return __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
+}
+// x = hi + lo to 22 bits (each part 11, the first rounded towards zero): for |x| between 2^-3 and 2^15
+// the rest is below 2^-22 |x|, under that below 2^-25. Both products with exact f16 operands are exact
+// in the matrix core's fp32 sums.
+__device__ __forceinline__ void SplitF16(float x, float y, h2& hi, h2& lo) {
+  hi = PackRtz(x, y);
+  lo = PackRtz(__builtin_fmaf(static_cast<float>(hi[0]), -1.f, x), __builtin_fmaf(static_cast<float>(hi[1]), -1.f, y));
+}
+
+// 2^(13 - e) for a row whose largest magnitude has the exponent e: the row then fills [2^13, 2^14).
+__device__ __forceinline__ float RowScale(uint32_t top_bits) {
+  const int32_t e = static_cast<int32_t>(top_bits >> 23) - 127;
+  return top_bits == 0 ? 1.f : __uint_as_float(static_cast<uint32_t>(min(13 - e, 127) + 127) << 23);
+}
+
+// Four codes, already biased by 128 (w ^ 0x80808080), as two pairs of f16: 0x64uu is 1024 + uu.
+__device__ __forceinline__ h2 CodesLow(uint32_t w) {
+  return __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - h2{1152, 1152};
+}
+__device__ __forceinline__ h2 CodesHigh(uint32_t w) {
+  return __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - h2{1152, 1152};
+}
+__device__ __forceinline__ h8 Join(h2 a, h2 b, h2 c, h2 d) { return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}; }
+
+// A row's softmax while its keys pass. m: the largest score (in log2 units) so far; l: the sum of
+// p = 2^(s - m). The weighted sum holds p * value scale * 2^power, where `power` keeps the largest
+// p * value scale so far (`top`, relative to m) in [2^14, 2^15): all of f16's range lies below it, and a
+// key that a row does not see has no say in it.
+struct RowState {
+  float m = -INFINITY, l = 0.f, top = 0.f;
+  int32_t power = 127;
+  __device__ __forceinline__ static int32_t PowerOf(float top) {
+    const int32_t e = static_cast<int32_t>(__float_as_uint(top) >> 23) - 127;
+    return min(14 - e, 127);
+  }
+};
+
+// Joins the key ranges' (m, l, sum) of each row (attention_q8.hip). partial: [rows][splits][2 + dim].
+void LaunchAttendJoin(const float* partial, float* out, int64_t rows, int32_t splits, int32_t dim, hipStream_t stream);
+
+}  // namespace accel_hip

@@ -1,4 +1,4 @@
-// Attention over the 8-bit cache, and with a sliding window over an fp32 one: for the row at p,
+// Attention with a sliding window over an fp32 cache: for the row at p,
 // out = sum_t e^(s_t - max s) v_t / sum_t e^(s_t - max s) over the keys it sees, t <= p with
 // t > p - window or t < sinks, s_t = (q . k_t) / sqrt(dim), in one pass with a running maximum.
 //
@@ -18,15 +18,6 @@ struct F32Rows {
   __device__ __forceinline__ float VScale(int64_t, int32_t, int32_t) const { return 1.f; }
   __device__ __forceinline__ float K(int64_t at) const { return k[at]; }
   __device__ __forceinline__ float V(int64_t at) const { return v[at]; }
-};
-
-struct Q8Rows {
-  Q8Plane k, v;
-  int32_t shift;
-  __device__ __forceinline__ float KScale(int64_t t, int32_t kv_heads, int32_t h) const { return k.scale[(t >> shift) * kv_heads + h]; }
-  __device__ __forceinline__ float VScale(int64_t t, int32_t kv_heads, int32_t h) const { return v.scale[(t >> shift) * kv_heads + h]; }
-  __device__ __forceinline__ float K(int64_t at) const { return static_cast<float>(k.code[at]); }
-  __device__ __forceinline__ float V(int64_t at) const { return static_cast<float>(v.code[at]); }
 };
 
 template <typename Rows>
@@ -79,12 +70,6 @@ __global__ __launch_bounds__(64) void AttendSimpleKernel(AttendArgs a, Rows rows
 }
 
 }  // namespace
-
-void LaunchAttentionQ8(const AttendArgs& a, const Q8Cache& cache, hipStream_t stream) {
-  hipLaunchKernelGGL(AttendSimpleKernel<Q8Rows>, dim3(static_cast<uint32_t>(a.seq) * a.heads), dim3(64), 0, stream, a,
-                     Q8Rows{cache.k, cache.v, cache.block_shift});
-  Check(hipGetLastError(), "AttendSimpleKernel launch");
-}
 
 void LaunchAttentionWindow(const AttendArgs& a, const float* k, const float* v, hipStream_t stream) {
   hipLaunchKernelGGL(AttendSimpleKernel<F32Rows>, dim3(static_cast<uint32_t>(a.seq) * a.heads), dim3(64), 0, stream, a,
