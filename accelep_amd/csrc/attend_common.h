@@ -3,6 +3,8 @@
 // of key ranges.
 #pragma once
 
+#include <algorithm>
+
 #include "device_common.h"
 
 namespace accel_hip {
@@ -84,6 +86,30 @@ struct RowState {
   }
 };
 
+// 4 codes from dim d on, 0 past the row.
+template <int kLoad>
+__device__ __forceinline__ uint32_t LoadCodes4(const int8_t* p, int d, int dim) {
+  if (kLoad >= 4) return d < dim ? *reinterpret_cast<const uint32_t*>(p) : 0u;
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (d + e < dim) w |= static_cast<uint32_t>(static_cast<uint8_t>(p[e])) << (8 * e);
+  return w;
+}
+
+// The most steps of a block of `rows` rows' key range.
+inline int64_t AttendRangeSteps(const AttendArgs& a, int64_t rows, int64_t step) {
+  const int64_t group = a.heads / a.kv_heads;
+  const int64_t queries = std::min<int64_t>(a.seq, (rows + group - 2) / group + 1);
+  const int64_t end = int64_t(a.position) + a.seq;
+  if (a.window == kNoWindow) return (end + step - 1) / step;
+  const int64_t keys = std::min<int64_t>(end, int64_t(a.window) + queries + step);
+  return (keys + step - 1) / step + (std::min<int64_t>(a.sinks, end) + step - 1) / step;
+}
+
+// Many rows (attend_prompt.hip). load: the bytes that a thread may load at once from keys and values.
+void LaunchAttendPromptQ8(const AttendArgs& a, const Q8Cache& c, int load, hipStream_t stream);
+void LaunchAttendPromptF32(const AttendArgs& a, const float* k, const float* v, int load, hipStream_t stream);
 // Joins the key ranges' (m, l, sum) of each row (attention_q8.hip). partial: [rows][splits][2 + dim].
 void LaunchAttendJoin(const float* partial, float* out, int64_t rows, int32_t splits, int32_t dim, hipStream_t stream);
 

@@ -1,0 +1,473 @@
+// Attention of many rows (a prompt) over the 8-bit cache and in a window over an fp32 one, on the f16
+// matrix cores: queries, softmax weights and fp32 keys and values as two f16 parts (22 bits), codes as
+// one, scales and powers of two beside them in fp32.
+//
+// One workgroup per (128 rows of a key head, key range): four waves of 32 rows share each tile of keys,
+// which is brought to f16 once, through LDS, while the tile before is worked on (two buffers, one
+// barrier a tile). Lane (j, g) = (lane % 32, lane / 32) serves row j. Per 32 keys
+//  * S^T = K Q^T on v_mfma_f32_32x32x16_f16, keys as rows: the lane's 16 results are the scores of keys
+//    8a + 4g + b (a, b < 4) of row j, so a row's softmax needs one exchange between two lanes;
+//  * O^T += V^T P^T: those scores are the lane's own k-slots of P^T if slot e of 16 keys is key
+//    (e % 4) + 8 (e / 4) + 4g, and the value operand is read transposed from the row-major tile
+//    (ds_read_b64_tr_b16 gives a lane four keys of one dim).
+// An fp32 row enters as its parts times a power of two, that of its largest magnitude, which takes the
+// place of a block's scale; a row that is not finite gets a NaN in its place and zeros as values.
+#include "attend_common.h"
+
+namespace accel_hip {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kWaveRows = 32;
+constexpr int kRows = kWaves * kWaveRows;
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+struct PromptArgs {
+  const void* k;  // codes or floats
+  const void* v;
+  const float* k_scale;  // 8-bit only
+  const float* v_scale;
+  int32_t block_shift, splits, tiles;
+  float* partial;
+};
+
+// kF32: an fp32 cache. kLoad: bytes that may be loaded at once (16, 4 or 1; 16 or 4 for fp32).
+// kUniform: a block holds whole tiles, one scale each.
+template <int DP, bool kF32, int kLoad, bool kUniform>
+__global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel(AttendArgs a, PromptArgs b) {
+  constexpr int kParts = kF32 ? 2 : 1;
+  constexpr int kKeys = kF32 ? 32 : 64;
+  constexpr int kSub = kKeys / 32;
+  constexpr int kSteps = DP / 16;
+  constexpr int kDims = DP / 32;
+  constexpr int kKStride = DP + 8;   // halves: 8 key rows' 16-byte pieces fall into different banks
+  constexpr int kVStride = DP + 16;  // and so do 4 key rows' 32-byte pieces
+  constexpr int kChunks = kF32 ? DP / 32 : kKeys * DP / 16 / kThreads;  // 16-byte pieces of a plane a thread stages
+  __shared__ __align__(16) _Float16 kt[2][kParts][kKeys][kKStride];
+  __shared__ __align__(16) _Float16 vt[2][kParts][kKeys][kVStride];
+  __shared__ __align__(16) float sk[2][kKeys];
+  __shared__ __align__(16) float sv[2][kKeys];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & 31;
+  const int g = lane >> 5;
+  const int32_t kv = static_cast<int32_t>(blockIdx.x) % a.kv_heads;
+  const int32_t rest = static_cast<int32_t>(blockIdx.x) / a.kv_heads;
+  const int32_t split = rest % b.splits;
+  const int32_t tile = b.tiles - 1 - rest / b.splits;  // the rows with the most keys first
+  const int32_t group = a.heads / a.kv_heads;
+  const int32_t rows = a.seq * group;
+  const int32_t r0 = tile * kRows;
+  const KeyRange<kKeys> range(a, r0, min(r0 + kRows, rows), group);
+  const int32_t per = (range.steps + b.splits - 1) / b.splits;
+  const int32_t begin = min(range.steps, split * per);
+  const int32_t end = min(range.steps, begin + per);
+  const int32_t w0 = r0 + wave * kWaveRows;  // the wave's rows
+  const int32_t row = min(w0 + j, rows - 1);
+  const int32_t s = row / group;
+  const int32_t head = kv * group + (row - s * group);
+  const int32_t p_row = w0 + j < rows ? a.position + s : -1;
+  const int32_t pw_first = a.position + min(w0, rows - 1) / group;
+  const int32_t pw_last = w0 < rows ? a.position + (min(w0 + kWaveRows, rows) - 1) / group : -1;
+  const bool full_rows = w0 + kWaveRows <= rows;
+  const int64_t kv_row = static_cast<int64_t>(a.kv_heads) * a.dim;
+
+  // ---- staging: a thread's pieces of the next tile, from memory to registers and on to LDS ----
+  uint4 kreg[kChunks], vreg[kChunks];
+  float ks_next = 0.f, vs_next = 0.f;
+  const auto fetch_plane = [&](const void* base, int32_t t0, uint4 (&x)[kChunks]) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int key = kF32 ? tid / 8 : (tid + i * kThreads) / (DP / 16);
+      const int d = kF32 ? 4 * (tid % 8 + 8 * i) : 16 * ((tid + i * kThreads) % (DP / 16));
+      const int64_t at = min(t0 + key, range.high - 1) * kv_row + static_cast<int64_t>(kv) * a.dim + d;
+      uint32_t w[4] = {0, 0, 0, 0};
+      if (kF32) {
+        const float* p = static_cast<const float*>(base) + at;
+        if (kLoad == 16) {
+          if (d < a.dim) x[i] = *reinterpret_cast<const uint4*>(p);
+          else x[i] = make_uint4(0, 0, 0, 0);
+          continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < a.dim) w[e] = __float_as_uint(p[e]);
+      } else {
+        const int8_t* p = static_cast<const int8_t*>(base) + at;
+        if (kLoad == 16) {
+          if (d < a.dim) x[i] = *reinterpret_cast<const uint4*>(p);
+          else x[i] = make_uint4(0, 0, 0, 0);
+          continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = LoadCodes4<(kLoad < 16 ? kLoad : 4)>(p + 4 * e, d + 4 * e, a.dim);
+      }
+      x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  };
+  const auto scale_at = [&](const float* scale, int32_t t) {
+    return scale[static_cast<int64_t>(min(t, range.high - 1) >> b.block_shift) * a.kv_heads + kv];
+  };
+  const auto fetch = [&](int32_t t0) {
+    fetch_plane(b.k, t0, kreg);
+    fetch_plane(b.v, t0, vreg);
+    if (!kF32) {
+      const int32_t t = kUniform ? t0 : t0 + (tid & (kKeys - 1));
+      ks_next = scale_at(b.k_scale, t);
+      vs_next = scale_at(b.v_scale, t);
+    }
+  };
+  // Writes a thread's pieces of one plane; tile row `key` begins at dst + key * stride, its second part
+  // `part` halves later.
+  const auto put_plane = [&](const uint4 (&x)[kChunks], _Float16* dst, int stride, int part, float* scales) {
+    if (kF32) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i)
+        top = max(max(top, max(x[i].x & 0x7fffffffu, x[i].y & 0x7fffffffu)), max(x[i].z & 0x7fffffffu, x[i].w & 0x7fffffffu));
+      top = max(top, XorLane<1>(top));
+      top = max(top, XorLane<2>(top));
+      top = max(top, XorLane<4>(top));
+      const bool bad = top >= 0x7f800000u;
+      const float scale = bad ? 0.f : RowScale(top);
+      if (tid % 8 == 0) scales[tid / 8] = bad ? NAN : 1.f / scale;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const float f0 = bad ? 0.f : __uint_as_float(x[i].x) * scale, f1 = bad ? 0.f : __uint_as_float(x[i].y) * scale;
+        const float f2 = bad ? 0.f : __uint_as_float(x[i].z) * scale, f3 = bad ? 0.f : __uint_as_float(x[i].w) * scale;
+        h2 h0, l0, h1, l1;
+        SplitF16(f0, f1, h0, l0);
+        SplitF16(f2, f3, h1, l1);
+        _Float16* p = dst + (tid / 8) * stride + 4 * (tid % 8 + 8 * i);
+        *reinterpret_cast<h4*>(p) = h4{h0[0], h0[1], h1[0], h1[1]};
+        *reinterpret_cast<h4*>(p + part) = h4{l0[0], l0[1], l1[0], l1[1]};
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int key = (tid + i * kThreads) / (DP / 16);
+        const int d = 16 * ((tid + i * kThreads) % (DP / 16));
+        const uint32_t x0 = x[i].x ^ 0x80808080u, x1 = x[i].y ^ 0x80808080u, x2 = x[i].z ^ 0x80808080u, x3 = x[i].w ^ 0x80808080u;
+        h8* p = reinterpret_cast<h8*>(dst + key * stride + d);
+        p[0] = Join(CodesLow(x0), CodesHigh(x0), CodesLow(x1), CodesHigh(x1));
+        p[1] = Join(CodesLow(x2), CodesHigh(x2), CodesLow(x3), CodesHigh(x3));
+      }
+    }
+  };
+  const auto put = [&](int buf) {
+    put_plane(kreg, &kt[buf][0][0][0], kKStride, kKeys * kKStride, sk[buf]);
+    put_plane(vreg, &vt[buf][0][0][0], kVStride, kKeys * kVStride, sv[buf]);
+    if (!kF32 && !kUniform && tid < kKeys) {
+      sk[buf][tid] = ks_next;
+      sv[buf][tid] = vs_next;
+    }
+  };
+  if (begin < end) fetch(range.Key(begin));
+
+  // ---- the rows' queries ----
+  h8 qh[kSteps], ql[kSteps];
+  float row_factor;
+  {
+    const float* q = a.q + s * a.q_stride + static_cast<int64_t>(head) * a.dim;
+    uint32_t top = 0;
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = 16 * st + 8 * g + e;
+        if (d < a.dim) top = max(top, __float_as_uint(q[d]) & 0x7fffffffu);
+      }
+    top = max(top, XorLane<32>(top));
+    const bool bad = top >= 0x7f800000u;
+    const float scale = RowScale(top);
+    row_factor = kLog2e / scale * __fdiv_rn(1.f, __fsqrt_rn(static_cast<float>(a.dim)));
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      h2 hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 16 * st + 8 * g + 2 * e;
+        const float x0 = d < a.dim ? q[d] * scale : 0.f, x1 = d + 1 < a.dim ? q[d + 1] * scale : 0.f;
+        SplitF16(bad ? NAN : x0, bad ? NAN : x1, hi[e], lo[e]);
+      }
+      qh[st] = Join(hi[0], hi[1], hi[2], hi[3]);
+      ql[st] = Join(lo[0], lo[1], lo[2], lo[3]);
+    }
+  }
+
+  float m = -INFINITY, l = 0.f, top = 0.f;
+  int32_t power = 127;
+  f16v acc[kDims];
+#pragma unroll
+  for (int t = 0; t < kDims; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
+
+  float ks = ks_next, vs = vs_next;
+  if (begin < end) put(0);
+  for (int32_t u = begin; u < end; ++u) {
+    const int buf = (u - begin) & 1;
+    const int32_t t0 = range.Key(u);
+    __syncthreads();
+    if (u + 1 < end) fetch(range.Key(u + 1));
+    __builtin_amdgcn_sched_barrier(0);
+    const int32_t last = t0 + kKeys - 1;
+    const bool none = t0 > pw_last || (last <= pw_first - a.window && t0 >= a.sinks);
+    if (!none) {  // uniform over the wave
+      const bool whole = full_rows && last <= pw_first && (t0 > pw_last - a.window || last < a.sinks);
+      f16v st[kSub];
+#pragma unroll
+      for (int h = 0; h < kSub; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[h][r] = 0.f;
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+        for (int h = 0; h < kSub; ++h) {
+          const h8 k8 = *reinterpret_cast<const h8*>(&kt[buf][0][32 * h + j][16 * step + 8 * g]);
+          st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qh[step], st[h], 0, 0, 0);
+          st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[step], st[h], 0, 0, 0);
+          if (kF32) {
+            const h8 k8l = *reinterpret_cast<const h8*>(&kt[buf][kParts - 1][32 * h + j][16 * step + 8 * g]);
+            st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8l, qh[step], st[h], 0, 0, 0);
+          }
+        }
+      float c = row_factor;
+      if (kUniform) {
+        c *= ks;
+      } else {
+#pragma unroll
+        for (int h = 0; h < kSub; ++h)
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const f4 f = *reinterpret_cast<const f4*>(&sk[buf][32 * h + 8 * r4 + 4 * g]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st[h][4 * r4 + e] *= f[e];
+          }
+      }
+      uint32_t seen[kSub];
+      if (!whole) {
+#pragma unroll
+        for (int h = 0; h < kSub; ++h) {
+          seen[h] = 0;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const bool in = Sees(a, p_row, t0 + 32 * h + (r & 3) + 8 * (r >> 2) + 4 * g);
+            seen[h] |= in ? 1u << r : 0u;
+            st[h][r] = in ? st[h][r] * c : -INFINITY;
+          }
+        }
+        c = 1.f;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < kSub; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[h][r]);
+      mx = fmaxf(mx, XorLane<32>(mx)) * c;
+      // The reference moves only when a score passes it by 2^8, so the sums are seldom scaled.
+      const float m_old = m;
+      if (mx > m + 8.f) m = mx;
+      const float base = m == -INFINITY ? 0.f : m;
+      const float corr = __builtin_amdgcn_exp2f(m_old - base);
+      float sum = 0.f;
+#pragma unroll
+      for (int h = 0; h < kSub; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          st[h][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[h][r], c, -base));
+          sum += st[h][r];
+        }
+      l = l * corr + sum;
+      // The weights times the values' scales, and their largest.
+      float tile_top = 0.f;
+      if (kUniform) {
+        tile_top = __builtin_amdgcn_exp2f(mx - base) * vs;
+      } else {
+#pragma unroll
+        for (int h = 0; h < kSub; ++h)
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const f4 f = *reinterpret_cast<const f4*>(&sv[buf][32 * h + 8 * r4 + 4 * g]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float x = st[h][4 * r4 + e] * f[e];
+              if (!whole) x = seen[h] >> (4 * r4 + e) & 1 ? x : 0.f;
+              st[h][4 * r4 + e] = x;
+              tile_top = fmaxf(tile_top, fabsf(x));
+            }
+          }
+        tile_top = fmaxf(tile_top, XorLane<32>(tile_top));
+      }
+      top = fmaxf(top * corr, tile_top);
+      const int32_t power_old = power;
+      const float at = ldexpf(top, power);
+      if (at >= 0x1p15f || (at < 8.f && top > 0.f)) {
+        const int32_t e = static_cast<int32_t>(__float_as_uint(top) >> 23) - 127;
+        power = min(6 - e, 127);
+      }
+      const float again = ldexpf(corr, power - power_old);
+      if (__any(again != 1.f)) {
+#pragma unroll
+        for (int t = 0; t < kDims; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[t][r] *= again;
+      }
+      if (kUniform) {
+        const float f = ldexpf(vs, power);
+        if (__any(!(f < 0x1p100f))) {  // a block that is far larger than the sum so far: in two steps
+#pragma unroll
+          for (int h = 0; h < kSub; ++h)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[h][r] = ldexpf(st[h][r] * vs, power);
+        } else {
+#pragma unroll
+          for (int h = 0; h < kSub; ++h)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[h][r] *= f;
+        }
+        if (!whole) {
+#pragma unroll
+          for (int h = 0; h < kSub; ++h)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[h][r] = seen[h] >> r & 1 ? st[h][r] : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < kSub; ++h)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) st[h][r] = ldexpf(st[h][r], power);
+      }
+      // O^T += V^T P^T, 16 keys at a time.
+      const _Float16* vrow = &vt[buf][0][4 * g + ((lane & 15) >> 2)][16 * ((lane >> 4) & 1) + 4 * (lane & 3)];
+#pragma unroll
+      for (int h = 0; h < kSub; ++h)
+#pragma unroll
+        for (int k16 = 0; k16 < 2; ++k16) {
+          h2 hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) SplitF16(st[h][8 * k16 + 2 * e], st[h][8 * k16 + 2 * e + 1], hi[e], lo[e]);
+          const h8 ph = Join(hi[0], hi[1], hi[2], hi[3]), pl = Join(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+          for (int t = 0; t < kDims; ++t) {
+            const auto read = [&](int part) {
+              const _Float16* p = vrow + part * kKeys * kVStride + (32 * h + 16 * k16) * kVStride + 32 * t;
+              const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
+              const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p + 8 * kVStride));
+              return __builtin_bit_cast(h8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            const h8 v8 = read(0);
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph, acc[t], 0, 0, 0);
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl, acc[t], 0, 0, 0);
+            if (kF32) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read(kParts - 1), ph, acc[t], 0, 0, 0);
+          }
+        }
+    }
+    if (u + 1 < end) {
+      put(buf ^ 1);
+      ks = ks_next;
+      vs = vs_next;
+    }
+  }
+
+  // acc[t][r] is O^T[dim 32t + 8 (r / 4) + 4g + r % 4][row j].
+  l = l + XorLane<32>(l);
+  if (w0 + j >= rows) return;
+  const int64_t out_row = static_cast<int64_t>(s) * a.heads + head;
+  float* dst = a.out + out_row * a.dim;
+  float by = 1.f;
+  if (b.splits > 1) {
+    dst = b.partial + (out_row * b.splits + split) * (2 + a.dim);
+    if (g == 0) {
+      dst[0] = m;
+      dst[1] = l;
+    }
+    dst += 2;
+  } else {
+    by = l;
+  }
+  const bool vec = b.splits == 1 && a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+#pragma unroll
+  for (int t = 0; t < kDims; ++t)
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const int d = 32 * t + 8 * r4 + 4 * g;
+      float o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[e] = ldexpf(acc[t][4 * r4 + e], -power);
+        if (b.splits == 1) o[e] = __fdiv_rn(o[e], by);
+      }
+      if (vec) {
+        if (d < a.dim) *reinterpret_cast<float4*>(dst + d) = make_float4(o[0], o[1], o[2], o[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < a.dim) dst[d + e] = o[e];
+      }
+    }
+}
+
+template <int DP, bool kF32>
+void LaunchPrompt(const AttendArgs& a, const PromptArgs& b, int load, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(int64_t(a.kv_heads) * b.splits * b.tiles)), block(kThreads);
+#define ACCEL_PROMPT(L, U) hipLaunchKernelGGL((AttendPromptKernel<DP, kF32, L, U>), grid, block, 0, stream, a, b)
+  if constexpr (kF32) {
+    if (load == 16) ACCEL_PROMPT(16, false);
+    else ACCEL_PROMPT(4, false);
+  } else if (load == 16 && b.block_shift >= 6) {
+    ACCEL_PROMPT(16, true);
+  } else if (load == 16) {
+    ACCEL_PROMPT(16, false);
+  } else if (load == 4) {
+    ACCEL_PROMPT(4, false);
+  } else {
+    ACCEL_PROMPT(1, false);
+  }
+#undef ACCEL_PROMPT
+  Check(hipGetLastError(), "AttendPromptKernel launch");
+}
+
+template <bool kF32>
+void LaunchPromptOf(const AttendArgs& a, PromptArgs b, int load, hipStream_t stream) {
+  const int64_t group = a.heads / a.kv_heads;
+  const int64_t tiles = (int64_t(a.seq) * group + kRows - 1) / kRows;
+  const int64_t units = tiles * a.kv_heads;
+  const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
+  if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
+  const int64_t steps = AttendRangeSteps(a, kRows, kF32 ? 32 : 64);
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(2 * cus / units, steps / 4));
+  const int64_t rows = int64_t(a.seq) * a.heads;
+  const size_t bytes = static_cast<size_t>(rows * splits * (2 + a.dim)) * sizeof(float);
+  if (splits > 1 && !ScratchReady(bytes, kTempFlags, 0)) splits = 1;
+  b.splits = static_cast<int32_t>(splits);
+  b.tiles = static_cast<int32_t>(tiles);
+  b.partial = splits > 1 ? static_cast<float*>(Workspace(bytes)) : nullptr;
+  if (a.dim <= 64) LaunchPrompt<64, kF32>(a, b, load, stream);
+  else if (a.dim <= 128) LaunchPrompt<128, kF32>(a, b, load, stream);
+  else LaunchPrompt<256, kF32>(a, b, load, stream);
+  if (splits > 1) LaunchAttendJoin(b.partial, a.out, rows, b.splits, a.dim, stream);
+}
+
+}  // namespace
+
+void LaunchAttendPromptQ8(const AttendArgs& a, const Q8Cache& c, int load, hipStream_t stream) {
+  PromptArgs b{};
+  b.k = c.k.code;
+  b.v = c.v.code;
+  b.k_scale = c.k.scale;
+  b.v_scale = c.v.scale;
+  b.block_shift = c.block_shift;
+  LaunchPromptOf<false>(a, b, load, stream);
+}
+
+void LaunchAttendPromptF32(const AttendArgs& a, const float* k, const float* v, int load, hipStream_t stream) {
+  PromptArgs b{};
+  b.k = k;
+  b.v = v;
+  LaunchPromptOf<true>(a, b, load, stream);
+}
+
+}  // namespace accel_hip

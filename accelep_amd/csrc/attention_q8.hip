@@ -4,8 +4,6 @@
 // of the blocks multiply scores and weights.
 //
 // Few rows (a decode step, drafted tokens): AttendQ8StepKernel below.
-#include <algorithm>
-
 #include "attend_common.h"
 
 namespace accel_hip {
@@ -15,16 +13,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kStepRows = 16;
 constexpr int kStepKeys = 32;
-
-template <int kLoad>
-__device__ __forceinline__ uint32_t LoadCodes4(const int8_t* p, int d, int dim) {  // 4 codes from dim d on, 0 past the row
-  if (kLoad >= 4) return d < dim ? *reinterpret_cast<const uint32_t*>(p) : 0u;
-  uint32_t w = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (d + e < dim) w |= static_cast<uint32_t>(static_cast<uint8_t>(p[e])) << (8 * e);
-  return w;
-}
+constexpr int64_t kPromptRows = 64;  // rows of a key head from which on the tiles go through LDS
 
 // One workgroup per (16 rows of a key head, key range); its waves take every fourth step of 32 keys.
 // Bound: the cache's bytes. Keys and values go from memory to registers, and there to f16: no LDS and
@@ -358,15 +347,6 @@ void LaunchAttendJoin(const float* partial, float* out, int64_t rows, int32_t sp
 
 namespace {
 
-// The most keys that some row of a block of `rows` sees, and with it the steps of its range.
-int64_t RangeSteps(const AttendArgs& a, int64_t rows, int64_t group, int64_t step) {
-  const int64_t queries = std::min<int64_t>(a.seq, (rows + group - 2) / group + 1);
-  const int64_t end = int64_t(a.position) + a.seq;
-  if (a.window == kNoWindow) return (end + step - 1) / step;
-  const int64_t keys = std::min<int64_t>(end, int64_t(a.window) + queries + step);
-  return (keys + step - 1) / step + (std::min<int64_t>(a.sinks, end) + step - 1) / step;
-}
-
 template <int DP>
 void LaunchStep(const AttendArgs& a, const Q8Cache& c, int load, int32_t splits, int32_t tiles, float* partial,
                 hipStream_t stream) {
@@ -394,9 +374,13 @@ void LaunchAttentionQ8(const AttendArgs& a, const Q8Cache& c, hipStream_t stream
   };
   const int load = aligned(16) ? 16 : aligned(4) ? 4 : 1;
   const int64_t group = a.heads / a.kv_heads;
+  if (int64_t(a.seq) * group > kPromptRows) {
+    LaunchAttendPromptQ8(a, c, load, stream);
+    return;
+  }
   const int64_t tiles = (int64_t(a.seq) * group + kStepRows - 1) / kStepRows;
   const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
-  const int64_t steps = RangeSteps(a, kStepRows, group, kStepKeys);
+  const int64_t steps = AttendRangeSteps(a, kStepRows, kStepKeys);
   const int64_t units = tiles * a.kv_heads;
   if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
   int64_t splits = std::max<int64_t>(1, std::min<int64_t>(2 * cus / units, steps / kWaves));

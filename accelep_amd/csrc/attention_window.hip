@@ -4,7 +4,7 @@
 //
 // The simplest form: one wave per (row, head), 64 keys at a time, a key a lane for the scores, then
 // dims over the lanes for the weighted sum.
-#include "device_common.h"
+#include "attend_common.h"
 
 namespace accel_hip {
 namespace {
@@ -72,6 +72,11 @@ __global__ __launch_bounds__(64) void AttendSimpleKernel(AttendArgs a, Rows rows
 }  // namespace
 
 void LaunchAttentionWindow(const AttendArgs& a, const float* k, const float* v, hipStream_t stream) {
+  if (int64_t(a.seq) * (a.heads / a.kv_heads) > 64) {
+    const bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0;
+    LaunchAttendPromptF32(a, k, v, vec ? 16 : 4, stream);
+    return;
+  }
   hipLaunchKernelGGL(AttendSimpleKernel<F32Rows>, dim3(static_cast<uint32_t>(a.seq) * a.heads), dim3(64), 0, stream, a,
                      F32Rows{k, v});
   Check(hipGetLastError(), "AttendSimpleKernel launch");
