@@ -107,6 +107,16 @@ inline int64_t AttendRangeSteps(const AttendArgs& a, int64_t rows, int64_t step)
   return (keys + step - 1) / step + (std::min<int64_t>(a.sinks, end) + step - 1) / step;
 }
 
+// Into how many key ranges `units` workgroups' worth of rows are cut, at most `most`: up to two
+// workgroups per CU. Where the partial sums have no room the range stays whole.
+struct AttendSplit {
+  int32_t count = 1;
+  float* partial = nullptr;
+};
+AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t most);
+
+// Rows of a key head above which the tiles of keys go through LDS.
+constexpr int64_t kAttendPromptRows = 64;
 // Many rows (attend_prompt.hip). load: the bytes that a thread may load at once from keys and values.
 void LaunchAttendPromptQ8(const AttendArgs& a, const Q8Cache& c, int load, hipStream_t stream);
 void LaunchAttendPromptF32(const AttendArgs& a, const float* k, const float* v, int load, hipStream_t stream);

@@ -435,20 +435,15 @@ void LaunchPromptOf(const AttendArgs& a, PromptArgs b, int load, hipStream_t str
   const int64_t group = a.heads / a.kv_heads;
   const int64_t tiles = (int64_t(a.seq) * group + kRows - 1) / kRows;
   const int64_t units = tiles * a.kv_heads;
-  const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
   if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
-  const int64_t steps = AttendRangeSteps(a, kRows, kF32 ? 32 : 64);
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(2 * cus / units, steps / 4));
-  const int64_t rows = int64_t(a.seq) * a.heads;
-  const size_t bytes = static_cast<size_t>(rows * splits * (2 + a.dim)) * sizeof(float);
-  if (splits > 1 && !ScratchReady(bytes, kTempFlags, 0)) splits = 1;
-  b.splits = static_cast<int32_t>(splits);
+  const AttendSplit split = SplitRange(a, units, AttendRangeSteps(a, kRows, kF32 ? 32 : 64) / 4);
+  b.splits = split.count;
   b.tiles = static_cast<int32_t>(tiles);
-  b.partial = splits > 1 ? static_cast<float*>(Workspace(bytes)) : nullptr;
+  b.partial = split.partial;
   if (a.dim <= 64) LaunchPrompt<64, kF32>(a, b, load, stream);
   else if (a.dim <= 128) LaunchPrompt<128, kF32>(a, b, load, stream);
   else LaunchPrompt<256, kF32>(a, b, load, stream);
-  if (splits > 1) LaunchAttendJoin(b.partial, a.out, rows, b.splits, a.dim, stream);
+  if (b.splits > 1) LaunchAttendJoin(b.partial, a.out, int64_t(a.seq) * a.heads, b.splits, a.dim, stream);
 }
 
 }  // namespace

@@ -13,7 +13,6 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kStepRows = 16;
 constexpr int kStepKeys = 32;
-constexpr int64_t kPromptRows = 64;  // rows of a key head from which on the tiles go through LDS
 
 // One workgroup per (16 rows of a key head, key range); its waves take every fourth step of 32 keys.
 // Bound: the cache's bytes. Keys and values go from memory to registers, and there to f16: no LDS and
@@ -345,6 +344,17 @@ void LaunchAttendJoin(const float* partial, float* out, int64_t rows, int32_t sp
   Check(hipGetLastError(), "AttendJoinKernel launch");
 }
 
+AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t most) {
+  const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
+  const int64_t count = std::max<int64_t>(1, std::min<int64_t>(2 * cus / units, most));
+  const size_t bytes = static_cast<size_t>(int64_t(a.seq) * a.heads * count * (2 + a.dim)) * sizeof(float);
+  AttendSplit split;
+  if (count == 1 || !ScratchReady(bytes, kTempFlags, 0)) return split;
+  split.count = static_cast<int32_t>(count);
+  split.partial = static_cast<float*>(Workspace(bytes));
+  return split;
+}
+
 namespace {
 
 template <int DP>
@@ -374,24 +384,18 @@ void LaunchAttentionQ8(const AttendArgs& a, const Q8Cache& c, hipStream_t stream
   };
   const int load = aligned(16) ? 16 : aligned(4) ? 4 : 1;
   const int64_t group = a.heads / a.kv_heads;
-  if (int64_t(a.seq) * group > kPromptRows) {
+  if (int64_t(a.seq) * group > kAttendPromptRows) {
     LaunchAttendPromptQ8(a, c, load, stream);
     return;
   }
   const int64_t tiles = (int64_t(a.seq) * group + kStepRows - 1) / kStepRows;
-  const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
-  const int64_t steps = AttendRangeSteps(a, kStepRows, kStepKeys);
   const int64_t units = tiles * a.kv_heads;
   if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(2 * cus / units, steps / kWaves));
-  const int64_t rows = int64_t(a.seq) * a.heads;
-  const size_t bytes = static_cast<size_t>(rows * splits * (2 + a.dim)) * sizeof(float);
-  if (splits > 1 && !ScratchReady(bytes, kTempFlags, 0)) splits = 1;
-  float* partial = splits > 1 ? static_cast<float*>(Workspace(bytes)) : nullptr;
-  if (a.dim <= 64) LaunchStep<64>(a, c, load, static_cast<int32_t>(splits), static_cast<int32_t>(tiles), partial, stream);
-  else if (a.dim <= 128) LaunchStep<128>(a, c, load, static_cast<int32_t>(splits), static_cast<int32_t>(tiles), partial, stream);
-  else LaunchStep<256>(a, c, load, static_cast<int32_t>(splits), static_cast<int32_t>(tiles), partial, stream);
-  if (splits > 1) LaunchAttendJoin(partial, a.out, rows, static_cast<int32_t>(splits), a.dim, stream);
+  const AttendSplit split = SplitRange(a, units, AttendRangeSteps(a, kStepRows, kStepKeys) / kWaves);
+  if (a.dim <= 64) LaunchStep<64>(a, c, load, split.count, static_cast<int32_t>(tiles), split.partial, stream);
+  else if (a.dim <= 128) LaunchStep<128>(a, c, load, split.count, static_cast<int32_t>(tiles), split.partial, stream);
+  else LaunchStep<256>(a, c, load, split.count, static_cast<int32_t>(tiles), split.partial, stream);
+  if (split.count > 1) LaunchAttendJoin(split.partial, a.out, int64_t(a.seq) * a.heads, split.count, a.dim, stream);
 }
 
 }  // namespace accel_hip

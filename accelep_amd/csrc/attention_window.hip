@@ -1,85 +1,245 @@
-// Attention with a sliding window over an fp32 cache: for the row at p,
-// out = sum_t e^(s_t - max s) v_t / sum_t e^(s_t - max s) over the keys it sees, t <= p with
-// t > p - window or t < sinks, s_t = (q . k_t) / sqrt(dim), in one pass with a running maximum.
+// Attention with a sliding window over an fp32 cache: the row at p sees the keys t <= p with
+// t > p - window or t < sinks, and reads no others.
 //
-// The simplest form: one wave per (row, head), 64 keys at a time, a key a lane for the scores, then
-// dims over the lanes for the weighted sum.
+// Few rows (a decode step, drafted tokens): AttendF32StepKernel below. Many: attend_prompt.hip.
 #include "attend_common.h"
 
 namespace accel_hip {
 namespace {
 
-constexpr int kMaxDim = 256;
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kRows = 16;
+constexpr int kKeys = 16;  // of a wave's step
 
-struct F32Rows {
-  const float* k;
-  const float* v;
-  __device__ __forceinline__ float KScale(int64_t, int32_t, int32_t) const { return 1.f; }
-  __device__ __forceinline__ float VScale(int64_t, int32_t, int32_t) const { return 1.f; }
-  __device__ __forceinline__ float K(int64_t at) const { return k[at]; }
-  __device__ __forceinline__ float V(int64_t at) const { return v[at]; }
-};
+// One workgroup per (16 rows of a key head, key range); its waves take every fourth step of 16 keys.
+// Bound: the bytes of the keys that are seen. Both products run on v_mfma_f32_16x16x4f32, which takes
+// fp32 as it is, with every operand straight from memory. Lane (j, g) = (lane % 16, lane / 16):
+//  * S^T = K Q^T: k slot g of instruction (i, e) is dim 16i + 4g + e, so a lane loads 16 bytes of key
+//    row j at a time and a key row's pieces lie side by side;
+//  * O^T += V^T P^T: S^T leaves the lane the scores of keys 4g .. 4g + 3 of row j; k slot g of
+//    instruction s is key 4g + s, the A operand of dim tile (c, t) float t of the 16 bytes at
+//    V[key][64c + 4j].
+// A key or value row that is not finite would reach rows that do not see it, as 0 * NaN: a step that
+// holds one (a test of the bits, uniform) has its values taken as zeros and its weights as NaN.
+template <int DP, int kLoad>
+__global__ __launch_bounds__(kThreads) void AttendF32StepKernel(AttendArgs a, const float* k, const float* v,
+                                                                int32_t splits, float* partial) {
+  constexpr int kI = DP / 16;  // 16-byte pieces of a key row per lane
+  constexpr int kC = DP / 64;  // of a value row
+  __shared__ __align__(16) float part_o[kWaves][kRows][DP + 4];
+  __shared__ float part_m[kWaves][kRows];
+  __shared__ float part_l[kWaves][kRows];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & 15;
+  const int g = lane >> 4;
+  const int32_t kv = static_cast<int32_t>(blockIdx.x) % a.kv_heads;
+  const int32_t rest = static_cast<int32_t>(blockIdx.x) / a.kv_heads;
+  const int32_t split = rest % splits;
+  const int32_t group = a.heads / a.kv_heads;
+  const int32_t rows = a.seq * group;
+  const int32_t r0 = rest / splits * kRows;
+  const KeyRange<kKeys> range(a, r0, min(r0 + kRows, rows), group);
+  const int32_t per = (range.steps + splits - 1) / splits;
+  const int32_t begin = min(range.steps, split * per);
+  const int32_t end = min(range.steps, begin + per);
+  const int32_t row = min(r0 + j, rows - 1);
+  const int32_t s = row / group;
+  const int32_t head = kv * group + (row - s * group);
+  const int32_t p_row = r0 + j < rows ? a.position + s : -1;  // a row past the last sees nothing
+  const int64_t kv_row = static_cast<int64_t>(a.kv_heads) * a.dim;
+  const float* kbase = k + static_cast<int64_t>(kv) * a.dim;
+  const float* vbase = v + static_cast<int64_t>(kv) * a.dim;
 
-template <typename Rows>
-__global__ __launch_bounds__(64) void AttendSimpleKernel(AttendArgs a, Rows rows) {
-  __shared__ float qs[kMaxDim];
-  __shared__ float es[64];
-  const int lane = threadIdx.x;
-  const int32_t s = static_cast<int32_t>(blockIdx.x / static_cast<uint32_t>(a.heads));
-  const int32_t h = static_cast<int32_t>(blockIdx.x) - s * a.heads;
-  const int32_t kv = h / (a.heads / a.kv_heads);
-  const int32_t p = a.position + s;
-  const float* q = a.q + s * a.q_stride + static_cast<int64_t>(h) * a.dim;
-  for (int d = lane; d < a.dim; d += 64) qs[d] = q[d];
-  const float scale = __fdiv_rn(1.f, __fsqrt_rn(static_cast<float>(a.dim)));
-  const int64_t stride = static_cast<int64_t>(a.kv_heads) * a.dim;
-  const int32_t low = a.window == kNoWindow ? 0 : max(0, p - a.window + 1);
-  const int32_t first = min(low, a.sinks);
+  f4 kx[kI], vx[4][kC];
+  const auto piece = [&](const float* p, int d) {
+    if (kLoad == 16) return d < a.dim ? *reinterpret_cast<const f4*>(p + d) : f4{0.f, 0.f, 0.f, 0.f};
+    f4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = d + e < a.dim ? p[d + e] : 0.f;
+    return x;
+  };
+  const auto load_k = [&](int32_t t0) {
+    const float* p = kbase + min(t0 + j, range.high - 1) * kv_row;
+#pragma unroll
+    for (int i = 0; i < kI; ++i) kx[i] = piece(p, 16 * i + 4 * g);
+  };
+  const auto load_v = [&](int32_t t0) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float* p = vbase + min(t0 + 4 * g + e, range.high - 1) * kv_row;
+#pragma unroll
+      for (int c = 0; c < kC; ++c) vx[e][c] = piece(p, 64 * c + 4 * j);
+    }
+  };
+  int32_t u = begin + wave;
+  if (u < end) {
+    const int32_t t0 = range.Key(u);
+    load_k(t0);
+    load_v(t0);
+  }
+  f4 q[kI];
+  {
+    const float* p = a.q + s * a.q_stride + static_cast<int64_t>(head) * a.dim;
+#pragma unroll
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[i][e] = 16 * i + 4 * g + e < a.dim ? p[16 * i + 4 * g + e] : 0.f;
+  }
+  const float factor = kLog2e * __fdiv_rn(1.f, __fsqrt_rn(static_cast<float>(a.dim)));
+
+  float m = -INFINITY, l = 0.f;  // l: this lane's share of the row's sum
+  f4 acc[kC][4];
+#pragma unroll
+  for (int c = 0; c < kC; ++c)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[c][t] = f4{0.f, 0.f, 0.f, 0.f};
+  for (; u < end; u += kWaves) {  // uniform over the wave
+    const int32_t t0 = range.Key(u);
+    const int32_t next = u + kWaves < end ? range.Key(u + kWaves) : -1;
+    f4 st0 = f4{0.f, 0.f, 0.f, 0.f}, st1 = st0;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        st0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[i][e], q[i][e], st0, 0, 0, 0);
+        st1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[i][e + 1], q[i][e + 1], st1, 0, 0, 0);
+        top = max(top, max(FloatBits(kx[i][e]) & 0x7fffffffu, FloatBits(kx[i][e + 1]) & 0x7fffffffu));
+      }
+    const uint64_t bad_keys = __ballot(top >= 0x7f800000u);
+    if (next >= 0) load_k(next);
+    __builtin_amdgcn_sched_barrier(0);
+    uint32_t vtop[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      vtop[e] = 0;
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) vtop[e] = max(vtop[e], FloatBits(vx[e][c][t]) & 0x7fffffffu);
+    }
+    uint32_t bad = 0;  // of the lane's keys 4g + e
+    if (__any(max(max(vtop[0], vtop[1]), max(vtop[2], vtop[3])) >= 0x7f800000u) || bad_keys != 0) {
+      const uint32_t keys16 = static_cast<uint32_t>(bad_keys | bad_keys >> 16 | bad_keys >> 32 | bad_keys >> 48) & 0xffffu;
+      bad = keys16 >> (4 * g) & 15u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint64_t lanes = __ballot(vtop[e] >= 0x7f800000u);
+        if ((lanes >> (16 * g) & 0xffffu) != 0) {
+          bad |= 1u << e;
+#pragma unroll
+          for (int c = 0; c < kC; ++c) vx[e][c] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+      }
+    }
+    float p[4];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool in = Sees(a, p_row, t0 + 4 * g + e);
+      p[e] = in ? (bad >> e & 1 ? NAN : (st0[e] + st1[e]) * factor) : -INFINITY;
+      mx = fmaxf(mx, p[e]);
+    }
+    mx = fmaxf(mx, XorLane<16>(mx));
+    mx = fmaxf(mx, XorLane<32>(mx));
+    const float m_new = fmaxf(m, mx);
+    const float base = m_new == -INFINITY ? 0.f : m_new;
+    const float corr = __builtin_amdgcn_exp2f(m - base);
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      p[e] = __builtin_amdgcn_exp2f(p[e] - base);
+      sum += p[e];
+    }
+    l = l * corr + sum;
+    m = m_new;
+    if (__any(corr != 1.f)) {
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[c][t] *= corr;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          acc[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[e][c][t], p[e], acc[c][t], 0, 0, 0);
+    if (next >= 0) load_v(next);
+  }
+  // acc[c][t][r] is O^T[dim 64c + 16g + 4r + t][row j]; the waves' parts meet in LDS.
+  l = l + XorLane<16>(l);
+  l = l + XorLane<32>(l);
+  if (g == 0) {
+    part_m[wave][j] = m;
+    part_l[wave][j] = l;
+  }
+#pragma unroll
+  for (int c = 0; c < kC; ++c)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<f4*>(&part_o[wave][j][64 * c + 16 * g + 4 * r]) =
+          f4{acc[c][0][r], acc[c][1][r], acc[c][2][r], acc[c][3][r]};
   __syncthreads();
-  float m = -INFINITY, l = 0.f, acc[kMaxDim / 64] = {0.f, 0.f, 0.f, 0.f};
-  for (int part = 0; part < 2; ++part) {
-    const int32_t begin = part == 0 ? 0 : low, end = part == 0 ? first : p + 1;
-    for (int32_t t0 = begin; t0 < end; t0 += 64) {
-      const int32_t n = min(64, end - t0);
-      const int64_t t = t0 + lane;
-      float x = -INFINITY;
-      if (lane < n) {
-        float dot = 0.f;
-        for (int d = 0; d < a.dim; ++d) dot += qs[d] * rows.K(t * stride + kv * a.dim + d);
-        x = dot * (scale * rows.KScale(t, a.kv_heads, kv));
+  for (int item = tid; item < kRows * DP; item += kThreads) {
+    const int rl = item / DP;
+    const int d = item % DP;
+    if (r0 + rl >= rows || d >= a.dim) continue;
+    float big = part_m[0][rl];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) big = fmaxf(big, part_m[w][rl]);
+    const float base = big == -INFINITY ? 0.f : big;
+    float total = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float wt = __builtin_amdgcn_exp2f(part_m[w][rl] - base);
+      total += wt * part_l[w][rl];
+      o += wt * part_o[w][rl][d];
+    }
+    const int32_t sr = (r0 + rl) / group;
+    const int64_t out_row = static_cast<int64_t>(sr) * a.heads + kv * group + (r0 + rl - sr * group);
+    if (splits > 1) {
+      float* dst = partial + (out_row * splits + split) * (2 + a.dim);
+      if (d == 0) {
+        dst[0] = big;
+        dst[1] = total;
       }
-      const float m_new = fmaxf(m, WaveButterfly(x, [](float u, float w) { return fmaxf(u, w); }));
-      const float corr = m == m_new ? 1.f : expf(m - m_new);
-      const float e = lane < n ? expf(x - m_new) : 0.f;
-      l = l * corr + WaveButterfly(e, [](float u, float w) { return u + w; });
-      m = m_new;
-      es[lane] = lane < n ? e * rows.VScale(t, a.kv_heads, kv) : 0.f;
-      __syncthreads();
-      for (int i = 0; i < kMaxDim / 64; ++i) {
-        const int d = lane + 64 * i;
-        acc[i] *= corr;
-        if (d < a.dim)
-          for (int j = 0; j < n; ++j) acc[i] += es[j] * rows.V((t0 + j) * stride + kv * a.dim + d);
-      }
-      __syncthreads();
+      dst[2 + d] = o;
+    } else {
+      a.out[out_row * a.dim + d] = __fdiv_rn(o, total);
     }
   }
-  for (int i = 0; i < kMaxDim / 64; ++i)
-    if (lane + 64 * i < a.dim)
-      a.out[(static_cast<int64_t>(s) * a.heads + h) * a.dim + lane + 64 * i] = __fdiv_rn(acc[i], l);
+}
+
+template <int DP>
+void LaunchStep(const AttendArgs& a, const float* k, const float* v, bool vec, int32_t splits, int64_t units,
+                float* partial, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(units * splits)), block(kThreads);
+  if (vec) hipLaunchKernelGGL((AttendF32StepKernel<DP, 16>), grid, block, 0, stream, a, k, v, splits, partial);
+  else hipLaunchKernelGGL((AttendF32StepKernel<DP, 4>), grid, block, 0, stream, a, k, v, splits, partial);
+  Check(hipGetLastError(), "AttendF32StepKernel launch");
 }
 
 }  // namespace
 
 void LaunchAttentionWindow(const AttendArgs& a, const float* k, const float* v, hipStream_t stream) {
-  if (int64_t(a.seq) * (a.heads / a.kv_heads) > 64) {
-    const bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0;
+  const bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0;
+  const int64_t group = a.heads / a.kv_heads;
+  if (int64_t(a.seq) * group > kAttendPromptRows) {
     LaunchAttendPromptF32(a, k, v, vec ? 16 : 4, stream);
     return;
   }
-  hipLaunchKernelGGL(AttendSimpleKernel<F32Rows>, dim3(static_cast<uint32_t>(a.seq) * a.heads), dim3(64), 0, stream, a,
-                     F32Rows{k, v});
-  Check(hipGetLastError(), "AttendSimpleKernel launch");
+  const int64_t units = (int64_t(a.seq) * group + kRows - 1) / kRows * a.kv_heads;
+  if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
+  const AttendSplit split = SplitRange(a, units, AttendRangeSteps(a, kRows, kKeys) / kWaves);
+  if (a.dim <= 64) LaunchStep<64>(a, k, v, vec, split.count, units, split.partial, stream);
+  else if (a.dim <= 128) LaunchStep<128>(a, k, v, vec, split.count, units, split.partial, stream);
+  else LaunchStep<256>(a, k, v, vec, split.count, units, split.partial, stream);
+  if (split.count > 1) LaunchAttendJoin(split.partial, a.out, int64_t(a.seq) * a.heads, split.count, a.dim, stream);
 }
 
 }  // namespace accel_hip
