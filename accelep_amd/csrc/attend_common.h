@@ -107,20 +107,98 @@ inline int64_t AttendRangeSteps(const AttendArgs& a, int64_t rows, int64_t step)
   return (keys + step - 1) / step + (std::min<int64_t>(a.sinks, end) + step - 1) / step;
 }
 
-// Into how many key ranges `units` workgroups' worth of rows are cut, at most `most`: up to two
-// workgroups per CU. Where the partial sums have no room the range stays whole.
-struct AttendSplit {
-  int32_t count = 1;
-  float* partial = nullptr;
-};
-AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t most);
-
 // Rows of a key head above which the tiles of keys go through LDS.
 constexpr int64_t kAttendPromptRows = 64;
 // Many rows (attend_prompt.hip). load: the bytes that a thread may load at once from keys and values.
 void LaunchAttendPromptQ8(const AttendArgs& a, const Q8Cache& c, int load, hipStream_t stream);
 void LaunchAttendPromptF32(const AttendArgs& a, const float* k, const float* v, int load, hipStream_t stream);
-// Joins the key ranges' (m, l, sum) of each row (attention_q8.hip). partial: [rows][splits][2 + dim].
-void LaunchAttendJoin(const float* partial, float* out, int64_t rows, int32_t splits, int32_t dim, hipStream_t stream);
+// kN floats of a query row from dim d on, 0 past the row. vec: whole 16-byte pieces (a.dim % 4 == 0).
+template <int kN>
+__device__ __forceinline__ void LoadQuery(const AttendArgs& a, const float* q, int d, bool vec, float (&x)[kN]) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < kN / 4; ++i) {
+      const f4 y = d + 4 * i < a.dim ? *reinterpret_cast<const f4*>(q + d + 4 * i) : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = y[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) x[e] = d + e < a.dim ? q[d + e] : 0.f;
+  }
+}
+__device__ __forceinline__ bool QueryVec(const AttendArgs& a) {  // uniform
+  return a.dim % 4 == 0 && a.q_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
+}
+
+// Partial results of key ranges: of each (row, range) the reference m and the sum l, and the weighted
+// sum of PartialDims(dim) floats, 16-byte aligned.
+inline __host__ __device__ int32_t PartialDims(int32_t dim) { return (dim + 3) & ~3; }
+struct AttendPartial {
+  float* ml;  // [rows][splits][2]
+  float* o;   // [rows][splits][PartialDims]
+};
+
+// The parts of a workgroup's kWaves waves for its kRows rows meet in LDS: each row's joined (m, l, sum)
+// goes to `partial`, or with one key range the quotient to the output.
+template <int DP, int kWaves, int kRows>
+struct WaveParts {
+  float o[kWaves][kRows][DP + 4];
+  float m[kWaves][kRows];
+  float l[kWaves][kRows];
+  __device__ __forceinline__ void Join(const AttendArgs& a, int32_t kv, int32_t group, int32_t r0, int32_t rows,
+                                       int32_t split, int32_t splits, const AttendPartial& partial) const {
+    const bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+    for (int item = threadIdx.x; item < kRows * DP / 4; item += 64 * kWaves) {
+      const int rl = item / (DP / 4);
+      const int d = item % (DP / 4) * 4;
+      const int32_t r = r0 + rl;
+      if (r >= rows || d >= a.dim) continue;
+      float big = m[0][rl];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) big = fmaxf(big, m[w][rl]);
+      const float base = big == -INFINITY ? 0.f : big;
+      float total = 0.f;
+      f4 x = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float wt = __builtin_amdgcn_exp2f(m[w][rl] - base);
+        total += wt * l[w][rl];
+        x += wt * *reinterpret_cast<const f4*>(&o[w][rl][d]);
+      }
+      const int32_t s = r / group;
+      const int64_t out_row = static_cast<int64_t>(s) * a.heads + kv * group + (r - s * group);
+      if (splits > 1) {
+        const int64_t at = out_row * splits + split;
+        if (d == 0) {
+          partial.ml[2 * at] = big;
+          partial.ml[2 * at + 1] = total;
+        }
+        *reinterpret_cast<f4*>(partial.o + at * PartialDims(a.dim) + d) = x;
+      } else {
+        float* dst = a.out + out_row * a.dim + d;
+        const f4 y = f4{__fdiv_rn(x[0], total), __fdiv_rn(x[1], total), __fdiv_rn(x[2], total), __fdiv_rn(x[3], total)};
+        if (vec) {
+          *reinterpret_cast<f4*>(dst) = y;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < a.dim) dst[e] = y[e];
+        }
+      }
+    }
+  }
+};
+
+// Into how many key ranges `units` workgroups' worth of rows are cut, at most `most`: up to two
+// workgroups per CU. Where the partial sums have no room the range stays whole.
+struct AttendSplit {
+  int32_t count = 1;
+  AttendPartial partial{nullptr, nullptr};
+};
+AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t most);
+
+// Joins the key ranges of each row into the output (attention_q8.hip).
+void LaunchAttendJoin(const AttendArgs& a, const AttendPartial& partial, int32_t splits, hipStream_t stream);
 
 }  // namespace accel_hip

@@ -29,7 +29,7 @@ struct PromptArgs {
   const float* k_scale;  // 8-bit only
   const float* v_scale;
   int32_t block_shift, splits, tiles;
-  float* partial;
+  AttendPartial partial;
 };
 
 // kF32: an fp32 cache. kLoad: bytes that may be loaded at once (16, 4 or 1; 16 or 4 for fp32).
@@ -171,14 +171,15 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   float row_factor;
   {
     const float* q = a.q + s * a.q_stride + static_cast<int64_t>(head) * a.dim;
+    const bool vec = QueryVec(a);
+    float x[kSteps][8];
     uint32_t top = 0;
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) LoadQuery(a, q, 16 * st + 8 * g, vec, x[st]);
 #pragma unroll
     for (int st = 0; st < kSteps; ++st)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = 16 * st + 8 * g + e;
-        if (d < a.dim) top = max(top, __float_as_uint(q[d]) & 0x7fffffffu);
-      }
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[st][e]) & 0x7fffffffu);
     top = max(top, XorLane<32>(top));
     const bool bad = top >= 0x7f800000u;
     const float scale = RowScale(top);
@@ -187,11 +188,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
     for (int st = 0; st < kSteps; ++st) {
       h2 hi[4], lo[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = 16 * st + 8 * g + 2 * e;
-        const float x0 = d < a.dim ? q[d] * scale : 0.f, x1 = d + 1 < a.dim ? q[d + 1] * scale : 0.f;
-        SplitF16(bad ? NAN : x0, bad ? NAN : x1, hi[e], lo[e]);
-      }
+      for (int e = 0; e < 4; ++e)
+        SplitF16(bad ? NAN : x[st][2 * e] * scale, bad ? NAN : x[st][2 * e + 1] * scale, hi[e], lo[e]);
       qh[st] = Join(hi[0], hi[1], hi[2], hi[3]);
       ql[st] = Join(lo[0], lo[1], lo[2], lo[3]);
     }
@@ -377,31 +375,29 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   if (w0 + j >= rows) return;
   const int64_t out_row = static_cast<int64_t>(s) * a.heads + head;
   float* dst = a.out + out_row * a.dim;
-  float by = 1.f;
+  bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
   if (b.splits > 1) {
-    dst = b.partial + (out_row * b.splits + split) * (2 + a.dim);
+    const int64_t at = out_row * b.splits + split;
+    dst = b.partial.o + at * PartialDims(a.dim);
+    vec = true;
     if (g == 0) {
-      dst[0] = m;
-      dst[1] = l;
+      b.partial.ml[2 * at] = m;
+      b.partial.ml[2 * at + 1] = l;
     }
-    dst += 2;
-  } else {
-    by = l;
   }
-  const bool vec = b.splits == 1 && a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
 #pragma unroll
   for (int t = 0; t < kDims; ++t)
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
       const int d = 32 * t + 8 * r4 + 4 * g;
-      float o[4];
+      f4 o;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         o[e] = ldexpf(acc[t][4 * r4 + e], -power);
-        if (b.splits == 1) o[e] = __fdiv_rn(o[e], by);
+        if (b.splits == 1) o[e] = __fdiv_rn(o[e], l);
       }
       if (vec) {
-        if (d < a.dim) *reinterpret_cast<float4*>(dst + d) = make_float4(o[0], o[1], o[2], o[3]);
+        if (d < a.dim) *reinterpret_cast<f4*>(dst + d) = o;
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -443,7 +439,7 @@ void LaunchPromptOf(const AttendArgs& a, PromptArgs b, int load, hipStream_t str
   if (a.dim <= 64) LaunchPrompt<64, kF32>(a, b, load, stream);
   else if (a.dim <= 128) LaunchPrompt<128, kF32>(a, b, load, stream);
   else LaunchPrompt<256, kF32>(a, b, load, stream);
-  if (b.splits > 1) LaunchAttendJoin(b.partial, a.out, int64_t(a.seq) * a.heads, b.splits, a.dim, stream);
+  if (b.splits > 1) LaunchAttendJoin(a, b.partial, b.splits, stream);
 }
 
 }  // namespace

@@ -25,15 +25,13 @@ constexpr int kStepKeys = 32;
 // The next step's keys are requested after the scores, its values after the sums.
 template <int DP, int kLoad, int kScales>
 __global__ __launch_bounds__(kThreads) void AttendQ8StepKernel(AttendArgs a, Q8Cache c, int32_t splits,
-                                                               int32_t tiles, float* partial) {
+                                                               AttendPartial partial) {
   constexpr int kC = DP / 64;       // 16-byte pieces of a key row per lane
   constexpr int kTiles = DP / 16;   // dim tiles
   constexpr int kVWords = DP / 64;  // 4-byte words of a value row per lane
   constexpr int kGroups = kScales == 1 ? 1 : 2;  // scale loads a step: one, one per 4 keys, one per key
   constexpr int kEach = kScales == 8 ? 4 : 1;
-  __shared__ __align__(16) float part_o[kWaves][kStepRows][DP + 4];
-  __shared__ float part_m[kWaves][kStepRows];
-  __shared__ float part_l[kWaves][kStepRows];
+  __shared__ __align__(16) WaveParts<DP, kWaves, kStepRows> parts;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -119,15 +117,14 @@ __global__ __launch_bounds__(kThreads) void AttendQ8StepKernel(AttendArgs a, Q8C
   {
     float x[kC][16];
     const float* q = a.q + s * a.q_stride + static_cast<int64_t>(head) * a.dim;
+    const bool vec = QueryVec(a);
     uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kC; ++i) LoadQuery(a, q, 64 * i + 16 * g, vec, x[i]);
 #pragma unroll
     for (int i = 0; i < kC; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int d = 64 * i + 16 * g + e;
-        x[i][e] = d < a.dim ? q[d] : 0.f;
-        top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
-      }
+      for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
     top = max(top, XorLane<16>(top));
     top = max(top, XorLane<32>(top));
     const bool bad = top >= 0x7f800000u;  // no finite row: all of it NaN
@@ -260,109 +257,123 @@ __global__ __launch_bounds__(kThreads) void AttendQ8StepKernel(AttendArgs a, Q8C
   l = l + XorLane<16>(l);
   l = l + XorLane<32>(l);
   if (g == 0) {
-    part_m[wave][j] = m;
-    part_l[wave][j] = l;
+    parts.m[wave][j] = m;
+    parts.l[wave][j] = l;
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) part_o[wave][j][kTiles * (4 * g + r) + t] = ldexpf(acc[t][r], -row_state.power);
+    for (int t = 0; t < kTiles; t += 4) {
+      const int32_t down = -row_state.power;
+      *reinterpret_cast<f4*>(&parts.o[wave][j][kTiles * (4 * g + r) + t]) =
+          f4{ldexpf(acc[t][r], down), ldexpf(acc[t + 1][r], down), ldexpf(acc[t + 2][r], down), ldexpf(acc[t + 3][r], down)};
+    }
   __syncthreads();
-  for (int item = tid; item < kStepRows * DP; item += kThreads) {
-    const int rl = item / DP;
-    const int d = item % DP;
-    if (r0 + rl >= rows || d >= a.dim) continue;
-    float big = part_m[0][rl];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) big = fmaxf(big, part_m[w][rl]);
-    const float base = big == -INFINITY ? 0.f : big;
-    float total = 0.f, o = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float wt = __builtin_amdgcn_exp2f(part_m[w][rl] - base);
-      total += wt * part_l[w][rl];
-      o += wt * part_o[w][rl][d];
-    }
-    const int32_t sr = (r0 + rl) / group;
-    const int64_t out_row = static_cast<int64_t>(sr) * a.heads + kv * group + (r0 + rl - sr * group);
-    if (splits > 1) {
-      float* dst = partial + (out_row * splits + split) * (2 + a.dim);
-      if (d == 0) {
-        dst[0] = big;
-        dst[1] = total;
-      }
-      dst[2 + d] = o;
-    } else {
-      a.out[out_row * a.dim + d] = __fdiv_rn(o, total);
-    }
-  }
+  parts.Join(a, kv, group, r0, rows, split, splits, partial);
 }
 
-// One workgroup per row; its waves take every fourth key range, their lanes the dims.
-__global__ __launch_bounds__(kThreads) void AttendJoinKernel(const float* partial, float* out, int32_t splits,
-                                                             int32_t dim) {
-  __shared__ float part[kWaves][256 + 1];
-  __shared__ float part_l[kWaves];
-  const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
+// One workgroup per row: its threads are the row's 16-byte pieces times the key ranges, 8 ranges of a
+// thread in flight at once, since a round trip to what other workgroups left is all this costs.
+constexpr int kJoinEach = 8;
+__global__ __launch_bounds__(kThreads) void AttendJoinKernel(const float* ml, const float* o, float* out, int32_t splits,
+                                                             int32_t dim, bool vec) {
+  __shared__ __align__(16) f4 part_o[kThreads];
+  __shared__ float part_m[kThreads];
+  __shared__ float part_l[kThreads];
+  const int dims = PartialDims(dim);
+  const int pieces = dims / 4;
+  const int lanes = kThreads / pieces;  // key ranges at a time
+  const int piece = threadIdx.x % pieces;
+  const int of = threadIdx.x / pieces;
   const int64_t row = blockIdx.x;
-  const float* p = partial + row * splits * (2 + dim);
-  const int stride = 2 + dim;
-  float big = -INFINITY;
-  for (int c = lane; c < splits; c += 64) big = fmaxf(big, p[c * stride]);
-  big = WaveButterfly(big, [](float x, float y) { return fmaxf(x, y); });
-  const float base = big == -INFINITY ? 0.f : big;
-  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int c = wave; c < splits; c += kWaves) {
-    const float* q = p + c * stride;
-    const float wt = __builtin_amdgcn_exp2f(q[0] - base);
-    l += wt * q[1];
+  ml += row * splits * 2;
+  o += row * splits * dims + 4 * piece;
+  float m = -INFINITY, l = 0.f;
+  f4 sum = f4{0.f, 0.f, 0.f, 0.f};
+  if (of < lanes) {
+    for (int c0 = of; c0 < splits; c0 += lanes * kJoinEach) {
+      float2 y[kJoinEach];
+      f4 x[kJoinEach];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 64 * i < dim) o[i] += wt * q[2 + lane + 64 * i];
+      for (int i = 0; i < kJoinEach; ++i) {
+        const int c = min(c0 + i * lanes, splits - 1);
+        y[i] = *reinterpret_cast<const float2*>(ml + 2 * c);
+        x[i] = *reinterpret_cast<const f4*>(o + static_cast<int64_t>(c) * dims);
+      }
+      float big = m;
+#pragma unroll
+      for (int i = 0; i < kJoinEach; ++i)
+        if (c0 + i * lanes < splits) big = fmaxf(big, y[i].x);
+      const float base = big == -INFINITY ? 0.f : big;
+      const float corr = __builtin_amdgcn_exp2f(m - base);
+      l *= corr;
+      sum *= corr;
+#pragma unroll
+      for (int i = 0; i < kJoinEach; ++i) {
+        if (c0 + i * lanes >= splits) break;
+        const float w = __builtin_amdgcn_exp2f(y[i].x - base);
+        l += w * y[i].y;
+        sum += w * x[i];
+      }
+      m = big;
+    }
+    part_m[threadIdx.x] = m;
+    part_l[threadIdx.x] = l;
+    part_o[threadIdx.x] = sum;
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) part[wave][lane + 64 * i] = o[i];
-  if (lane == 0) part_l[wave] = l;
   __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= dim) return;
-  float total = part_l[0], sum = part[0][d];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
-    total += part_l[w];
-    sum += part[w][d];
+  if (of != 0) return;
+  float big = part_m[piece];
+  for (int i = 1; i < lanes; ++i) big = fmaxf(big, part_m[piece + i * pieces]);
+  const float base = big == -INFINITY ? 0.f : big;
+  float total = 0.f;
+  sum = f4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < lanes; ++i) {
+    const float w = __builtin_amdgcn_exp2f(part_m[piece + i * pieces] - base);
+    total += w * part_l[piece + i * pieces];
+    sum += w * part_o[piece + i * pieces];
   }
-  out[row * dim + d] = __fdiv_rn(sum, total);
+  float* dst = out + row * dim + 4 * piece;
+  const f4 y = f4{__fdiv_rn(sum[0], total), __fdiv_rn(sum[1], total), __fdiv_rn(sum[2], total), __fdiv_rn(sum[3], total)};
+  if (vec) {
+    *reinterpret_cast<f4*>(dst) = y;
+  } else {
+    for (int e = 0; e < 4; ++e)
+      if (4 * piece + e < dim) dst[e] = y[e];
+  }
 }
 
 }  // namespace
 
-void LaunchAttendJoin(const float* partial, float* out, int64_t rows, int32_t splits, int32_t dim, hipStream_t stream) {
-  hipLaunchKernelGGL(AttendJoinKernel, dim3(static_cast<uint32_t>(rows)), dim3(kThreads), 0, stream, partial, out, splits, dim);
+void LaunchAttendJoin(const AttendArgs& a, const AttendPartial& partial, int32_t splits, hipStream_t stream) {
+  const bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+  hipLaunchKernelGGL(AttendJoinKernel, dim3(static_cast<uint32_t>(a.seq) * static_cast<uint32_t>(a.heads)), dim3(kThreads), 0,
+                     stream, partial.ml, partial.o, a.out, splits, a.dim, vec);
   Check(hipGetLastError(), "AttendJoinKernel launch");
 }
 
 AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t most) {
   const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
   const int64_t count = std::max<int64_t>(1, std::min<int64_t>(2 * cus / units, most));
-  const size_t bytes = static_cast<size_t>(int64_t(a.seq) * a.heads * count * (2 + a.dim)) * sizeof(float);
+  const int64_t parts = int64_t(a.seq) * a.heads * count;
+  const size_t ml_bytes = (static_cast<size_t>(parts) * 2 * sizeof(float) + 15) & ~size_t(15);
+  const size_t bytes = ml_bytes + static_cast<size_t>(parts * PartialDims(a.dim)) * sizeof(float);
   AttendSplit split;
   if (count == 1 || !ScratchReady(bytes, kTempFlags, 0)) return split;
   split.count = static_cast<int32_t>(count);
-  split.partial = static_cast<float*>(Workspace(bytes));
+  split.partial.ml = static_cast<float*>(Workspace(bytes));
+  split.partial.o = split.partial.ml + ml_bytes / sizeof(float);
   return split;
 }
 
 namespace {
 
 template <int DP>
-void LaunchStep(const AttendArgs& a, const Q8Cache& c, int load, int32_t splits, int32_t tiles, float* partial,
+void LaunchStep(const AttendArgs& a, const Q8Cache& c, int load, const AttendSplit& split, int64_t units,
                 hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(int64_t(a.kv_heads) * splits * tiles)), block(kThreads);
+  const dim3 grid(static_cast<uint32_t>(units * split.count)), block(kThreads);
 #define ACCEL_STEP(L, S) \
-  hipLaunchKernelGGL((AttendQ8StepKernel<DP, L, S>), grid, block, 0, stream, a, c, splits, tiles, partial)
+  hipLaunchKernelGGL((AttendQ8StepKernel<DP, L, S>), grid, block, 0, stream, a, c, split.count, split.partial)
   if (load == 16) {
     if (c.block_shift >= 5) ACCEL_STEP(16, 1);
     else if (c.block_shift >= 2) ACCEL_STEP(16, 2);
@@ -392,10 +403,10 @@ void LaunchAttentionQ8(const AttendArgs& a, const Q8Cache& c, hipStream_t stream
   const int64_t units = tiles * a.kv_heads;
   if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
   const AttendSplit split = SplitRange(a, units, AttendRangeSteps(a, kStepRows, kStepKeys) / kWaves);
-  if (a.dim <= 64) LaunchStep<64>(a, c, load, split.count, static_cast<int32_t>(tiles), split.partial, stream);
-  else if (a.dim <= 128) LaunchStep<128>(a, c, load, split.count, static_cast<int32_t>(tiles), split.partial, stream);
-  else LaunchStep<256>(a, c, load, split.count, static_cast<int32_t>(tiles), split.partial, stream);
-  if (split.count > 1) LaunchAttendJoin(split.partial, a.out, int64_t(a.seq) * a.heads, split.count, a.dim, stream);
+  if (a.dim <= 64) LaunchStep<64>(a, c, load, split, units, stream);
+  else if (a.dim <= 128) LaunchStep<128>(a, c, load, split, units, stream);
+  else LaunchStep<256>(a, c, load, split, units, stream);
+  if (split.count > 1) LaunchAttendJoin(a, split.partial, split.count, stream);
 }
 
 }  // namespace accel_hip

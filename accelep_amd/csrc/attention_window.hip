@@ -24,12 +24,10 @@ constexpr int kKeys = 16;  // of a wave's step
 // holds one (a test of the bits, uniform) has its values taken as zeros and its weights as NaN.
 template <int DP, int kLoad>
 __global__ __launch_bounds__(kThreads) void AttendF32StepKernel(AttendArgs a, const float* k, const float* v,
-                                                                int32_t splits, float* partial) {
+                                                                int32_t splits, AttendPartial partial) {
   constexpr int kI = DP / 16;  // 16-byte pieces of a key row per lane
   constexpr int kC = DP / 64;  // of a value row
-  __shared__ __align__(16) float part_o[kWaves][kRows][DP + 4];
-  __shared__ float part_m[kWaves][kRows];
-  __shared__ float part_l[kWaves][kRows];
+  __shared__ __align__(16) WaveParts<DP, kWaves, kRows> parts;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -83,10 +81,13 @@ __global__ __launch_bounds__(kThreads) void AttendF32StepKernel(AttendArgs a, co
   f4 q[kI];
   {
     const float* p = a.q + s * a.q_stride + static_cast<int64_t>(head) * a.dim;
+    const bool vec = QueryVec(a);
 #pragma unroll
-    for (int i = 0; i < kI; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) q[i][e] = 16 * i + 4 * g + e < a.dim ? p[16 * i + 4 * g + e] : 0.f;
+    for (int i = 0; i < kI; ++i) {
+      float x[4];
+      LoadQuery(a, p, 16 * i + 4 * g, vec, x);
+      q[i] = f4{x[0], x[1], x[2], x[3]};
+    }
   }
   const float factor = kLog2e * __fdiv_rn(1.f, __fsqrt_rn(static_cast<float>(a.dim)));
 
@@ -175,52 +176,25 @@ __global__ __launch_bounds__(kThreads) void AttendF32StepKernel(AttendArgs a, co
   l = l + XorLane<16>(l);
   l = l + XorLane<32>(l);
   if (g == 0) {
-    part_m[wave][j] = m;
-    part_l[wave][j] = l;
+    parts.m[wave][j] = m;
+    parts.l[wave][j] = l;
   }
 #pragma unroll
   for (int c = 0; c < kC; ++c)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      *reinterpret_cast<f4*>(&part_o[wave][j][64 * c + 16 * g + 4 * r]) =
+      *reinterpret_cast<f4*>(&parts.o[wave][j][64 * c + 16 * g + 4 * r]) =
           f4{acc[c][0][r], acc[c][1][r], acc[c][2][r], acc[c][3][r]};
   __syncthreads();
-  for (int item = tid; item < kRows * DP; item += kThreads) {
-    const int rl = item / DP;
-    const int d = item % DP;
-    if (r0 + rl >= rows || d >= a.dim) continue;
-    float big = part_m[0][rl];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) big = fmaxf(big, part_m[w][rl]);
-    const float base = big == -INFINITY ? 0.f : big;
-    float total = 0.f, o = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float wt = __builtin_amdgcn_exp2f(part_m[w][rl] - base);
-      total += wt * part_l[w][rl];
-      o += wt * part_o[w][rl][d];
-    }
-    const int32_t sr = (r0 + rl) / group;
-    const int64_t out_row = static_cast<int64_t>(sr) * a.heads + kv * group + (r0 + rl - sr * group);
-    if (splits > 1) {
-      float* dst = partial + (out_row * splits + split) * (2 + a.dim);
-      if (d == 0) {
-        dst[0] = big;
-        dst[1] = total;
-      }
-      dst[2 + d] = o;
-    } else {
-      a.out[out_row * a.dim + d] = __fdiv_rn(o, total);
-    }
-  }
+  parts.Join(a, kv, group, r0, rows, split, splits, partial);
 }
 
 template <int DP>
-void LaunchStep(const AttendArgs& a, const float* k, const float* v, bool vec, int32_t splits, int64_t units,
-                float* partial, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(units * splits)), block(kThreads);
-  if (vec) hipLaunchKernelGGL((AttendF32StepKernel<DP, 16>), grid, block, 0, stream, a, k, v, splits, partial);
-  else hipLaunchKernelGGL((AttendF32StepKernel<DP, 4>), grid, block, 0, stream, a, k, v, splits, partial);
+void LaunchStep(const AttendArgs& a, const float* k, const float* v, bool vec, const AttendSplit& split,
+                int64_t units, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(units * split.count)), block(kThreads);
+  if (vec) hipLaunchKernelGGL((AttendF32StepKernel<DP, 16>), grid, block, 0, stream, a, k, v, split.count, split.partial);
+  else hipLaunchKernelGGL((AttendF32StepKernel<DP, 4>), grid, block, 0, stream, a, k, v, split.count, split.partial);
   Check(hipGetLastError(), "AttendF32StepKernel launch");
 }
 
@@ -236,10 +210,10 @@ void LaunchAttentionWindow(const AttendArgs& a, const float* k, const float* v, 
   const int64_t units = (int64_t(a.seq) * group + kRows - 1) / kRows * a.kv_heads;
   if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
   const AttendSplit split = SplitRange(a, units, AttendRangeSteps(a, kRows, kKeys) / kWaves);
-  if (a.dim <= 64) LaunchStep<64>(a, k, v, vec, split.count, units, split.partial, stream);
-  else if (a.dim <= 128) LaunchStep<128>(a, k, v, vec, split.count, units, split.partial, stream);
-  else LaunchStep<256>(a, k, v, vec, split.count, units, split.partial, stream);
-  if (split.count > 1) LaunchAttendJoin(split.partial, a.out, int64_t(a.seq) * a.heads, split.count, a.dim, stream);
+  if (a.dim <= 64) LaunchStep<64>(a, k, v, vec, split, units, stream);
+  else if (a.dim <= 128) LaunchStep<128>(a, k, v, vec, split, units, stream);
+  else LaunchStep<256>(a, k, v, vec, split, units, stream);
+  if (split.count > 1) LaunchAttendJoin(a, split.partial, split.count, stream);
 }
 
 }  // namespace accel_hip
