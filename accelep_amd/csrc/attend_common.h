@@ -55,7 +55,10 @@ __device__ __forceinline__ h2 PackRtz(float x, float y) {
 // in the matrix core's fp32 sums.
 __device__ __forceinline__ void SplitF16(float x, float y, h2& hi, h2& lo) {
   hi = PackRtz(x, y);
-  lo = PackRtz(__builtin_fmaf(static_cast<float>(hi[0]), -1.f, x), __builtin_fmaf(static_cast<float>(hi[1]), -1.f, y));
+  float rx, ry;  // x - hi[0], y - hi[1]: one instruction each, which the compiler makes two of
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rx) : "v"(hi), "v"(x));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(ry) : "v"(hi), "v"(y));
+  lo = PackRtz(rx, ry);
 }
 
 // 2^(13 - e) for a row whose largest magnitude has the exponent e: the row then fills [2^13, 2^14).
@@ -73,28 +76,54 @@ __device__ __forceinline__ h2 CodesHigh(uint32_t w) {
 }
 __device__ __forceinline__ h8 Join(h2 a, h2 b, h2 c, h2 d) { return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}; }
 
-// A row's softmax while its keys pass. m: the largest score (in log2 units) so far; l: the sum of
-// p = 2^(s - m). The weighted sum holds p * value scale * 2^power, where `power` keeps the largest
-// p * value scale so far (`top`, relative to m) in [2^14, 2^15): all of f16's range lies below it, and a
-// key that a row does not see has no say in it.
-struct RowState {
-  float m = -INFINITY, l = 0.f, top = 0.f;
-  int32_t power = 127;
-  __device__ __forceinline__ static int32_t PowerOf(float top) {
-    const int32_t e = static_cast<int32_t>(__float_as_uint(top) >> 23) - 127;
-    return min(14 - e, 127);
-  }
-};
+// A row's softmax while its keys pass holds m, a reference for its scores in log2 units, l, the sum of
+// p = 2^(s - m), and `top`, the largest p * value scale so far. The weighted sum holds p * value scale *
+// 2^power, with top * 2^power kept in [2^3, 2^15): a weight then has 22 bits down to 2^-6 of the largest
+// and is off by 2^-28 of that below, whatever the scales, and a key that a row does not see has no say.
+constexpr int32_t kPowerMax = 127;
+__device__ __forceinline__ int32_t WeightPower(float top, int32_t power) {
+  const float at = ldexpf(top, power);
+  if (at < 0x1p15f && (at >= 8.f || !(top > 0.f))) return power;
+  const int32_t e = static_cast<int32_t>(__float_as_uint(top) >> 23) - 127;
+  return min(6 - e, kPowerMax);
+}
 
-// 4 codes from dim d on, 0 past the row.
-template <int kLoad>
-__device__ __forceinline__ uint32_t LoadCodes4(const int8_t* p, int d, int dim) {
-  if (kLoad >= 4) return d < dim ? *reinterpret_cast<const uint32_t*>(p) : 0u;
-  uint32_t w = 0;
+// Codes are read through buffer descriptors whose bounds are the range's last key row: rows past it read
+// as 0, with no address to clamp. Dims past a head's read whatever lies there, a code of the next head or
+// 0, which meets a query of 0, or as a value makes a dim that is not stored.
+typedef __amdgpu_buffer_rsrc_t CodeRows;
+__device__ __forceinline__ CodeRows RowsFrom(const int8_t* head, int32_t kv_row, int32_t dim, int32_t t0, int32_t high) {
+  // The bytes from this head's part of row t0 to its end in the last row; a step's offsets stay below 2^30.
+  const int64_t bytes = static_cast<int64_t>(high - 1 - t0) * kv_row + dim;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(head + static_cast<int64_t>(t0) * kv_row), 0,
+                                           static_cast<int32_t>(min(bytes, int64_t(1) << 30)), 0x00027000);
+}
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+// kWords * 4 codes at the offset; kLoad: the bytes that lie at a multiple of themselves (4 or more: words).
+template <int kWords, int kLoad>
+__device__ __forceinline__ void LoadCodes(CodeRows rows, uint32_t offset, uint32_t (&w)[kWords]) {
+  if constexpr (kLoad == 16 && kWords == 4) {
+    const u4 x = __builtin_amdgcn_raw_buffer_load_b128(rows, offset, 0, 0);
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (d + e < dim) w |= static_cast<uint32_t>(static_cast<uint8_t>(p[e])) << (8 * e);
-  return w;
+    for (int e = 0; e < 4; ++e) w[e] = x[e];
+  } else if constexpr (kLoad == 16 && kWords == 2) {
+    const u2 x = __builtin_amdgcn_raw_buffer_load_b64(rows, offset, 0, 0);
+    w[0] = x[0];
+    w[1] = x[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if (kLoad >= 4) {
+        w[i] = __builtin_amdgcn_raw_buffer_load_b32(rows, offset + 4 * i, 0, 0);
+      } else {
+        w[i] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[i] |= static_cast<uint32_t>(__builtin_amdgcn_raw_buffer_load_b8(rows, offset + 4 * i + e, 0, 0)) << (8 * e);
+      }
+    }
+  }
 }
 
 // The most steps of a block of `rows` rows' key range.
@@ -107,11 +136,14 @@ inline int64_t AttendRangeSteps(const AttendArgs& a, int64_t rows, int64_t step)
   return (keys + step - 1) / step + (std::min<int64_t>(a.sinks, end) + step - 1) / step;
 }
 
+// Bytes (or floats) of a key row, all heads, up to which a step's rows lie within 32-bit offsets.
+constexpr int32_t kAttendRowMax = 1 << 24;
 // Rows of a key head above which the tiles of keys go through LDS.
 constexpr int64_t kAttendPromptRows = 64;
 // Many rows (attend_prompt.hip). load: the bytes that a thread may load at once from keys and values.
 void LaunchAttendPromptQ8(const AttendArgs& a, const Q8Cache& c, int load, hipStream_t stream);
 void LaunchAttendPromptF32(const AttendArgs& a, const float* k, const float* v, int load, hipStream_t stream);
+
 // kN floats of a query row from dim d on, 0 past the row. vec: whole 16-byte pieces (a.dim % 4 == 0).
 template <int kN>
 __device__ __forceinline__ void LoadQuery(const AttendArgs& a, const float* q, int d, bool vec, float (&x)[kN]) {
@@ -139,35 +171,37 @@ struct AttendPartial {
   float* o;   // [rows][splits][PartialDims]
 };
 
-// The parts of a workgroup's kWaves waves for its kRows rows meet in LDS: each row's joined (m, l, sum)
-// goes to `partial`, or with one key range the quotient to the output.
+// The results of a workgroup's waves for kRows rows meet in LDS. Wave w serves head w % heads of the
+// workgroup's `heads` key heads and has every (waves / heads)-th step of the key range: each row's joined
+// (m, l, sum) goes to `partial`, or with one key range the quotient to the output.
 template <int DP, int kWaves, int kRows>
 struct WaveParts {
   float o[kWaves][kRows][DP + 4];
   float m[kWaves][kRows];
   float l[kWaves][kRows];
-  __device__ __forceinline__ void Join(const AttendArgs& a, int32_t kv, int32_t group, int32_t r0, int32_t rows,
-                                       int32_t split, int32_t splits, const AttendPartial& partial) const {
+  __device__ __forceinline__ void Join(const AttendArgs& a, int32_t kv0, int32_t heads, int32_t group, int32_t r0,
+                                       int32_t rows, int32_t split, int32_t splits, const AttendPartial& partial) const {
     const bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
-    for (int item = threadIdx.x; item < kRows * DP / 4; item += 64 * kWaves) {
-      const int rl = item / (DP / 4);
-      const int d = item % (DP / 4) * 4;
-      const int32_t r = r0 + rl;
-      if (r >= rows || d >= a.dim) continue;
-      float big = m[0][rl];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) big = fmaxf(big, m[w][rl]);
+    const int32_t n = min(kRows, rows - r0);
+    const int32_t waves = static_cast<int32_t>(blockDim.x) / 64;
+    for (int32_t item = threadIdx.x; item < heads * n * (DP / 4); item += blockDim.x) {
+      const int32_t hr = item / (DP / 4);
+      const int32_t d = item % (DP / 4) * 4;
+      const int32_t h = hr / n;
+      const int32_t rl = hr - h * n;
+      if (d >= a.dim) continue;
+      float big = -INFINITY;
+      for (int32_t w = h; w < waves; w += heads) big = fmaxf(big, m[w][rl]);
       const float base = big == -INFINITY ? 0.f : big;
       float total = 0.f;
       f4 x = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+      for (int32_t w = h; w < waves; w += heads) {
         const float wt = __builtin_amdgcn_exp2f(m[w][rl] - base);
         total += wt * l[w][rl];
         x += wt * *reinterpret_cast<const f4*>(&o[w][rl][d]);
       }
-      const int32_t s = r / group;
-      const int64_t out_row = static_cast<int64_t>(s) * a.heads + kv * group + (r - s * group);
+      const int32_t s = (r0 + rl) / group;
+      const int64_t out_row = static_cast<int64_t>(s) * a.heads + (kv0 + h) * group + (r0 + rl - s * group);
       if (splits > 1) {
         const int64_t at = out_row * splits + split;
         if (d == 0) {
@@ -190,13 +224,13 @@ struct WaveParts {
   }
 };
 
-// Into how many key ranges `units` workgroups' worth of rows are cut, at most `most`: up to two
-// workgroups per CU. Where the partial sums have no room the range stays whole.
+// Into how many key ranges the rows of `units` workgroups are cut: up to per_cu workgroups per CU, at
+// most `most` ranges. Where the partial sums have no room the range stays whole.
 struct AttendSplit {
   int32_t count = 1;
   AttendPartial partial{nullptr, nullptr};
 };
-AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t most);
+AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t per_cu, int64_t most);
 
 // Joins the key ranges of each row into the output (attention_q8.hip).
 void LaunchAttendJoin(const AttendArgs& a, const AttendPartial& partial, int32_t splits, hipStream_t stream);

@@ -78,33 +78,30 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   uint4 kreg[kChunks], vreg[kChunks];
   float ks_next = 0.f, vs_next = 0.f;
   const auto fetch_plane = [&](const void* base, int32_t t0, uint4 (&x)[kChunks]) {
+    if constexpr (kF32) {
+      // A row past the range reads its last one, a piece past a head's dims its last: both are not used.
+      const float* p = static_cast<const float*>(base) + min(t0 + tid / 8, range.high - 1) * kv_row + static_cast<int64_t>(kv) * a.dim;
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int key = kF32 ? tid / 8 : (tid + i * kThreads) / (DP / 16);
-      const int d = kF32 ? 4 * (tid % 8 + 8 * i) : 16 * ((tid + i * kThreads) % (DP / 16));
-      const int64_t at = min(t0 + key, range.high - 1) * kv_row + static_cast<int64_t>(kv) * a.dim + d;
-      uint32_t w[4] = {0, 0, 0, 0};
-      if (kF32) {
-        const float* p = static_cast<const float*>(base) + at;
+      for (int i = 0; i < kChunks; ++i) {
+        const int d = 4 * (tid % 8 + 8 * i);
         if (kLoad == 16) {
-          if (d < a.dim) x[i] = *reinterpret_cast<const uint4*>(p);
-          else x[i] = make_uint4(0, 0, 0, 0);
-          continue;
+          x[i] = *reinterpret_cast<const uint4*>(p + min(d, a.dim - 4));
+        } else {
+          const auto at = [&](int e) { return __float_as_uint(p[min(d + e, a.dim - 1)]); };
+          x[i] = make_uint4(at(0), at(1), at(2), at(3));
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (d + e < a.dim) w[e] = __float_as_uint(p[e]);
-      } else {
-        const int8_t* p = static_cast<const int8_t*>(base) + at;
-        if (kLoad == 16) {
-          if (d < a.dim) x[i] = *reinterpret_cast<const uint4*>(p);
-          else x[i] = make_uint4(0, 0, 0, 0);
-          continue;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = LoadCodes4<(kLoad < 16 ? kLoad : 4)>(p + 4 * e, d + 4 * e, a.dim);
       }
-      x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      const CodeRows rows = RowsFrom(static_cast<const int8_t*>(base) + static_cast<int64_t>(kv) * a.dim,
+                                     static_cast<int32_t>(kv_row), a.dim, t0, range.high);
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int key = (tid + i * kThreads) / (DP / 16);
+        const int d = 16 * ((tid + i * kThreads) % (DP / 16));
+        uint32_t w[4];
+        LoadCodes<4, kLoad>(rows, static_cast<uint32_t>(key * static_cast<int32_t>(kv_row) + d), w);
+        x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
     }
   };
   const auto scale_at = [&](const float* scale, int32_t t) {
@@ -196,7 +193,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   }
 
   float m = -INFINITY, l = 0.f, top = 0.f;
-  int32_t power = 127;
+  int32_t power = kPowerMax;
   f16v acc[kDims];
 #pragma unroll
   for (int t = 0; t < kDims; ++t)
@@ -301,11 +298,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       }
       top = fmaxf(top * corr, tile_top);
       const int32_t power_old = power;
-      const float at = ldexpf(top, power);
-      if (at >= 0x1p15f || (at < 8.f && top > 0.f)) {
-        const int32_t e = static_cast<int32_t>(__float_as_uint(top) >> 23) - 127;
-        power = min(6 - e, 127);
-      }
+      power = WeightPower(top, power);
       const float again = ldexpf(corr, power - power_old);
       if (__any(again != 1.f)) {
 #pragma unroll
@@ -432,7 +425,7 @@ void LaunchPromptOf(const AttendArgs& a, PromptArgs b, int load, hipStream_t str
   const int64_t tiles = (int64_t(a.seq) * group + kRows - 1) / kRows;
   const int64_t units = tiles * a.kv_heads;
   if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
-  const AttendSplit split = SplitRange(a, units, AttendRangeSteps(a, kRows, kF32 ? 32 : 64) / 4);
+  const AttendSplit split = SplitRange(a, units, 1, AttendRangeSteps(a, kRows, kF32 ? 32 : 64) / 4);
   b.splits = split.count;
   b.tiles = static_cast<int32_t>(tiles);
   b.partial = split.partial;

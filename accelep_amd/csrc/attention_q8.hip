@@ -9,12 +9,14 @@
 namespace accel_hip {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
+// Waves of a step workgroup at most: 8, and 4 where a head's 256 dims leave one wave a SIMD.
+constexpr int StepWaves(int dp) { return dp > 128 ? 4 : 8; }
 constexpr int kStepRows = 16;
 constexpr int kStepKeys = 32;
 
-// One workgroup per (16 rows of a key head, key range); its waves take every fourth step of 32 keys.
+// One workgroup per (16 rows of up to 4 key heads, key range): wave w serves head w % hw of them, and the
+// waves of a head take its steps of 32 keys in turn, so that a workgroup reads a key row's heads together
+// (131072 keys of 8 heads of 128: a workgroup a head read them at 4.7 TB/s, 4 heads at 5.7).
 // Bound: the cache's bytes. Keys and values go from memory to registers, and there to f16: no LDS and
 // no barrier in the loop. Lane (j, g) = (lane % 16, lane / 16). Per step
 //  * S^T = K Q^T on v_mfma_f32_16x16x32_f16: the A operand of instruction (c, half) are the codes
@@ -24,24 +26,27 @@ constexpr int kStepKeys = 32;
 //    the lane loads at V[key][DP / 16 * j], transposed in registers.
 // The next step's keys are requested after the scores, its values after the sums.
 template <int DP, int kLoad, int kScales>
-__global__ __launch_bounds__(kThreads) void AttendQ8StepKernel(AttendArgs a, Q8Cache c, int32_t splits,
-                                                               AttendPartial partial) {
+__global__ __launch_bounds__(64 * StepWaves(DP), DP > 128 ? 1 : 2) void AttendQ8StepKernel(
+    AttendArgs a, Q8Cache c, int32_t hw, int32_t splits, AttendPartial partial) {
   constexpr int kC = DP / 64;       // 16-byte pieces of a key row per lane
   constexpr int kTiles = DP / 16;   // dim tiles
   constexpr int kVWords = DP / 64;  // 4-byte words of a value row per lane
   constexpr int kGroups = kScales == 1 ? 1 : 2;  // scale loads a step: one, one per 4 keys, one per key
   constexpr int kEach = kScales == 8 ? 4 : 1;
-  __shared__ __align__(16) WaveParts<DP, kWaves, kStepRows> parts;
+  __shared__ __align__(16) WaveParts<DP, StepWaves(DP), kStepRows> parts;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int j = lane & 15;
   const int g = lane >> 4;
   const int32_t unit = static_cast<int32_t>(blockIdx.x);
-  const int32_t kv = unit % a.kv_heads;
-  const int32_t rest = unit / a.kv_heads;
+  const int32_t head_groups = a.kv_heads / hw;
+  const int32_t kv0 = unit % head_groups * hw;
+  const int32_t kv = kv0 + wave % hw;
+  const int32_t rest = unit / head_groups;
   const int32_t split = rest % splits;
   const int32_t tile = rest / splits;
+  const int32_t sw = static_cast<int32_t>(blockDim.x) / 64 / hw;  // waves of a head
   const int32_t group = a.heads / a.kv_heads;
   const int32_t rows = a.seq * group;
   const int32_t r0 = tile * kStepRows;
@@ -52,46 +57,26 @@ __global__ __launch_bounds__(kThreads) void AttendQ8StepKernel(AttendArgs a, Q8C
   const int32_t s = row / group;
   const int32_t head = kv * group + (row - s * group);
   const int32_t p_row = r0 + j < rows ? a.position + s : -1;  // a row past the last sees nothing
-  const int64_t kv_row = static_cast<int64_t>(a.kv_heads) * a.dim;
+  const int32_t kv_row = a.kv_heads * a.dim;
   const int8_t* kbase = c.k.code + static_cast<int64_t>(kv) * a.dim;
   const int8_t* vbase = c.v.code + static_cast<int64_t>(kv) * a.dim;
 
   uint32_t kx[2][kC][4];    // [16-key half][piece][word]
   uint32_t vx[8][kVWords];  // [key slot][word]
   float ks[kGroups][kEach], vs[kGroups][kEach];
+  const uint32_t koff = static_cast<uint32_t>(j * kv_row + 16 * g);
+  const uint32_t voff = static_cast<uint32_t>(4 * g * kv_row + DP / 16 * j);
   const auto load_k = [&](int32_t t0) {
+    const CodeRows rows = RowsFrom(kbase, kv_row, a.dim, t0, range.high);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int8_t* p = kbase + min(t0 + 16 * h + j, range.high - 1) * kv_row;
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < kC; ++i) {
-        const int d = 64 * i + 16 * g;
-        if (kLoad == 16) {
-          const uint4 w = d < a.dim ? *reinterpret_cast<const uint4*>(p + d) : make_uint4(0, 0, 0, 0);
-          kx[h][i][0] = w.x, kx[h][i][1] = w.y, kx[h][i][2] = w.z, kx[h][i][3] = w.w;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) kx[h][i][e] = LoadCodes4<kLoad>(p + d + 4 * e, d + 4 * e, a.dim);
-        }
-      }
-    }
+      for (int i = 0; i < kC; ++i) LoadCodes<4, kLoad>(rows, koff + 16 * h * kv_row + 64 * i, kx[h][i]);
   };
   const auto load_v = [&](int32_t t0) {
+    const CodeRows rows = RowsFrom(vbase, kv_row, a.dim, t0, range.high);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int d = DP / 16 * j;
-      const int8_t* p = vbase + min(t0 + (e & 4) * 4 + 4 * g + (e & 3), range.high - 1) * kv_row + d;
-      if (kLoad == 16 && kVWords == 2) {
-        const uint2 w = d < a.dim ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
-        vx[e][0] = w.x, vx[e][1 % kVWords] = w.y;
-      } else if (kLoad == 16 && kVWords == 4) {
-        const uint4 w = d < a.dim ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
-        vx[e][0] = w.x, vx[e][1 % kVWords] = w.y, vx[e][2 % kVWords] = w.z, vx[e][3 % kVWords] = w.w;
-      } else {
-#pragma unroll
-        for (int w = 0; w < kVWords; ++w) vx[e][w] = LoadCodes4<kLoad>(p + 4 * w, d + 4 * w, a.dim);
-      }
-    }
+    for (int e = 0; e < 8; ++e) LoadCodes<kVWords, kLoad>(rows, voff + ((e & 4) * 4 + (e & 3)) * kv_row, vx[e]);
   };
   const auto load_scales = [&](const float* scale, int32_t t0, float (&x)[kGroups][kEach]) {
 #pragma unroll
@@ -103,7 +88,7 @@ __global__ __launch_bounds__(kThreads) void AttendQ8StepKernel(AttendArgs a, Q8C
       }
   };
 
-  int32_t u = split * per + wave;
+  int32_t u = split * per + wave / hw;
   if (u < end) {
     const int32_t t0 = range.Key(u);
     load_k(t0);
@@ -145,15 +130,14 @@ __global__ __launch_bounds__(kThreads) void AttendQ8StepKernel(AttendArgs a, Q8C
       }
   }
 
-  RowState row_state;
-  float& m = row_state.m;
-  float& l = row_state.l;  // this lane's share of the row's sum
+  float m = -INFINITY, l = 0.f, top = 0.f;  // l: this lane's share of the row's sum
+  int32_t power = kPowerMax;
   f4 acc[kTiles];
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
-  for (; u < end; u += kWaves) {  // uniform over the wave
+  for (; u < end; u += sw) {  // uniform over the wave
     const int32_t t0 = range.Key(u);
-    const int32_t next = u + kWaves < end ? range.Key(u + kWaves) : -1;
+    const int32_t next = u + sw < end ? range.Key(u + sw) : -1;
     f4 st[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -181,8 +165,9 @@ __global__ __launch_bounds__(kThreads) void AttendQ8StepKernel(AttendArgs a, Q8C
       load_scales(c.k.scale, next, ks);
     }
     __builtin_amdgcn_sched_barrier(0);
-    // Scores, and the row's largest.
-    const bool whole = range.Whole(a, t0) && r0 + kStepRows <= rows;
+    // Scores, and the row's largest. The reference m moves only when a score passes it by 2^8, so the
+    // sums are seldom scaled.
+    const bool whole = range.Whole(a, t0);  // a row past the last may see what it likes
     uint32_t seen = 255;
     if (!whole) {
       seen = 0;
@@ -193,38 +178,68 @@ __global__ __launch_bounds__(kThreads) void AttendQ8StepKernel(AttendArgs a, Q8C
     float p[8];
     float mx = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      p[e] = seen >> e & 1 ? st[e >> 2][e & 3] * factor[(e >> 2) % kGroups][(e & 3) % kEach] : -INFINITY;
-      mx = fmaxf(mx, p[e]);
+    for (int e = 0; e < 8; ++e) p[e] = st[e >> 2][e & 3] * factor[(e >> 2) % kGroups][(e & 3) % kEach];
+    if (!whole) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = seen >> e & 1 ? p[e] : -INFINITY;
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, p[e]);
     mx = fmaxf(mx, XorLane<16>(mx));
     mx = fmaxf(mx, XorLane<32>(mx));
-    const float m_new = fmaxf(m, mx);
-    const float base = m_new == -INFINITY ? 0.f : m_new;
-    const float corr = __builtin_amdgcn_exp2f(m - base);
-    float sum = 0.f, top = 0.f;
+    const float m_old = m;
+    if (mx > m + 8.f) m = mx;
+    const float base = m == -INFINITY ? 0.f : m;
+    const float corr = __builtin_amdgcn_exp2f(m_old - base);
+    float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       p[e] = __builtin_amdgcn_exp2f(p[e] - base);
       sum += p[e];
-      p[e] = seen >> e & 1 ? p[e] * value[(e >> 2) % kGroups][(e & 3) % kEach] : 0.f;
-      top = fmaxf(top, fabsf(p[e]));
     }
     l = l * corr + sum;
-    m = m_new;
-    top = fmaxf(top, XorLane<16>(top));
-    top = fmaxf(top, XorLane<32>(top));
-    row_state.top = fmaxf(row_state.top * corr, top);
-    const int32_t power = RowState::PowerOf(row_state.top);
-    const float again = ldexpf(corr, power - row_state.power);
-    row_state.power = power;
+    // The weights times the values' scales, and their largest.
+    float step_top = 0.f;
+    if (kScales == 1) {
+      step_top = __builtin_amdgcn_exp2f(mx - base) * value[0][0];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] *= value[(e >> 2) % kGroups][(e & 3) % kEach];
+        if (!whole) p[e] = seen >> e & 1 ? p[e] : 0.f;
+        step_top = fmaxf(step_top, fabsf(p[e]));
+      }
+      step_top = fmaxf(step_top, XorLane<16>(step_top));
+      step_top = fmaxf(step_top, XorLane<32>(step_top));
+    }
+    top = fmaxf(top * corr, step_top);
+    const int32_t power_old = power;
+    power = WeightPower(top, power);
+    const float again = ldexpf(corr, power - power_old);
     if (__any(again != 1.f)) {
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) acc[t] *= again;
     }
+    if (kScales == 1) {
+      const float f = ldexpf(value[0][0], power);
+      if (__any(!(f < 0x1p100f))) {  // a block that is far larger than the sum so far: in two steps
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = ldexpf(p[e] * value[0][0], power);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] *= f;
+      }
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = seen >> e & 1 ? p[e] : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = ldexpf(p[e], power);
+    }
     h2 ph[4], pl[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) SplitF16(ldexpf(p[2 * e], power), ldexpf(p[2 * e + 1], power), ph[e], pl[e]);
+    for (int e = 0; e < 4; ++e) SplitF16(p[2 * e], p[2 * e + 1], ph[e], pl[e]);
     const h8 p_hi = Join(ph[0], ph[1], ph[2], ph[3]), p_lo = Join(pl[0], pl[1], pl[2], pl[3]);
 #pragma unroll
     for (int w = 0; w < kVWords; ++w) {
@@ -264,33 +279,37 @@ __global__ __launch_bounds__(kThreads) void AttendQ8StepKernel(AttendArgs a, Q8C
   for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int t = 0; t < kTiles; t += 4) {
-      const int32_t down = -row_state.power;
+      const int32_t down = -power;
       *reinterpret_cast<f4*>(&parts.o[wave][j][kTiles * (4 * g + r) + t]) =
           f4{ldexpf(acc[t][r], down), ldexpf(acc[t + 1][r], down), ldexpf(acc[t + 2][r], down), ldexpf(acc[t + 3][r], down)};
     }
   __syncthreads();
-  parts.Join(a, kv, group, r0, rows, split, splits, partial);
+  parts.Join(a, kv0, hw, group, r0, rows, split, splits, partial);
 }
 
-// One workgroup per row: its threads are the row's 16-byte pieces times the key ranges, 8 ranges of a
-// thread in flight at once, since a round trip to what other workgroups left is all this costs.
+// A workgroup's threads are (row, key range, 16-byte piece), `lanes` ranges of a row at a time, up to 8
+// of a thread in flight at once: a round trip to what other workgroups left is all this costs.
+constexpr int kJoinThreads = 512;
 constexpr int kJoinEach = 8;
-__global__ __launch_bounds__(kThreads) void AttendJoinKernel(const float* ml, const float* o, float* out, int32_t splits,
-                                                             int32_t dim, bool vec) {
-  __shared__ __align__(16) f4 part_o[kThreads];
-  __shared__ float part_m[kThreads];
-  __shared__ float part_l[kThreads];
+__global__ __launch_bounds__(kJoinThreads) void AttendJoinKernel(const float* ml, const float* o, float* out, int32_t rows,
+                                                                 int32_t splits, int32_t dim, int32_t lanes, bool vec) {
+  __shared__ __align__(16) f4 part_o[kJoinThreads];
+  __shared__ float part_m[kJoinThreads];
+  __shared__ float part_l[kJoinThreads];
   const int dims = PartialDims(dim);
   const int pieces = dims / 4;
-  const int lanes = kThreads / pieces;  // key ranges at a time
-  const int piece = threadIdx.x % pieces;
-  const int of = threadIdx.x / pieces;
-  const int64_t row = blockIdx.x;
-  ml += row * splits * 2;
-  o += row * splits * dims + 4 * piece;
+  const int per_row = pieces * lanes;
+  const int local = threadIdx.x / per_row;
+  const int rest = threadIdx.x - local * per_row;
+  const int of = rest / pieces;
+  const int piece = rest - of * pieces;
+  const int row = static_cast<int>(blockIdx.x) * (kJoinThreads / per_row) + local;
+  const bool active = local < kJoinThreads / per_row && row < rows;
+  ml += static_cast<int64_t>(row) * splits * 2;
+  o += static_cast<int64_t>(row) * splits * dims + 4 * piece;
   float m = -INFINITY, l = 0.f;
   f4 sum = f4{0.f, 0.f, 0.f, 0.f};
-  if (of < lanes) {
+  if (active) {
     for (int c0 = of; c0 < splits; c0 += lanes * kJoinEach) {
       float2 y[kJoinEach];
       f4 x[kJoinEach];
@@ -322,18 +341,19 @@ __global__ __launch_bounds__(kThreads) void AttendJoinKernel(const float* ml, co
     part_o[threadIdx.x] = sum;
   }
   __syncthreads();
-  if (of != 0) return;
-  float big = part_m[piece];
-  for (int i = 1; i < lanes; ++i) big = fmaxf(big, part_m[piece + i * pieces]);
+  if (!active || of != 0) return;
+  const int first = threadIdx.x;
+  float big = -INFINITY;
+  for (int i = 0; i < lanes; ++i) big = fmaxf(big, part_m[first + i * pieces]);
   const float base = big == -INFINITY ? 0.f : big;
   float total = 0.f;
   sum = f4{0.f, 0.f, 0.f, 0.f};
   for (int i = 0; i < lanes; ++i) {
-    const float w = __builtin_amdgcn_exp2f(part_m[piece + i * pieces] - base);
-    total += w * part_l[piece + i * pieces];
-    sum += w * part_o[piece + i * pieces];
+    const float w = __builtin_amdgcn_exp2f(part_m[first + i * pieces] - base);
+    total += w * part_l[first + i * pieces];
+    sum += w * part_o[first + i * pieces];
   }
-  float* dst = out + row * dim + 4 * piece;
+  float* dst = out + static_cast<int64_t>(row) * dim + 4 * piece;
   const f4 y = f4{__fdiv_rn(sum[0], total), __fdiv_rn(sum[1], total), __fdiv_rn(sum[2], total), __fdiv_rn(sum[3], total)};
   if (vec) {
     *reinterpret_cast<f4*>(dst) = y;
@@ -347,14 +367,18 @@ __global__ __launch_bounds__(kThreads) void AttendJoinKernel(const float* ml, co
 
 void LaunchAttendJoin(const AttendArgs& a, const AttendPartial& partial, int32_t splits, hipStream_t stream) {
   const bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
-  hipLaunchKernelGGL(AttendJoinKernel, dim3(static_cast<uint32_t>(a.seq) * static_cast<uint32_t>(a.heads)), dim3(kThreads), 0,
-                     stream, partial.ml, partial.o, a.out, splits, a.dim, vec);
+  const int32_t rows = a.seq * a.heads;
+  const int32_t pieces = PartialDims(a.dim) / 4;
+  const int32_t lanes = std::min(splits, kJoinThreads / pieces);
+  const int32_t per_group = kJoinThreads / (pieces * lanes);
+  hipLaunchKernelGGL(AttendJoinKernel, dim3(static_cast<uint32_t>((rows + per_group - 1) / per_group)), dim3(kJoinThreads), 0,
+                     stream, partial.ml, partial.o, a.out, rows, splits, a.dim, lanes, vec);
   Check(hipGetLastError(), "AttendJoinKernel launch");
 }
 
-AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t most) {
+AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t per_cu, int64_t most) {
   const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
-  const int64_t count = std::max<int64_t>(1, std::min<int64_t>(2 * cus / units, most));
+  const int64_t count = std::max<int64_t>(1, std::min<int64_t>(per_cu * cus / units, most));
   const int64_t parts = int64_t(a.seq) * a.heads * count;
   const size_t ml_bytes = (static_cast<size_t>(parts) * 2 * sizeof(float) + 15) & ~size_t(15);
   const size_t bytes = ml_bytes + static_cast<size_t>(parts * PartialDims(a.dim)) * sizeof(float);
@@ -369,11 +393,21 @@ AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t most) {
 namespace {
 
 template <int DP>
-void LaunchStep(const AttendArgs& a, const Q8Cache& c, int load, const AttendSplit& split, int64_t units,
-                hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(units * split.count)), block(kThreads);
+void LaunchStep(const AttendArgs& a, const Q8Cache& c, int load, hipStream_t stream) {
+  // Heads together where each wave has several steps; a short range is latency, and fewer parts to join.
+  const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
+  const int64_t group = a.heads / a.kv_heads;
+  const int64_t steps = AttendRangeSteps(a, kStepRows, kStepKeys);
+  const int64_t all = steps * a.kv_heads * ((int64_t(a.seq) * group + kStepRows - 1) / kStepRows);
+  int32_t hw = all >= 4 * cus * StepWaves(DP) ? 4 : 1;
+  while (a.kv_heads % hw != 0) --hw;
+  const int32_t sw = StepWaves(DP) / hw;
+  const int64_t units = (int64_t(a.seq) * group + kStepRows - 1) / kStepRows * (a.kv_heads / hw);
+  if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
+  const AttendSplit split = SplitRange(a, units, 1, steps / sw);
+  const dim3 grid(static_cast<uint32_t>(units * split.count)), block(64 * hw * sw);
 #define ACCEL_STEP(L, S) \
-  hipLaunchKernelGGL((AttendQ8StepKernel<DP, L, S>), grid, block, 0, stream, a, c, split.count, split.partial)
+  hipLaunchKernelGGL((AttendQ8StepKernel<DP, L, S>), grid, block, 0, stream, a, c, hw, split.count, split.partial)
   if (load == 16) {
     if (c.block_shift >= 5) ACCEL_STEP(16, 1);
     else if (c.block_shift >= 2) ACCEL_STEP(16, 2);
@@ -385,6 +419,7 @@ void LaunchStep(const AttendArgs& a, const Q8Cache& c, int load, const AttendSpl
   }
 #undef ACCEL_STEP
   Check(hipGetLastError(), "AttendQ8StepKernel launch");
+  if (split.count > 1) LaunchAttendJoin(a, split.partial, split.count, stream);
 }
 
 }  // namespace
@@ -394,19 +429,10 @@ void LaunchAttentionQ8(const AttendArgs& a, const Q8Cache& c, hipStream_t stream
     return a.dim % to == 0 && reinterpret_cast<uintptr_t>(c.k.code) % to == 0 && reinterpret_cast<uintptr_t>(c.v.code) % to == 0;
   };
   const int load = aligned(16) ? 16 : aligned(4) ? 4 : 1;
-  const int64_t group = a.heads / a.kv_heads;
-  if (int64_t(a.seq) * group > kAttendPromptRows) {
-    LaunchAttendPromptQ8(a, c, load, stream);
-    return;
-  }
-  const int64_t tiles = (int64_t(a.seq) * group + kStepRows - 1) / kStepRows;
-  const int64_t units = tiles * a.kv_heads;
-  if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
-  const AttendSplit split = SplitRange(a, units, AttendRangeSteps(a, kStepRows, kStepKeys) / kWaves);
-  if (a.dim <= 64) LaunchStep<64>(a, c, load, split, units, stream);
-  else if (a.dim <= 128) LaunchStep<128>(a, c, load, split, units, stream);
-  else LaunchStep<256>(a, c, load, split, units, stream);
-  if (split.count > 1) LaunchAttendJoin(a, split.partial, split.count, stream);
+  if (int64_t(a.seq) * (a.heads / a.kv_heads) > kAttendPromptRows) LaunchAttendPromptQ8(a, c, load, stream);
+  else if (a.dim <= 64) LaunchStep<64>(a, c, load, stream);
+  else if (a.dim <= 128) LaunchStep<128>(a, c, load, stream);
+  else LaunchStep<256>(a, c, load, stream);
 }
 
 }  // namespace accel_hip

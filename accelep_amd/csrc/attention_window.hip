@@ -23,7 +23,7 @@ constexpr int kKeys = 16;  // of a wave's step
 // A key or value row that is not finite would reach rows that do not see it, as 0 * NaN: a step that
 // holds one (a test of the bits, uniform) has its values taken as zeros and its weights as NaN.
 template <int DP, int kLoad>
-__global__ __launch_bounds__(kThreads) void AttendF32StepKernel(AttendArgs a, const float* k, const float* v,
+__global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendF32StepKernel(AttendArgs a, const float* k, const float* v,
                                                                 int32_t splits, AttendPartial partial) {
   constexpr int kI = DP / 16;  // 16-byte pieces of a key row per lane
   constexpr int kC = DP / 64;  // of a value row
@@ -52,11 +52,13 @@ __global__ __launch_bounds__(kThreads) void AttendF32StepKernel(AttendArgs a, co
   const float* vbase = v + static_cast<int64_t>(kv) * a.dim;
 
   f4 kx[kI], vx[4][kC];
+  // A piece past a head's dims reads its last (it meets a query of 0, or makes a dim that is not stored), a
+  // row past the range the last one.
   const auto piece = [&](const float* p, int d) {
-    if (kLoad == 16) return d < a.dim ? *reinterpret_cast<const f4*>(p + d) : f4{0.f, 0.f, 0.f, 0.f};
+    if (kLoad == 16) return *reinterpret_cast<const f4*>(p + min(d, a.dim - 4));
     f4 x;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = d + e < a.dim ? p[d + e] : 0.f;
+    for (int e = 0; e < 4; ++e) x[e] = p[min(d + e, a.dim - 1)];
     return x;
   };
   const auto load_k = [&](int32_t t0) {
@@ -186,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void AttendF32StepKernel(AttendArgs a, co
       *reinterpret_cast<f4*>(&parts.o[wave][j][64 * c + 16 * g + 4 * r]) =
           f4{acc[c][0][r], acc[c][1][r], acc[c][2][r], acc[c][3][r]};
   __syncthreads();
-  parts.Join(a, kv, group, r0, rows, split, splits, partial);
+  parts.Join(a, kv, 1, group, r0, rows, split, splits, partial);
 }
 
 template <int DP>
@@ -209,7 +211,7 @@ void LaunchAttentionWindow(const AttendArgs& a, const float* k, const float* v, 
   }
   const int64_t units = (int64_t(a.seq) * group + kRows - 1) / kRows * a.kv_heads;
   if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
-  const AttendSplit split = SplitRange(a, units, AttendRangeSteps(a, kRows, kKeys) / kWaves);
+  const AttendSplit split = SplitRange(a, units, 2, AttendRangeSteps(a, kRows, kKeys) / kWaves);
   if (a.dim <= 64) LaunchStep<64>(a, k, v, vec, split, units, stream);
   else if (a.dim <= 128) LaunchStep<128>(a, k, v, vec, split, units, stream);
   else LaunchStep<256>(a, k, v, vec, split, units, stream);

@@ -15,6 +15,7 @@ namespace {
 constexpr int64_t kMaxHeadDim = 256;
 constexpr int64_t kMaxBlock = 256;
 constexpr int64_t kMaxRows = 0x7fffffff - 256;  // positions and row counts are 32-bit in the kernels
+constexpr int64_t kMaxKvRow = 1 << 24;           // and a step's offsets from its first key row
 constexpr double kTwoPi = 6.283185307179586476925286766559;
 
 void Invalid(const char* what) { Fail(ACCEL_HIP_INVALID_ARGUMENT, what); }
@@ -77,7 +78,7 @@ Q8Cache CheckedCache(const AccelHipCacheQ8* c) {
 // Everything of the two attention calls but the cache. False: nothing to do.
 bool CheckedAttend(const AccelHipBuffer& q, const AccelHipBuffer& out, int64_t seq, int64_t position, int64_t heads,
                    int64_t kv_heads, int64_t dim, int64_t row_stride, int64_t window, int64_t sinks, AttendArgs* a) {
-  if (kv_heads <= 0 || (heads > 0 && heads % kv_heads != 0)) Invalid("Attention kv heads are out of range");
+  if (kv_heads <= 0 || kv_heads > kMaxRows || (heads > 0 && heads % kv_heads != 0)) Invalid("Attention kv heads are out of range");
   if (window < 0 || sinks < 0) Invalid("Attention window is out of range");
   if (heads < 0 || dim < 0) Invalid("negative matrix dimension");
   if (dim > kMaxHeadDim) Invalid("Attention head_dim must be in 1..256");
@@ -91,6 +92,7 @@ bool CheckedAttend(const AccelHipBuffer& q, const AccelHipBuffer& out, int64_t s
   RequireAligned(q, sizeof(float), "Attention query is not aligned");
   RequireAligned(out, sizeof(float), "Attention output is not aligned");
   if (Overlap(q, q_bytes, out, out_bytes)) Invalid("Attention output overlaps the query");
+  if (kv_heads * dim > kMaxKvRow) Invalid("Attention is too large");
   if (seen > kMaxRows || (heads > 0 && seq > kMaxRows / heads)) Invalid("Attention is too large");
   a->q = static_cast<const float*>(q.data);
   a->out = static_cast<float*>(out.data);
