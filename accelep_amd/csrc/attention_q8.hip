@@ -9,7 +9,7 @@
 namespace accel_hip {
 namespace {
 
-// Waves of a step workgroup at most: 8, and 4 where a head's 256 dims leave one wave a SIMD.
+// Waves of a step workgroup at most: what a CU's registers hold.
 constexpr int StepWaves(int dp) { return dp > 128 ? 4 : 8; }
 constexpr int kStepRows = 16;
 constexpr int kStepKeys = 32;
@@ -26,7 +26,7 @@ constexpr int kStepKeys = 32;
 //    the lane loads at V[key][DP / 16 * j], transposed in registers.
 // The next step's keys are requested after the scores, its values after the sums.
 template <int DP, int kLoad, int kScales>
-__global__ __launch_bounds__(64 * StepWaves(DP), DP > 128 ? 1 : 2) void AttendQ8StepKernel(
+__global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
     AttendArgs a, Q8Cache c, int32_t hw, int32_t splits, AttendPartial partial) {
   constexpr int kC = DP / 64;       // 16-byte pieces of a key row per lane
   constexpr int kTiles = DP / 16;   // dim tiles
@@ -392,34 +392,35 @@ AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t per_cu, int64
 
 namespace {
 
-template <int DP>
-void LaunchStep(const AttendArgs& a, const Q8Cache& c, int load, hipStream_t stream) {
-  // Heads together where each wave has several steps; a short range is latency, and fewer parts to join.
+template <int DP, int kLoad, int kScales>
+void LaunchStep(const AttendArgs& a, const Q8Cache& c, hipStream_t stream) {
+  constexpr int kWaves = StepWaves(DP);
   const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
   const int64_t group = a.heads / a.kv_heads;
+  const int64_t tiles = (int64_t(a.seq) * group + kStepRows - 1) / kStepRows;
   const int64_t steps = AttendRangeSteps(a, kStepRows, kStepKeys);
-  const int64_t all = steps * a.kv_heads * ((int64_t(a.seq) * group + kStepRows - 1) / kStepRows);
-  int32_t hw = all >= 4 * cus * StepWaves(DP) ? 4 : 1;
+  // Heads together where each wave has several steps; a short range is latency, and fewer parts to join.
+  int32_t hw = steps * a.kv_heads * tiles >= 4 * cus * kWaves ? 4 : 1;
   while (a.kv_heads % hw != 0) --hw;
-  const int32_t sw = StepWaves(DP) / hw;
-  const int64_t units = (int64_t(a.seq) * group + kStepRows - 1) / kStepRows * (a.kv_heads / hw);
+  const int64_t units = tiles * (a.kv_heads / hw);
   if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
-  const AttendSplit split = SplitRange(a, units, 1, steps / sw);
-  const dim3 grid(static_cast<uint32_t>(units * split.count)), block(64 * hw * sw);
-#define ACCEL_STEP(L, S) \
-  hipLaunchKernelGGL((AttendQ8StepKernel<DP, L, S>), grid, block, 0, stream, a, c, hw, split.count, split.partial)
-  if (load == 16) {
-    if (c.block_shift >= 5) ACCEL_STEP(16, 1);
-    else if (c.block_shift >= 2) ACCEL_STEP(16, 2);
-    else ACCEL_STEP(16, 8);
-  } else if (load == 4) {
-    ACCEL_STEP(4, 8);
-  } else {
-    ACCEL_STEP(1, 8);
-  }
-#undef ACCEL_STEP
+  // Steps that do not fill the CUs are spread one wave a SIMD (2048 keys, 9 heads of 64: 7.6 us in
+  // workgroups of four waves, 9.0 of eight, 14.2 in one of sixteen a key head).
+  const int32_t sw = hw == 1 && units * steps < cus * kWaves ? 4 : kWaves / hw;
+  const AttendSplit split = SplitRange(a, units, 1, steps <= 2 * sw ? 1 : steps / sw);
+  hipLaunchKernelGGL((AttendQ8StepKernel<DP, kLoad, kScales>), dim3(static_cast<uint32_t>(units * split.count)),
+                     dim3(64 * hw * sw), 0, stream, a, c, hw, split.count, split.partial);
   Check(hipGetLastError(), "AttendQ8StepKernel launch");
   if (split.count > 1) LaunchAttendJoin(a, split.partial, split.count, stream);
+}
+
+template <int DP>
+void LaunchStepOf(const AttendArgs& a, const Q8Cache& c, int load, hipStream_t stream) {
+  if (load == 1) LaunchStep<DP, 1, 8>(a, c, stream);
+  else if (load == 4) LaunchStep<DP, 4, 8>(a, c, stream);
+  else if (c.block_shift >= 5) LaunchStep<DP, 16, 1>(a, c, stream);
+  else if (c.block_shift >= 2) LaunchStep<DP, 16, 2>(a, c, stream);
+  else LaunchStep<DP, 16, 8>(a, c, stream);
 }
 
 }  // namespace
@@ -430,9 +431,9 @@ void LaunchAttentionQ8(const AttendArgs& a, const Q8Cache& c, hipStream_t stream
   };
   const int load = aligned(16) ? 16 : aligned(4) ? 4 : 1;
   if (int64_t(a.seq) * (a.heads / a.kv_heads) > kAttendPromptRows) LaunchAttendPromptQ8(a, c, load, stream);
-  else if (a.dim <= 64) LaunchStep<64>(a, c, load, stream);
-  else if (a.dim <= 128) LaunchStep<128>(a, c, load, stream);
-  else LaunchStep<256>(a, c, load, stream);
+  else if (a.dim <= 64) LaunchStepOf<64>(a, c, load, stream);
+  else if (a.dim <= 128) LaunchStepOf<128>(a, c, load, stream);
+  else LaunchStepOf<256>(a, c, load, stream);
 }
 
 }  // namespace accel_hip

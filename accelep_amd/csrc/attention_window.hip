@@ -7,12 +7,12 @@
 namespace accel_hip {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
+// Waves of a workgroup: what a CU's registers hold.
+constexpr int StepWaves(int dp) { return dp > 128 ? 4 : 8; }
 constexpr int kRows = 16;
 constexpr int kKeys = 16;  // of a wave's step
 
-// One workgroup per (16 rows of a key head, key range); its waves take every fourth step of 16 keys.
+// One workgroup per (16 rows of a key head, key range); its waves take its steps of 16 keys in turn.
 // Bound: the bytes of the keys that are seen. Both products run on v_mfma_f32_16x16x4f32, which takes
 // fp32 as it is, with every operand straight from memory. Lane (j, g) = (lane % 16, lane / 16):
 //  * S^T = K Q^T: k slot g of instruction (i, e) is dim 16i + 4g + e, so a lane loads 16 bytes of key
@@ -23,11 +23,12 @@ constexpr int kKeys = 16;  // of a wave's step
 // A key or value row that is not finite would reach rows that do not see it, as 0 * NaN: a step that
 // holds one (a test of the bits, uniform) has its values taken as zeros and its weights as NaN.
 template <int DP, int kLoad>
-__global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendF32StepKernel(AttendArgs a, const float* k, const float* v,
-                                                                int32_t splits, AttendPartial partial) {
+__global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
+    AttendArgs a, const float* k, const float* v, int32_t splits, AttendPartial partial) {
+  const int32_t waves = static_cast<int32_t>(blockDim.x) / 64;
   constexpr int kI = DP / 16;  // 16-byte pieces of a key row per lane
   constexpr int kC = DP / 64;  // of a value row
-  __shared__ __align__(16) WaveParts<DP, kWaves, kRows> parts;
+  __shared__ __align__(16) WaveParts<DP, StepWaves(DP), kRows> parts;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -99,9 +100,9 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendF32StepKerne
   for (int c = 0; c < kC; ++c)
 #pragma unroll
     for (int t = 0; t < 4; ++t) acc[c][t] = f4{0.f, 0.f, 0.f, 0.f};
-  for (; u < end; u += kWaves) {  // uniform over the wave
+  for (; u < end; u += waves) {  // uniform over the wave
     const int32_t t0 = range.Key(u);
-    const int32_t next = u + kWaves < end ? range.Key(u + kWaves) : -1;
+    const int32_t next = u + waves < end ? range.Key(u + waves) : -1;
     f4 st0 = f4{0.f, 0.f, 0.f, 0.f}, st1 = st0;
     uint32_t top = 0;
 #pragma unroll
@@ -192,30 +193,31 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendF32StepKerne
 }
 
 template <int DP>
-void LaunchStep(const AttendArgs& a, const float* k, const float* v, bool vec, const AttendSplit& split,
-                int64_t units, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(units * split.count)), block(kThreads);
+void LaunchStep(const AttendArgs& a, const float* k, const float* v, bool vec, hipStream_t stream) {
+  constexpr int kWaves = StepWaves(DP);
+  const int64_t group = a.heads / a.kv_heads;
+  const int64_t units = (int64_t(a.seq) * group + kRows - 1) / kRows * a.kv_heads;
+  if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
+  const int64_t steps = AttendRangeSteps(a, kRows, kKeys);
+  // Steps that do not fill the CUs are spread one wave a SIMD.
+  const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
+  const int32_t waves = units * steps < cus * kWaves ? 4 : kWaves;
+  const AttendSplit split = SplitRange(a, units, 1, steps <= 2 * waves ? 1 : steps / waves);
+  const dim3 grid(static_cast<uint32_t>(units * split.count)), block(64 * waves);
   if (vec) hipLaunchKernelGGL((AttendF32StepKernel<DP, 16>), grid, block, 0, stream, a, k, v, split.count, split.partial);
   else hipLaunchKernelGGL((AttendF32StepKernel<DP, 4>), grid, block, 0, stream, a, k, v, split.count, split.partial);
   Check(hipGetLastError(), "AttendF32StepKernel launch");
+  if (split.count > 1) LaunchAttendJoin(a, split.partial, split.count, stream);
 }
 
 }  // namespace
 
 void LaunchAttentionWindow(const AttendArgs& a, const float* k, const float* v, hipStream_t stream) {
   const bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0;
-  const int64_t group = a.heads / a.kv_heads;
-  if (int64_t(a.seq) * group > kAttendPromptRows) {
-    LaunchAttendPromptF32(a, k, v, vec ? 16 : 4, stream);
-    return;
-  }
-  const int64_t units = (int64_t(a.seq) * group + kRows - 1) / kRows * a.kv_heads;
-  if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
-  const AttendSplit split = SplitRange(a, units, 2, AttendRangeSteps(a, kRows, kKeys) / kWaves);
-  if (a.dim <= 64) LaunchStep<64>(a, k, v, vec, split, units, stream);
-  else if (a.dim <= 128) LaunchStep<128>(a, k, v, vec, split, units, stream);
-  else LaunchStep<256>(a, k, v, vec, split, units, stream);
-  if (split.count > 1) LaunchAttendJoin(a, split.partial, split.count, stream);
+  if (int64_t(a.seq) * (a.heads / a.kv_heads) > kAttendPromptRows) LaunchAttendPromptF32(a, k, v, vec ? 16 : 4, stream);
+  else if (a.dim <= 64) LaunchStep<64>(a, k, v, vec, stream);
+  else if (a.dim <= 128) LaunchStep<128>(a, k, v, vec, stream);
+  else LaunchStep<256>(a, k, v, vec, stream);
 }
 
 }  // namespace accel_hip
