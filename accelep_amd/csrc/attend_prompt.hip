@@ -217,6 +217,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       for (int h = 0; h < kSub; ++h)
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[h][r] = 0.f;
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int step = 0; step < kSteps; ++step)
 #pragma unroll
@@ -229,6 +230,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
             st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8l, qh[step], st[h], 0, 0, 0);
           }
         }
+      __builtin_amdgcn_s_setprio(0);
       float c = row_factor;
       if (kUniform) {
         c *= ks;
@@ -332,6 +334,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
           for (int r = 0; r < 16; ++r) st[h][r] = ldexpf(st[h][r], power);
       }
       // O^T += V^T P^T, 16 keys at a time.
+      __builtin_amdgcn_s_setprio(1);
       const _Float16* vrow = &vt[buf][0][4 * g + ((lane & 15) >> 2)][16 * ((lane >> 4) & 1) + 4 * (lane & 3)];
 #pragma unroll
       for (int h = 0; h < kSub; ++h)
@@ -356,6 +359,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
           }
         }
     }
+    __builtin_amdgcn_s_setprio(0);
     if (u + 1 < end) {
       put(buf ^ 1);
       ks = ks_next;
