@@ -10,8 +10,10 @@
 //  * O^T += V^T P^T: those scores are the lane's own k-slots of P^T if slot e of 16 keys is key
 //    (e % 4) + 8 (e / 4) + 4g, and the value operand is read transposed from the row-major tile
 //    (ds_read_b64_tr_b16 gives a lane four keys of one dim).
-// An fp32 row enters as its parts times a power of two, that of its largest magnitude, which takes the
-// place of a block's scale; a row that is not finite gets a NaN in its place and zeros as values.
+// An fp32 row enters as its parts times a power of two, whose inverse takes the place of a block's scale:
+// 2^9 for rows whose largest magnitude lies in [2^-6, 2^6) (or that are zero), which keeps 22 bits of all
+// of them, and a tile of such rows has one scale; otherwise one from the row's own largest magnitude. A
+// row that is not finite has a NaN for a scale and zeros for values.
 #include "attend_common.h"
 
 namespace accel_hip {
@@ -20,6 +22,8 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kWaveRows = 32;
+constexpr float kCommonScale = 0x1p9f;
+constexpr uint32_t kCommonLow = 121u << 23, kCommonHigh = 133u << 23;  // bits of 2^-6 and 2^6
 constexpr int kRows = kWaves * kWaveRows;
 typedef short s4 __attribute__((ext_vector_type(4)));
 
@@ -48,6 +52,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   __shared__ __align__(16) _Float16 vt[2][kParts][kKeys][kVStride];
   __shared__ __align__(16) float sk[2][kKeys];
   __shared__ __align__(16) float sv[2][kKeys];
+  __shared__ int odd[3];  // fp32: the tile has rows of scales of their own
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -118,25 +123,40 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   };
   // Writes a thread's pieces of one plane; tile row `key` begins at dst + key * stride, its second part
   // `part` halves later.
-  const auto put_plane = [&](const uint4 (&x)[kChunks], _Float16* dst, int stride, int part, float* scales) {
+  const auto put_plane = [&](uint4 (&x)[kChunks], _Float16* dst, int stride, int part, float* scales, int slot) {
     if (kF32) {
-      uint32_t top = 0;
+      // The row's largest magnitude: of the bits as signed numbers for its positive values, as unsigned
+      // ones for its negative.
+      int32_t pos = 0;
+      uint32_t neg = 0;
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i)
-        top = max(max(top, max(x[i].x & 0x7fffffffu, x[i].y & 0x7fffffffu)), max(x[i].z & 0x7fffffffu, x[i].w & 0x7fffffffu));
+      for (int i = 0; i < kChunks; ++i) {
+        pos = max(max(pos, max(static_cast<int32_t>(x[i].x), static_cast<int32_t>(x[i].y))),
+                  max(static_cast<int32_t>(x[i].z), static_cast<int32_t>(x[i].w)));
+        neg = max(max(neg, max(x[i].x, x[i].y)), max(x[i].z, x[i].w));
+      }
+      uint32_t top = max(static_cast<uint32_t>(pos), neg & 0x7fffffffu);
       top = max(top, XorLane<1>(top));
       top = max(top, XorLane<2>(top));
       top = max(top, XorLane<4>(top));
-      const bool bad = top >= 0x7f800000u;
-      const float scale = bad ? 0.f : RowScale(top);
-      if (tid % 8 == 0) scales[tid / 8] = bad ? NAN : 1.f / scale;
+      float scale = kCommonScale, back = 1.f / kCommonScale;
+      const bool common = top == 0 || (top >= kCommonLow && top < kCommonHigh);
+      if (!__all(common)) {
+        odd[slot] = 1;
+        const bool bad = top >= 0x7f800000u;
+        scale = RowScale(top);
+        back = bad ? NAN : 1.f / scale;
+        if (bad) {
+#pragma unroll
+          for (int i = 0; i < kChunks; ++i) x[i] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (tid % 8 == 0) scales[tid / 8] = back;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        const float f0 = bad ? 0.f : __uint_as_float(x[i].x) * scale, f1 = bad ? 0.f : __uint_as_float(x[i].y) * scale;
-        const float f2 = bad ? 0.f : __uint_as_float(x[i].z) * scale, f3 = bad ? 0.f : __uint_as_float(x[i].w) * scale;
         h2 h0, l0, h1, l1;
-        SplitF16(f0, f1, h0, l0);
-        SplitF16(f2, f3, h1, l1);
+        SplitF16(__uint_as_float(x[i].x) * scale, __uint_as_float(x[i].y) * scale, h0, l0);
+        SplitF16(__uint_as_float(x[i].z) * scale, __uint_as_float(x[i].w) * scale, h1, l1);
         _Float16* p = dst + (tid / 8) * stride + 4 * (tid % 8 + 8 * i);
         *reinterpret_cast<h4*>(p) = h4{h0[0], h0[1], h1[0], h1[1]};
         *reinterpret_cast<h4*>(p + part) = h4{l0[0], l0[1], l1[0], l1[1]};
@@ -153,9 +173,9 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       }
     }
   };
-  const auto put = [&](int buf) {
-    put_plane(kreg, &kt[buf][0][0][0], kKStride, kKeys * kKStride, sk[buf]);
-    put_plane(vreg, &vt[buf][0][0][0], kVStride, kKeys * kVStride, sv[buf]);
+  const auto put = [&](int buf, int slot) {
+    put_plane(kreg, &kt[buf][0][0][0], kKStride, kKeys * kKStride, sk[buf], slot);
+    put_plane(vreg, &vt[buf][0][0][0], kVStride, kKeys * kVStride, sv[buf], slot);
     if (!kF32 && !kUniform && tid < kKeys) {
       sk[buf][tid] = ks_next;
       sv[buf][tid] = vs_next;
@@ -201,11 +221,14 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
     for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
 
   float ks = ks_next, vs = vs_next;
-  if (begin < end) put(0);
+  if (tid < 3) odd[tid] = 0;
+  __syncthreads();
+  if (begin < end) put(0, 0);
   for (int32_t u = begin; u < end; ++u) {
     const int buf = (u - begin) & 1;
     const int32_t t0 = range.Key(u);
     __syncthreads();
+    if (kF32 && tid == 0) odd[(u + 2 - begin) % 3] = 0;  // next written behind the next barrier
     if (u + 1 < end) fetch(range.Key(u + 1));
     __builtin_amdgcn_sched_barrier(0);
     const int32_t last = t0 + kKeys - 1;
@@ -231,10 +254,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
           }
         }
       __builtin_amdgcn_s_setprio(0);
-      float c = row_factor;
-      if (kUniform) {
-        c *= ks;
-      } else {
+      const bool one_scale = kUniform || (kF32 && odd[(u - begin) % 3] == 0);  // uniform
+      if (!one_scale) {
 #pragma unroll
         for (int h = 0; h < kSub; ++h)
 #pragma unroll
@@ -244,6 +265,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
             for (int e = 0; e < 4; ++e) st[h][4 * r4 + e] *= f[e];
           }
       }
+      float c = row_factor;
+      if (one_scale) c *= kF32 ? 1.f / kCommonScale : ks;
       uint32_t seen[kSub];
       if (!whole) {
 #pragma unroll
@@ -279,9 +302,10 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
         }
       l = l * corr + sum;
       // The weights times the values' scales, and their largest.
+      const float v_scale = kF32 ? 1.f / kCommonScale : vs;
       float tile_top = 0.f;
-      if (kUniform) {
-        tile_top = __builtin_amdgcn_exp2f(mx - base) * vs;
+      if (one_scale) {
+        tile_top = __builtin_amdgcn_exp2f(mx - base) * v_scale;
       } else {
 #pragma unroll
         for (int h = 0; h < kSub; ++h)
@@ -308,20 +332,20 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[t][r] *= again;
       }
-      if (kUniform) {
-        const float f = ldexpf(vs, power);
-        if (__any(!(f < 0x1p100f))) {  // a block that is far larger than the sum so far: in two steps
+      if (one_scale) {
+        const float f = ldexpf(v_scale, power);
+        if (!kF32 && __any(!(f < 0x1p100f))) {  // a block that is far larger than the sum so far: in two steps
 #pragma unroll
           for (int h = 0; h < kSub; ++h)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) st[h][r] = ldexpf(st[h][r] * vs, power);
+            for (int r = 0; r < 16; ++r) st[h][r] = ldexpf(st[h][r] * v_scale, power);
         } else {
 #pragma unroll
           for (int h = 0; h < kSub; ++h)
 #pragma unroll
             for (int r = 0; r < 16; ++r) st[h][r] *= f;
         }
-        if (!whole) {
+        if (!kF32 && !whole) {  // a scale may be NaN
 #pragma unroll
           for (int h = 0; h < kSub; ++h)
 #pragma unroll
@@ -361,7 +385,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
     }
     __builtin_amdgcn_s_setprio(0);
     if (u + 1 < end) {
-      put(buf ^ 1);
+      put(buf ^ 1, (u + 1 - begin) % 3);
       ks = ks_next;
       vs = vs_next;
     }
