@@ -46,7 +46,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   constexpr int kSteps = DP / 16;
   constexpr int kDims = DP / 32;
   constexpr int kKStride = DP + 8;   // halves: 8 key rows' 16-byte pieces fall into different banks
-  constexpr int kVStride = DP + 16;  // and so do 4 key rows' 32-byte pieces
+  constexpr int kVStride = DP + 32;  // and so do 4 key rows' 64-byte pieces (two tile reads)
   constexpr int kChunks = kF32 ? DP / 32 : kKeys * DP / 16 / kThreads;  // 16-byte pieces of a plane a thread stages
   __shared__ __align__(16) _Float16 kt[2][kParts][kKeys][kKStride];
   __shared__ __align__(16) _Float16 vt[2][kParts][kKeys][kVStride];
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       const float* p = static_cast<const float*>(base) + min(t0 + tid / 8, range.high - 1) * kv_row + static_cast<int64_t>(kv) * a.dim;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        const int d = 4 * (tid % 8 + 8 * i);
+        const int d = 8 * (tid % 8 + 8 * (i / 2)) + 4 * (i % 2);
         if (kLoad == 16) {
           x[i] = *reinterpret_cast<const uint4*>(p + min(d, a.dim - 4));
         } else {
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   };
   // Writes a thread's pieces of one plane; tile row `key` begins at dst + key * stride, its second part
   // `part` halves later.
-  const auto put_plane = [&](uint4 (&x)[kChunks], _Float16* dst, int stride, int part, float* scales, int slot) {
+  const auto put_plane = [&](const uint4 (&x)[kChunks], _Float16* dst, int stride, int part, float* scales, int slot) {
     if (kF32) {
       // The row's largest magnitude: of the bits as signed numbers for its positive values, as unsigned
       // ones for its negative.
@@ -143,23 +143,26 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       const bool common = top == 0 || (top >= kCommonLow && top < kCommonHigh);
       if (!__all(common)) {
         odd[slot] = 1;
-        const bool bad = top >= 0x7f800000u;
         scale = RowScale(top);
-        back = bad ? NAN : 1.f / scale;
-        if (bad) {
-#pragma unroll
-          for (int i = 0; i < kChunks; ++i) x[i] = make_uint4(0, 0, 0, 0);
-        }
+        back = top >= 0x7f800000u ? NAN : 1.f / scale;
       }
       if (tid % 8 == 0) scales[tid / 8] = back;
+      h8* p = reinterpret_cast<h8*>(dst + (tid / 8) * stride + 8 * (tid % 8));
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        h2 h0, l0, h1, l1;
-        SplitF16(__uint_as_float(x[i].x) * scale, __uint_as_float(x[i].y) * scale, h0, l0);
-        SplitF16(__uint_as_float(x[i].z) * scale, __uint_as_float(x[i].w) * scale, h1, l1);
-        _Float16* p = dst + (tid / 8) * stride + 4 * (tid % 8 + 8 * i);
-        *reinterpret_cast<h4*>(p) = h4{h0[0], h0[1], h1[0], h1[1]};
-        *reinterpret_cast<h4*>(p + part) = h4{l0[0], l0[1], l1[0], l1[1]};
+      for (int i = 0; i < kChunks; i += 2) {
+        const uint4 a0 = x[i], a1 = x[i + 1];
+        h2 hi[4], lo[4];
+        SplitF16(__uint_as_float(a0.x) * scale, __uint_as_float(a0.y) * scale, hi[0], lo[0]);
+        SplitF16(__uint_as_float(a0.z) * scale, __uint_as_float(a0.w) * scale, hi[1], lo[1]);
+        SplitF16(__uint_as_float(a1.x) * scale, __uint_as_float(a1.y) * scale, hi[2], lo[2]);
+        SplitF16(__uint_as_float(a1.z) * scale, __uint_as_float(a1.w) * scale, hi[3], lo[3]);
+        p[4 * i] = Join(hi[0], hi[1], hi[2], hi[3]);
+        p[4 * i + part / 8] = Join(lo[0], lo[1], lo[2], lo[3]);
+      }
+      if (top >= 0x7f800000u) {  // written again: zeros
+        const _Float16 z = 0;
+#pragma unroll
+        for (int i = 0; i < kChunks; i += 2) p[4 * i] = p[4 * i + part / 8] = h8{z, z, z, z, z, z, z, z};
       }
     } else {
 #pragma unroll
