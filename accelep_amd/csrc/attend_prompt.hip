@@ -123,7 +123,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   };
   // Writes a thread's pieces of one plane; tile row `key` begins at dst + key * stride, its second part
   // `part` halves later.
-  const auto put_plane = [&](const uint4 (&x)[kChunks], _Float16* dst, int stride, int part, float* scales, int slot) {
+  const auto put_plane = [&](const uint4 (&x)[kChunks], _Float16* dst, int stride, int part, float& row_back, int slot) {
     if (kF32) {
       // The row's largest magnitude: of the bits as signed numbers for its positive values, as unsigned
       // ones for its negative.
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
         scale = RowScale(top);
         back = top >= 0x7f800000u ? NAN : 1.f / scale;
       }
-      if (tid % 8 == 0) scales[tid / 8] = back;
+      row_back = back;
       h8* p = reinterpret_cast<h8*>(dst + (tid / 8) * stride + 8 * (tid % 8));
 #pragma unroll
       for (int i = 0; i < kChunks; i += 2) {
@@ -176,12 +176,30 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       }
     }
   };
+  // A value scale that is not finite moves to its keys, as NaN: the scores of the rows that see them are
+  // NaN then, and a weight of 0 stays one.
+  const auto move_nan = [](float& key, float& value) {
+    if (!(fabsf(value) < INFINITY)) {
+      key = NAN;
+      value = 0.f;
+    }
+  };
   const auto put = [&](int buf, int slot) {
-    put_plane(kreg, &kt[buf][0][0][0], kKStride, kKeys * kKStride, sk[buf], slot);
-    put_plane(vreg, &vt[buf][0][0][0], kVStride, kKeys * kVStride, sv[buf], slot);
-    if (!kF32 && !kUniform && tid < kKeys) {
-      sk[buf][tid] = ks_next;
-      sv[buf][tid] = vs_next;
+    float k_back = 1.f, v_back = 1.f;
+    put_plane(kreg, &kt[buf][0][0][0], kKStride, kKeys * kKStride, k_back, slot);
+    put_plane(vreg, &vt[buf][0][0][0], kVStride, kKeys * kVStride, v_back, slot);
+    if (kF32) {
+      move_nan(k_back, v_back);
+      if (tid % 8 == 0) {
+        sk[buf][tid / 8] = k_back;
+        sv[buf][tid / 8] = v_back;
+      }
+    } else {
+      move_nan(ks_next, vs_next);
+      if (!kUniform && tid < kKeys) {
+        sk[buf][tid] = ks_next;
+        sv[buf][tid] = vs_next;
+      }
     }
   };
   if (begin < end) fetch(range.Key(begin));
@@ -223,10 +241,10 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
 
-  float ks = ks_next, vs = vs_next;
   if (tid < 3) odd[tid] = 0;
   __syncthreads();
   if (begin < end) put(0, 0);
+  float ks = ks_next, vs = vs_next;
   for (int32_t u = begin; u < end; ++u) {
     const int buf = (u - begin) & 1;
     const int32_t t0 = range.Key(u);
@@ -270,18 +288,12 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       }
       float c = row_factor;
       if (one_scale) c *= kF32 ? 1.f / kCommonScale : ks;
-      uint32_t seen[kSub];
       if (!whole) {
 #pragma unroll
-        for (int h = 0; h < kSub; ++h) {
-          seen[h] = 0;
+        for (int h = 0; h < kSub; ++h)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const bool in = Sees(a, p_row, t0 + 32 * h + (r & 3) + 8 * (r >> 2) + 4 * g);
-            seen[h] |= in ? 1u << r : 0u;
-            st[h][r] = in ? st[h][r] * c : -INFINITY;
-          }
-        }
+          for (int r = 0; r < 16; ++r)
+            st[h][r] = Sees(a, p_row, t0 + 32 * h + (r & 3) + 8 * (r >> 2) + 4 * g) ? st[h][r] * c : -INFINITY;
         c = 1.f;
       }
       float mx = -INFINITY;
@@ -317,10 +329,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
             const f4 f = *reinterpret_cast<const f4*>(&sv[buf][32 * h + 8 * r4 + 4 * g]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float x = st[h][4 * r4 + e] * f[e];
-              if (!whole) x = seen[h] >> (4 * r4 + e) & 1 ? x : 0.f;
-              st[h][4 * r4 + e] = x;
-              tile_top = fmaxf(tile_top, fabsf(x));
+              st[h][4 * r4 + e] *= f[e];
+              tile_top = fmaxf(tile_top, fabsf(st[h][4 * r4 + e]));
             }
           }
         tile_top = fmaxf(tile_top, XorLane<32>(tile_top));
@@ -347,12 +357,6 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
           for (int h = 0; h < kSub; ++h)
 #pragma unroll
             for (int r = 0; r < 16; ++r) st[h][r] *= f;
-        }
-        if (!kF32 && !whole) {  // a scale may be NaN
-#pragma unroll
-          for (int h = 0; h < kSub; ++h)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) st[h][r] = seen[h] >> r & 1 ? st[h][r] : 0.f;
         }
       } else {
 #pragma unroll

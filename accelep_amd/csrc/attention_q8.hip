@@ -157,8 +157,10 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
     for (int h = 0; h < kGroups; ++h)
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
-        factor[h][e] = row_factor * ks[h][e];
-        value[h][e] = vs[h][e];
+        // A value scale that is not finite makes the scores NaN, and a weight of 0 stays one.
+        const bool finite = fabsf(vs[h][e]) < INFINITY;
+        factor[h][e] = finite ? row_factor * ks[h][e] : NAN;
+        value[h][e] = finite ? vs[h][e] : 0.f;
       }
     if (next >= 0) {
       load_k(next);
@@ -168,20 +170,14 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
     // Scores, and the row's largest. The reference m moves only when a score passes it by 2^8, so the
     // sums are seldom scaled.
     const bool whole = range.Whole(a, t0);  // a row past the last may see what it likes
-    uint32_t seen = 255;
-    if (!whole) {
-      seen = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        seen |= Sees(a, p_row, t0 + (e & 4) * 4 + 4 * g + (e & 3)) ? 1u << e : 0u;
-    }
     float p[8];
     float mx = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) p[e] = st[e >> 2][e & 3] * factor[(e >> 2) % kGroups][(e & 3) % kEach];
     if (!whole) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] = seen >> e & 1 ? p[e] : -INFINITY;
+      for (int e = 0; e < 8; ++e)
+        p[e] = Sees(a, p_row, t0 + (e & 4) * 4 + 4 * g + (e & 3)) ? p[e] : -INFINITY;
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) mx = fmaxf(mx, p[e]);
@@ -206,7 +202,6 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         p[e] *= value[(e >> 2) % kGroups][(e & 3) % kEach];
-        if (!whole) p[e] = seen >> e & 1 ? p[e] : 0.f;
         step_top = fmaxf(step_top, fabsf(p[e]));
       }
       step_top = fmaxf(step_top, XorLane<16>(step_top));
@@ -228,10 +223,6 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) p[e] *= f;
-      }
-      if (!whole) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = seen >> e & 1 ? p[e] : 0.f;
       }
     } else {
 #pragma unroll
