@@ -263,17 +263,21 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
         for (int r = 0; r < 16; ++r) st[h][r] = 0.f;
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int step = 0; step < kSteps; ++step)
+      for (int step = 0; step < kSteps; ++step) {
+        // Neighbouring instructions add to different sums.
+        h8 k8[kSub];
 #pragma unroll
         for (int h = 0; h < kSub; ++h) {
-          const h8 k8 = *reinterpret_cast<const h8*>(&kt[buf][0][32 * h + j][16 * step + 8 * g]);
-          st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qh[step], st[h], 0, 0, 0);
-          st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[step], st[h], 0, 0, 0);
-          if (kF32) {
-            const h8 k8l = *reinterpret_cast<const h8*>(&kt[buf][kParts - 1][32 * h + j][16 * step + 8 * g]);
-            st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8l, qh[step], st[h], 0, 0, 0);
-          }
+          k8[h] = *reinterpret_cast<const h8*>(&kt[buf][0][32 * h + j][16 * step + 8 * g]);
+          st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[h], qh[step], st[h], 0, 0, 0);
         }
+#pragma unroll
+        for (int h = 0; h < kSub; ++h) st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[h], ql[step], st[h], 0, 0, 0);
+        if (kF32) {
+          const h8 k8l = *reinterpret_cast<const h8*>(&kt[buf][kParts - 1][j][16 * step + 8 * g]);
+          st[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8l, qh[step], st[0], 0, 0, 0);
+        }
+      }
       __builtin_amdgcn_s_setprio(0);
       const bool one_scale = kUniform || (kF32 && odd[(u - begin) % 3] == 0);  // uniform
       if (!one_scale) {
@@ -376,17 +380,22 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
           for (int e = 0; e < 4; ++e) SplitF16(st[h][8 * k16 + 2 * e], st[h][8 * k16 + 2 * e + 1], hi[e], lo[e]);
           const h8 ph = Join(hi[0], hi[1], hi[2], hi[3]), pl = Join(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
-          for (int t = 0; t < kDims; ++t) {
-            const auto read = [&](int part) {
+          for (int t0 = 0; t0 < kDims; t0 += 2) {
+            const auto read = [&](int t, int part) {
               const _Float16* p = vrow + part * kKeys * kVStride + (32 * h + 16 * k16) * kVStride + 32 * t;
               const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
               const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p + 8 * kVStride));
               return __builtin_bit_cast(h8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
             };
-            const h8 v8 = read(0);
-            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph, acc[t], 0, 0, 0);
-            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl, acc[t], 0, 0, 0);
-            if (kF32) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read(kParts - 1), ph, acc[t], 0, 0, 0);
+            const h8 v0 = read(t0, 0), v1 = read(t0 + 1, 0);
+            acc[t0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, ph, acc[t0], 0, 0, 0);
+            acc[t0 + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, ph, acc[t0 + 1], 0, 0, 0);
+            acc[t0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pl, acc[t0], 0, 0, 0);
+            acc[t0 + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, pl, acc[t0 + 1], 0, 0, 0);
+            if (kF32) {
+              acc[t0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read(t0, kParts - 1), ph, acc[t0], 0, 0, 0);
+              acc[t0 + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read(t0 + 1, kParts - 1), ph, acc[t0 + 1], 0, 0, 0);
+            }
           }
         }
     }
