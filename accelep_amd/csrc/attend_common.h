@@ -138,8 +138,19 @@ inline int64_t AttendRangeSteps(const AttendArgs& a, int64_t rows, int64_t step)
 
 // Bytes (or floats) of a key row, all heads, up to which a step's rows lie within 32-bit offsets.
 constexpr int32_t kAttendRowMax = 1 << 24;
-// Rows of a key head above which the tiles of keys go through LDS.
-constexpr int64_t kAttendPromptRows = 64;
+// Whether the rows are many enough for the tiles of keys to go through LDS: more than 16 of a key head,
+// and `pairs` of rows (in 16s) and keys. Below, the step kernels' spread over the CUs wins. 16 heads, 4 key
+// heads of 128, us (step kernel, prompt kernel): 8-bit, 24 rows of 1000 keys 11.3, 18.2; 24 of 16000 25.9,
+// 26.3 (6.1 M pairs); 32 of 16000 30.0, 27.7; fp32, 16 rows of 1000 12.6, 19.1; 8 of 16000 26.2, 30.3; 16
+// of 16000 38.6, 31.2 (4.1 M pairs).
+constexpr int64_t kPromptPairsQ8 = 6 << 20;
+constexpr int64_t kPromptPairsF32 = 3 << 20;
+inline bool AttendManyRows(const AttendArgs& a, int64_t pairs) {
+  const int64_t rows = int64_t(a.seq) * (a.heads / a.kv_heads);
+  if (rows <= 16) return false;
+  const int64_t each = AttendRangeSteps(a, 16, 32) * 32 * a.kv_heads;
+  return (rows + 15) / 16 * 16 >= (pairs + each - 1) / each;
+}
 // Many rows (attend_prompt.hip). load: the bytes that a thread may load at once from keys and values.
 void LaunchAttendPromptQ8(const AttendArgs& a, const Q8Cache& c, int load, hipStream_t stream);
 void LaunchAttendPromptF32(const AttendArgs& a, const float* k, const float* v, int load, hipStream_t stream);

@@ -421,7 +421,7 @@ void LaunchAttentionQ8(const AttendArgs& a, const Q8Cache& c, hipStream_t stream
     return a.dim % to == 0 && reinterpret_cast<uintptr_t>(c.k.code) % to == 0 && reinterpret_cast<uintptr_t>(c.v.code) % to == 0;
   };
   const int load = aligned(16) ? 16 : aligned(4) ? 4 : 1;
-  if (int64_t(a.seq) * (a.heads / a.kv_heads) > kAttendPromptRows) LaunchAttendPromptQ8(a, c, load, stream);
+  if (AttendManyRows(a, kPromptPairsQ8)) LaunchAttendPromptQ8(a, c, load, stream);
   else if (a.dim <= 64) LaunchStepOf<64>(a, c, load, stream);
   else if (a.dim <= 128) LaunchStepOf<128>(a, c, load, stream);
   else LaunchStepOf<256>(a, c, load, stream);

@@ -214,7 +214,7 @@ void LaunchStep(const AttendArgs& a, const float* k, const float* v, bool vec, h
 
 void LaunchAttentionWindow(const AttendArgs& a, const float* k, const float* v, hipStream_t stream) {
   const bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0;
-  if (int64_t(a.seq) * (a.heads / a.kv_heads) > kAttendPromptRows) LaunchAttendPromptF32(a, k, v, vec ? 16 : 4, stream);
+  if (AttendManyRows(a, kPromptPairsF32)) LaunchAttendPromptF32(a, k, v, vec ? 16 : 4, stream);
   else if (a.dim <= 64) LaunchStep<64>(a, k, v, vec, stream);
   else if (a.dim <= 128) LaunchStep<128>(a, k, v, vec, stream);
   else LaunchStep<256>(a, k, v, vec, stream);

@@ -15,10 +15,11 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kHeld = 8;  // items of a unit a thread holds in registers
 
-// The integer nearest to the true quotient x / s (ties to even), |x| <= 127.5 s. The product with the
-// rounded reciprocal is off by a little over 2^-17 at most, so its nearest integer is the quotient's
-// or a neighbour of it; the remainder x - r s tells which, since the fma forms it with one rounding
-// and near s / 2, where it matters, without any (x and r s are multiples of half an ulp of s there).
+// The integer nearest to the true quotient x / s (ties to even), |x| <= 127.5 s. x times the rounded
+// reciprocal is off by 2^-17 at most, so its nearest integer is the quotient's unless it lies within
+// 2^-16 of the middle between two (one wave in 64 has such a value). There the remainder x - r s tells,
+// since the fma forms it with one rounding and near s / 2, where it matters, without any (x and r s are
+// multiples of half an ulp of s there).
 struct Coder {
   float s, half, inv, pre;
   __device__ __forceinline__ explicit Coder(float scale) {
@@ -27,14 +28,35 @@ struct Coder {
     half = 0.5f * s;
     inv = scale > 0.f ? __fdiv_rn(1.f, s) : 0.f;  // no scale, or NaN: every code is 0
   }
-  __device__ __forceinline__ int32_t operator()(float x0) const {
+  __device__ __forceinline__ int32_t Exact(float x0) const {
     const float x = x0 * pre;
-    float r = rintf(x * inv);
+    const float r = rintf(x * inv);
     const float e = fmaf(-r, s, x);
     const float ae = fabsf(e);
     const int32_t n = static_cast<int32_t>(r);
     const bool off = ae > half || (ae == half && (n & 1) != 0);
     return n + (off && inv != 0.f ? (e < 0.f ? -1 : 1) : 0);
+  }
+  // The codes of x[0 .. kN) in the bytes of a word. 3 * 2^22 + r holds r in its low bits.
+  template <int kN>
+  __device__ __forceinline__ uint32_t Word(const float (&x0)[4]) const {
+    constexpr float kMagic = 12582912.f;
+    uint32_t bits[4] = {0, 0, 0, 0};
+    float off = 0.f;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      const float x = x0[e] * pre;
+      const float m = fmaf(x, inv, kMagic);
+      bits[e] = __float_as_uint(m);
+      off = fmaxf(off, fabsf(fmaf(x, inv, kMagic - m)));
+    }
+    if (__any(!(off < 0.5f - 0x1p-16f)) || !(inv > 0.f)) {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) bits[e] = static_cast<uint32_t>(Exact(x0[e]));
+    }
+    const uint32_t low = __builtin_amdgcn_perm(bits[1], bits[0], 0x0c0c0400u);
+    const uint32_t high = __builtin_amdgcn_perm(bits[3], bits[2], 0x04000c0cu);
+    return low | high;
   }
 };
 
@@ -135,11 +157,9 @@ __global__ __launch_bounds__(kThreads) void AppendQ8Kernel(AppendArgs a) {
   const auto store = [&](int32_t item, const float4& v) {
     const int32_t r = static_cast<int32_t>(static_cast<uint32_t>(item) / static_cast<uint32_t>(per_row));
     int8_t* p = codes + (lo + r) * code_row + (item - r * per_row) * kDims;
-    if (kVec)
-      *reinterpret_cast<uint32_t*>(p) = (static_cast<uint32_t>(code(v.x)) & 255u) | (static_cast<uint32_t>(code(v.y)) & 255u) << 8 |
-                                        (static_cast<uint32_t>(code(v.z)) & 255u) << 16 | static_cast<uint32_t>(code(v.w)) << 24;
-    else
-      *p = static_cast<int8_t>(code(v.x));
+    const float y[4] = {v.x, v.y, v.z, v.w};
+    if (kVec) *reinterpret_cast<uint32_t*>(p) = code.Word<4>(y);
+    else *p = static_cast<int8_t>(code.Word<1>(y));
   };
   if (held) {
 #pragma unroll

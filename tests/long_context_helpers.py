@@ -73,6 +73,9 @@ class Cache:
             by_row = np.repeat(self.scale[n], self.block, axis=0)[:self.shape[0], :, None]
             return (self.codes[n].astype(np.float32) * by_row).astype(np.float32)
 
+    def value_scale(self, rows):
+        return np.repeat(self.scale["v"], self.block, axis=0)[:rows]
+
     def on_device(self):
         return ({n: self.d_codes[n].numpy() for n in "kv"}, {n: self.d_scale[n].numpy() for n in "kv"})
 
@@ -93,13 +96,18 @@ def sees(position, seq, rows, window, sinks):
     return seen
 
 
-def attend(q, k, v, position, window, sinks, rows=None):
+def attend(q, k, v, position, window, sinks, rows=None, value_scale=None):
     """(out, bound) in 64 bits: softmax attention of the rows `rows` (all), and how far fp32 sums may be off.
 
     A score is a dot of D products, each off by U with either sign, and so is its sum: 8 sqrt(D) U sum|q k|
     (the probabilistic bound, at 8 standard deviations), plus the 22-bit query (4 U of the same sum) and the
     exponent's rounding (4 U (1 + |s|)). A weight is off by that, twice (numerator and sum), and the weighted
-    sums over n keys by 8 sqrt(n) U each, and 4 U for the 22-bit weight; the quotient adds 2 U."""
+    sums over n keys by 8 sqrt(n) U each, and 4 U for the 22-bit weight; the quotient adds 2 U.
+
+    value_scale [rows, kv_heads], for the 8-bit cache: the 22 bits of a weight are relative to the largest. A weight
+    enters as w = p * scale * 2^e with the largest w of the row in [2^3, 2^15), in two f16 parts cut towards zero:
+    off by 2^-22 w where the second part is a normal number, and by less than the spacing of f16's subnormal ones,
+    2^-24, where it is not, which is 2^-27 of the largest w. So a key adds at most 2^-27 max(p * scale) |code|."""
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
     seq, heads, dim = q.shape
     group = heads // k.shape[1]
@@ -118,14 +126,20 @@ def attend(q, k, v, position, window, sinks, rows=None):
             out[i, h] = p @ vv
             share = p * (d + 16 * np.sqrt(len(at)) * U + 6 * U)
             bound[i, h] = share @ np.abs(vv) + share.sum() * np.abs(out[i, h])
+            if value_scale is not None:
+                scale = np.asarray(value_scale, np.float64)[at, h // group]
+                bound[i, h] += 2.0 ** -27 * (p * scale).max() * (np.abs(vv) / scale[:, None]).sum(axis=0)
     return out, bound
 
 
 def assert_within(got, want, bound, floor=1e-30):
     err = np.abs(np.asarray(got, np.float64) - want)
     bad = ~(err <= bound + floor)
-    assert not bad.any(), (f"{bad.sum()} of {bad.size} beyond the bound; first at {np.argwhere(bad)[0]}, "
-                           f"worst ratio {np.nanmax(err / (bound + floor)):.3g}")
+    if bad.any():
+        at = tuple(np.argwhere(bad)[0])
+        near = np.sort(np.where(np.isfinite(err), err, 0).ravel())[-8:]
+        raise AssertionError(f"{bad.sum()} of {bad.size} beyond the bound; first at {at}: {got[at]!r}, {want[at]!r} wanted, "
+                             f"bound {np.broadcast_to(bound, err.shape)[at]:.3g}; largest errors {near}")
 
 
 def attention_q8_call(q, cache, position, window=0, sinks=0, row_stride=0, shape=None):

@@ -225,11 +225,24 @@ SHAPES = [
     (40, 1000, 8, 2, 128, 1, 333, 70), (200, 3, 2, 1, 256, 128, 77, 0), (70, 300, 2, 1, 100, 4, 0, 0),
     (31, 129, 4, 2, 63, 32, 40, 8), (260, 0, 1, 1, 64, 256, 0, 0), (129, 640, 16, 4, 64, 64, 128, 128),
 ]
+# And enough rows and keys for the kernels that bring tiles of keys through LDS: all dims and scale layouts, row blocks
+# and key tiles whole and partial, a range in several parts, windows narrower than a tile and wider, rows that see
+# nothing of a tile.
+SHAPES += [
+    (300, 0, 64, 8, 64, 64, 0, 0), (130, 1500, 64, 8, 128, 64, 0, 0), (97, 4001, 32, 4, 128, 128, 0, 0),
+    (77, 3000, 40, 8, 80, 16, 0, 0), (65, 2500, 64, 4, 100, 64, 0, 0), (90, 2000, 48, 3, 33, 4, 0, 0),
+    (64, 2100, 64, 16, 256, 32, 0, 0), (200, 1001, 64, 64, 64, 1, 0, 0), (513, 700, 56, 8, 128, 64, 300, 4),
+    (1000, 37, 64, 8, 64, 32, 150, 70), (2100, 0, 64, 8, 128, 256, 33, 2), (400, 5000, 32, 1, 96, 2, 1000, 1000),
+    (700, 300, 64, 2, 64, 64, 500, 0), (300, 2000, 24, 8, 255, 8, 900, 5), (600, 900, 32, 32, 128, 64, 1, 0),
+    (17, 30000, 32, 2, 128, 64, 0, 0), (2500, 100, 64, 8, 64, 64, 16, 300), (150, 3000, 32, 8, 1, 64, 0, 0),
+]
 IDS = ["-".join(map(str, s)) for s in SHAPES]
 
 
 def some_rows(seq):
-    return np.arange(seq) if seq <= 40 else np.unique(np.r_[0:9, 15:18, 31:34, seq // 2, seq - 9:seq])
+    if seq <= 40:
+        return np.arange(seq)
+    return np.unique(np.r_[0:9, 15:18, 31:34, seq // 2, seq - 9:seq] if seq <= 260 else np.r_[0:3, 31:33, seq // 2, seq - 3:seq])
 
 
 @pytest.mark.parametrize("seq,position,heads,kv_heads,dim,block,window,sinks", SHAPES, ids=IDS)
@@ -243,7 +256,7 @@ def test_attention_q8(seq, position, heads, kv_heads, dim, block, window, sinks)
             for n in "kv")
     got = attention_q8_call(q, cache, position, window, sinks)
     rows = some_rows(seq)
-    want, bound = attend(q, k[:position + seq], v[:position + seq], position, window, sinks, rows)
+    want, bound = attend(q, k[:position + seq], v[:position + seq], position, window, sinks, rows, cache.value_scale(position + seq))
     assert_within(got[rows], want, bound)
 
 
@@ -283,9 +296,10 @@ def test_attention_of_rows_of_a_fused_projection(seq, position, window, sinks):
     assert_within(out.numpy(), want, bound)
 
 
-@pytest.mark.parametrize("seq,position,window,sinks", [(1, 400, 100, 4), (5, 400, 100, 4), (80, 400, 100, 4), (200, 0, 33, 2)])
+@pytest.mark.parametrize("seq,position,window,sinks,copies", [
+    (1, 400, 100, 4, 1), (5, 400, 100, 4, 1), (80, 400, 100, 4, 1), (200, 0, 33, 2, 1), (80, 400, 100, 4, 128), (200, 0, 33, 2, 128)])
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf, 3e38])
-def test_keys_that_a_row_does_not_see_do_not_reach_it(seq, position, window, sinks, value):
+def test_keys_that_a_row_does_not_see_do_not_reach_it(seq, position, window, sinks, copies, value):
     """One key and its value are not finite (or huge): the rows that see it may be anything, the others keep their
     results. Keys before the window and behind the first tokens, inside and at its border, and future ones."""
     r = np.random.default_rng(2)
@@ -294,7 +308,10 @@ def test_keys_that_a_row_does_not_see_do_not_reach_it(seq, position, window, sin
     for t in sorted({4, max(0, position - window), max(0, position - window + 1), position + seq // 2, rows - 1}):
         kk, vv = k.copy(), v.copy()
         kk[t, 0, 3] = vv[t, 0, 5] = value
-        got = attention_window_call(q, kk, vv, position, window, sinks)
+        # `copies` of each query head: more rows, for the kernel of many of them
+        got = attention_window_call(np.repeat(q, copies, axis=1), kk, vv, position, window, sinks)
+        np.testing.assert_array_equal(got[:, 1::copies], got[:, ::copies]) if copies > 1 else None
+        got = got[:, ::copies]
         p = position + np.arange(seq)
         blind = np.flatnonzero(~((t <= p) & ((t > p - window) | (t < sinks))))
         want, bound = attend(q, np.nan_to_num(kk, posinf=0, neginf=0), np.nan_to_num(vv, posinf=0, neginf=0), position,
@@ -307,9 +324,10 @@ def test_keys_that_a_row_does_not_see_do_not_reach_it(seq, position, window, sin
             assert not np.isfinite(got[seen, :2, 5]).any()
 
 
-@pytest.mark.parametrize("seq,position,window,sinks,block", [(1, 400, 100, 4, 16), (6, 400, 100, 4, 32), (80, 400, 100, 4, 8),
-                                                             (200, 0, 33, 2, 64), (90, 100, 0, 0, 16)])
-def test_blocks_that_a_row_does_not_see_do_not_reach_it(seq, position, window, sinks, block):
+@pytest.mark.parametrize("seq,position,window,sinks,block,copies", [
+    (1, 400, 100, 4, 16, 1), (6, 400, 100, 4, 32, 1), (80, 400, 100, 4, 8, 1), (200, 0, 33, 2, 64, 1), (90, 100, 0, 0, 16, 1),
+    (80, 400, 100, 4, 8, 128), (200, 0, 33, 2, 64, 256), (90, 100, 0, 0, 16, 256), (200, 300, 64, 4, 32, 64)])
+def test_blocks_that_a_row_does_not_see_do_not_reach_it(seq, position, window, sinks, block, copies):
     """A NaN scale makes a block's keys (or values) NaN: rows that see none of the block keep their results."""
     r = np.random.default_rng(4)
     rows = position + seq
@@ -322,7 +340,7 @@ def test_blocks_that_a_row_does_not_see_do_not_reach_it(seq, position, window, s
             kept = cache.scale[plane][b, 0]
             cache.scale[plane][b, 0] = np.nan
             cache.upload()
-            got = attention_q8_call(q, cache, position, window, sinks)
+            got = attention_q8_call(np.repeat(q, copies, axis=1), cache, position, window, sinks)[:, ::copies]
             cache.scale[plane][b, 0] = kept
             p = position + np.arange(seq)[:, None]
             t = np.arange(b * block, min(rows, (b + 1) * block))[None, :]
@@ -336,24 +354,26 @@ def test_blocks_that_a_row_does_not_see_do_not_reach_it(seq, position, window, s
             assert np.isnan(got[seen, :2]).all()
 
 
-@pytest.mark.parametrize("seq", [1, 40])
-def test_attention_q8_over_scales_of_many_magnitudes(seq):
+@pytest.mark.parametrize("seq,block", [(1, 16), (40, 16), (1, 64), (40, 64)])
+@pytest.mark.parametrize("copies", [1, 128])
+def test_attention_q8_over_scales_of_many_magnitudes(seq, block, copies):
     """Blocks whose scales lie apart by up to 2^16 in values, and queries whose rows do by 2^40: the weights' range."""
     r = np.random.default_rng(6)
-    cache = Cache(600, 1, 64, 16)
+    cache = Cache(600, 1, 64, block)
     cache.fill(r, 600)
     cache.scale["v"][:] = 2.0 ** r.integers(-16, 1, cache.scale["v"].shape)
     cache.upload()
     q = (r.standard_normal((seq, 3, 64)) * 2.0 ** np.array([-20, 0, 3])[None, :, None]).astype(np.float32)
     q[:, 1, 7] *= 1000
     position = 600 - seq
-    want, bound = attend(q, cache.values("k"), cache.values("v"), position, 0, 0)
-    assert_within(attention_q8_call(q, cache, position), want, bound)
+    want, bound = attend(q, cache.values("k"), cache.values("v"), position, 0, 0, None, cache.value_scale(600))
+    assert_within(attention_q8_call(np.repeat(q, copies, axis=1), cache, position)[:, ::copies], want, bound)
 
 
 @pytest.mark.parametrize("seq", [1, 40])
+@pytest.mark.parametrize("copies", [1, 160])
 @pytest.mark.parametrize("exponent", [-100, 100])
-def test_attention_q8_of_very_small_and_large_values(seq, exponent):
+def test_attention_q8_of_very_small_and_large_values(seq, copies, exponent):
     r = np.random.default_rng(7)
     cache = Cache(300, 2, 64, 32)
     cache.fill(r, 300)
@@ -361,7 +381,39 @@ def test_attention_q8_of_very_small_and_large_values(seq, exponent):
     cache.upload()
     q = r.standard_normal((seq, 2, 64)).astype(np.float32)
     want, bound = attend(q, cache.values("k"), cache.values("v").astype(np.float64), 300 - seq, 0, 0)
-    assert_within(attention_q8_call(q, cache, 300 - seq), want, bound, floor=0)
+    assert_within(attention_q8_call(np.repeat(q, copies, axis=1), cache, 300 - seq)[:, ::copies], want, bound, floor=0)
+
+
+@pytest.mark.parametrize("seq,copies", [(3, 1), (64, 64)])
+@pytest.mark.parametrize("low,high", [(-3, 3), (-40, 40), (-100, 20), (0, 0)])
+def test_attention_window_over_rows_of_many_magnitudes(seq, copies, low, high):
+    """Key and value rows whose magnitudes lie apart by powers of two: common ones, and ones that need their own."""
+    r = np.random.default_rng(17)
+    rows = 900
+    q, k, v = (r.standard_normal(s).astype(np.float32) for s in ((seq, 4, 64), (rows, 2, 64), (rows, 2, 64)))
+    v *= (2.0 ** r.integers(low, high + 1, (rows, 2, 1))).astype(np.float32)
+    k *= (2.0 ** np.minimum(r.integers(low, high + 1, (rows, 2, 1)), 2)).astype(np.float32)
+    k[::7], v[::5] = 0, 0
+    want, bound = attend(q, k, v, rows - seq, 0, 0)
+    assert_within(attention_window_call(np.repeat(q, copies, axis=1), k, v, rows - seq)[:, ::copies], want, bound)
+
+
+@pytest.mark.parametrize("copies", [1, 128])
+def test_a_block_of_large_values_that_counts_for_little(copies):
+    """One block's values lie 2^90 above the others' and its scores 2^7 below: its weight, 2^-120 and less, times its
+    values is next to nothing, and the weights of the others keep their bits."""
+    r = np.random.default_rng(18)
+    cache = Cache(640, 1, 64, 64)
+    cache.fill(r, 640)
+    cache.codes["k"][:, 0, 0] = 64
+    cache.codes["k"][192:256, 0, 0] = -64
+    cache.scale["k"][:] = 1 / 64
+    cache.scale["v"][3] *= np.float32(2.0 ** 90)
+    cache.upload()
+    q = r.standard_normal((24, 2, 64)).astype(np.float32) / 8
+    q[:, :, 0] = 400  # scores of +-50 from this dim: weights e^-100
+    want, bound = attend(q, cache.values("k"), cache.values("v"), 616, 0, 0, None, cache.value_scale(640))
+    assert_within(attention_q8_call(np.repeat(q, copies, axis=1), cache, 616)[:, ::copies], want, bound)
 
 
 @pytest.mark.parametrize("seq", [1, 24])
@@ -383,13 +435,16 @@ def test_a_query_row_that_is_not_finite_stays_alone(value):
     r = np.random.default_rng(9)
     cache = Cache(300, 1, 64, 64)
     cache.fill(r, 300)
-    for seq in (2, 40):
+    for seq, copies in ((2, 1), (40, 1), (40, 256)):
         q = r.standard_normal((seq, 2, 64)).astype(np.float32)
         q[1, 0, 9] = value
         clean = q.copy()
         clean[1, 0, 9] = 0
         want, bound = attend(clean, cache.values("k"), cache.values("v"), 300 - seq, 0, 0)
-        for got in (attention_q8_call(q, cache, 300 - seq), attention_window_call(q, cache.values("k"), cache.values("v"), 300 - seq)):
+        many = np.repeat(q, copies, axis=1)
+        for got in (attention_q8_call(many, cache, 300 - seq),
+                    attention_window_call(many, cache.values("k"), cache.values("v"), 300 - seq)):
+            got = got[:, ::copies]
             assert np.isnan(got[1, 0]).all()
             keep = np.ones((seq, 2), bool)
             keep[1, 0] = False
@@ -477,7 +532,7 @@ def test_captured_and_replayed():
     r = np.random.default_rng(13)
     L = lib()
     heads, kv, dim, block = 8, 2, 128, 64
-    for seq, position in ((1, 6000), (48, 2000)):
+    for seq, position in ((1, 6000), (48, 2000), (700, 2000)):
         cache = Cache(position + seq, kv, dim, block)
         cache.fill(r, position + seq)
         x = r.standard_normal((seq, heads, dim)).astype(np.float32)
