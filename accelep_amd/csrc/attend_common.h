@@ -15,8 +15,6 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
-constexpr float kLog2e = 1.4426950408889634f;
-
 // Rows are pairs (query s, head g of a key head's group), row = s * group + g: a key head's rows share
 // its keys. The keys that rows [r0, r1) read, in steps of kStep keys: first those before `low` that
 // stay visible, then [low, high). Both parts begin at a multiple of kStep, so a step lies in one part,
@@ -59,6 +57,13 @@ __device__ __forceinline__ void SplitF16(float x, float y, h2& hi, h2& lo) {
   asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rx) : "v"(hi), "v"(x));
   asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(ry) : "v"(hi), "v"(y));
   lo = PackRtz(rx, ry);
+}
+
+// The same with both parts rounded to nearest, for what is split once: the second part's sign is then no
+// longer the first's, so the product of two second parts, which the fp32 kernels leave out, has no bias.
+__device__ __forceinline__ void SplitF16Nearest(float x, float y, h2& hi, h2& lo) {
+  hi = h2{static_cast<_Float16>(x), static_cast<_Float16>(y)};
+  lo = h2{static_cast<_Float16>(x - static_cast<float>(hi[0])), static_cast<_Float16>(y - static_cast<float>(hi[1]))};
 }
 
 // 2^(13 - e) for a row whose largest magnitude has the exponent e: the row then fills [2^13, 2^14).

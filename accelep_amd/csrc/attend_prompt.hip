@@ -221,13 +221,13 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
     top = max(top, XorLane<32>(top));
     const bool bad = top >= 0x7f800000u;
     const float scale = RowScale(top);
-    row_factor = kLog2e / scale * __fdiv_rn(1.f, __fsqrt_rn(static_cast<float>(a.dim)));
+    row_factor = a.factor / scale;  // by a power of two
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
       h2 hi[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        SplitF16(bad ? NAN : x[st][2 * e] * scale, bad ? NAN : x[st][2 * e + 1] * scale, hi[e], lo[e]);
+        SplitF16Nearest(bad ? NAN : x[st][2 * e] * scale, bad ? NAN : x[st][2 * e + 1] * scale, hi[e], lo[e]);
       qh[st] = Join(hi[0], hi[1], hi[2], hi[3]);
       ql[st] = Join(lo[0], lo[1], lo[2], lo[3]);
     }

@@ -114,7 +114,7 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
     top = max(top, XorLane<32>(top));
     const bool bad = top >= 0x7f800000u;  // no finite row: all of it NaN
     const float scale = RowScale(top);
-    row_factor = kLog2e / scale * __fdiv_rn(1.f, __fsqrt_rn(static_cast<float>(a.dim)));
+    row_factor = a.factor / scale;  // by a power of two
 #pragma unroll
     for (int i = 0; i < kC; ++i)
 #pragma unroll
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float y0 = x[i][8 * half + 2 * e] * scale, y1 = x[i][8 * half + 2 * e + 1] * scale;
-          SplitF16(bad ? NAN : y0, bad ? NAN : y1, hi[e], lo[e]);
+          SplitF16Nearest(bad ? NAN : y0, bad ? NAN : y1, hi[e], lo[e]);
         }
         qh[i][half] = Join(hi[0], hi[1], hi[2], hi[3]);
         ql[i][half] = Join(lo[0], lo[1], lo[2], lo[3]);
@@ -138,19 +138,25 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
   for (; u < end; u += sw) {  // uniform over the wave
     const int32_t t0 = range.Key(u);
     const int32_t next = u + sw < end ? range.Key(u + sw) : -1;
+    // The second parts' products first: they are rounded among themselves, before the sums are large.
     f4 st[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      h8 k8[kC][2];
       st[h] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < kC; ++i)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const uint32_t w0 = kx[h][i][2 * half] ^ 0x80808080u, w1 = kx[h][i][2 * half + 1] ^ 0x80808080u;
-          const h8 k8 = Join(CodesLow(w0), CodesHigh(w0), CodesLow(w1), CodesHigh(w1));
-          st[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[i][half], st[h], 0, 0, 0);
-          st[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[i][half], st[h], 0, 0, 0);
+          k8[i][half] = Join(CodesLow(w0), CodesHigh(w0), CodesLow(w1), CodesHigh(w1));
+          st[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[i][half], ql[i][half], st[h], 0, 0, 0);
         }
+#pragma unroll
+      for (int i = 0; i < kC; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          st[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[i][half], qh[i][half], st[h], 0, 0, 0);
     }
     float factor[kGroups][kEach], value[kGroups][kEach];
 #pragma unroll
@@ -190,7 +196,9 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      p[e] = __builtin_amdgcn_exp2f(p[e] - base);
+      // The product once more, unrounded: near the reference little is left of it.
+      const float x = __builtin_fmaf(st[e >> 2][e & 3], factor[(e >> 2) % kGroups][(e & 3) % kEach], -base);
+      p[e] = __builtin_amdgcn_exp2f(whole || p[e] != -INFINITY ? x : -INFINITY);
       sum += p[e];
     }
     l = l * corr + sum;

@@ -92,7 +92,6 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
       q[i] = f4{x[0], x[1], x[2], x[3]};
     }
   }
-  const float factor = kLog2e * __fdiv_rn(1.f, __fsqrt_rn(static_cast<float>(a.dim)));
 
   float m = -INFINITY, l = 0.f;  // l: this lane's share of the row's sum
   f4 acc[kC][4];
@@ -144,18 +143,18 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const bool in = Sees(a, p_row, t0 + 4 * g + e);
-      p[e] = in ? (bad >> e & 1 ? NAN : (st0[e] + st1[e]) * factor) : -INFINITY;
-      mx = fmaxf(mx, p[e]);
+      st0[e] = in ? (bad >> e & 1 ? NAN : st0[e] + st1[e]) : -INFINITY;
+      mx = fmaxf(mx, st0[e]);
     }
     mx = fmaxf(mx, XorLane<16>(mx));
-    mx = fmaxf(mx, XorLane<32>(mx));
+    mx = fmaxf(mx, XorLane<32>(mx)) * a.factor;
     const float m_new = fmaxf(m, mx);
     const float base = m_new == -INFINITY ? 0.f : m_new;
     const float corr = __builtin_amdgcn_exp2f(m - base);
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      p[e] = __builtin_amdgcn_exp2f(p[e] - base);
+      p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st0[e], a.factor, -base));
       sum += p[e];
     }
     l = l * corr + sum;

@@ -492,6 +492,7 @@ struct AttendArgs {
   int64_t q_stride;
   int32_t seq, position, heads, kv_heads, dim;  // position + seq < 2^31 - 256
   int32_t window, sinks;
+  float factor;  // log2(e) / sqrt(dim): scores in log2 units
 };
 void LaunchAttentionQ8(const AttendArgs& a, const Q8Cache& cache, hipStream_t stream);
 void LaunchAttentionWindow(const AttendArgs& a, const float* k, const float* v, hipStream_t stream);

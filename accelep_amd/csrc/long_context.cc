@@ -17,6 +17,7 @@ constexpr int64_t kMaxBlock = 256;
 constexpr int64_t kMaxRows = 0x7fffffff - 256;  // positions and row counts are 32-bit in the kernels
 constexpr int64_t kMaxKvRow = 1 << 24;           // and a step's offsets from its first key row
 constexpr double kTwoPi = 6.283185307179586476925286766559;
+constexpr double kLog2e = 1.4426950408889634073599246810019;
 
 void Invalid(const char* what) { Fail(ACCEL_HIP_INVALID_ARGUMENT, what); }
 
@@ -104,6 +105,7 @@ bool CheckedAttend(const AccelHipBuffer& q, const AccelHipBuffer& out, int64_t s
   a->dim = static_cast<int32_t>(dim);
   a->window = window == 0 || window >= seen ? kNoWindow : static_cast<int32_t>(window);
   a->sinks = static_cast<int32_t>(std::min(sinks, seen));
+  a->factor = dim > 0 ? static_cast<float>(kLog2e / std::sqrt(static_cast<double>(dim))) : 0.f;
   return out_bytes > 0;
 }
 
