@@ -141,8 +141,6 @@ inline int64_t AttendRangeSteps(const AttendArgs& a, int64_t rows, int64_t step)
   return (keys + step - 1) / step + (std::min<int64_t>(a.sinks, end) + step - 1) / step;
 }
 
-// Bytes (or floats) of a key row, all heads, up to which a step's rows lie within 32-bit offsets.
-constexpr int32_t kAttendRowMax = 1 << 24;
 // Whether the rows are many enough for the tiles of keys to go through LDS: more than 16 of a key head,
 // and `pairs` of rows (in 16s) and keys. Below, the step kernels' spread over the CUs wins. 16 heads, 4 key
 // heads of 128, us (step kernel, prompt kernel): 8-bit, 24 rows of 1000 keys 11.3, 18.2; 24 of 16000 25.9,

@@ -445,7 +445,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
 
 template <int DP, bool kF32>
 void LaunchPrompt(const AttendArgs& a, const PromptArgs& b, int load, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(int64_t(a.kv_heads) * b.splits * b.tiles)), block(kThreads);
+  const dim3 grid(GridOf(int64_t(a.kv_heads) * b.splits * b.tiles, kThreads, "Attention is too large")), block(kThreads);
 #define ACCEL_PROMPT(L, U) hipLaunchKernelGGL((AttendPromptKernel<DP, kF32, L, U>), grid, block, 0, stream, a, b)
   if constexpr (kF32) {
     if (load == 16) ACCEL_PROMPT(16, false);

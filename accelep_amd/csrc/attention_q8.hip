@@ -370,7 +370,7 @@ void LaunchAttendJoin(const AttendArgs& a, const AttendPartial& partial, int32_t
   const int32_t pieces = PartialDims(a.dim) / 4;
   const int32_t lanes = std::min(splits, kJoinThreads / pieces);
   const int32_t per_group = kJoinThreads / (pieces * lanes);
-  hipLaunchKernelGGL(AttendJoinKernel, dim3(static_cast<uint32_t>((rows + per_group - 1) / per_group)), dim3(kJoinThreads), 0,
+  hipLaunchKernelGGL(AttendJoinKernel, dim3(GridOf((int64_t(rows) + per_group - 1) / per_group, kJoinThreads, "Attention is too large")), dim3(kJoinThreads), 0,
                      stream, partial.ml, partial.o, a.out, rows, splits, a.dim, lanes, vec);
   Check(hipGetLastError(), "AttendJoinKernel launch");
 }
@@ -407,7 +407,7 @@ void LaunchStep(const AttendArgs& a, const Q8Cache& c, hipStream_t stream) {
   // workgroups of four waves, 9.0 of eight, 14.2 in one of sixteen a key head).
   const int32_t sw = hw == 1 && units * steps < cus * kWaves ? 4 : kWaves / hw;
   const AttendSplit split = SplitRange(a, units, 1, steps <= 2 * sw ? 1 : steps / sw);
-  hipLaunchKernelGGL((AttendQ8StepKernel<DP, kLoad, kScales>), dim3(static_cast<uint32_t>(units * split.count)),
+  hipLaunchKernelGGL((AttendQ8StepKernel<DP, kLoad, kScales>), dim3(GridOf(units * split.count, 64 * hw * sw, "Attention is too large")),
                      dim3(64 * hw * sw), 0, stream, a, c, hw, split.count, split.partial);
   Check(hipGetLastError(), "AttendQ8StepKernel launch");
   if (split.count > 1) LaunchAttendJoin(a, split.partial, split.count, stream);

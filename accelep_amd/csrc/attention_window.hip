@@ -202,7 +202,7 @@ void LaunchStep(const AttendArgs& a, const float* k, const float* v, bool vec, h
   const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
   const int32_t waves = units * steps < cus * kWaves ? 4 : kWaves;
   const AttendSplit split = SplitRange(a, units, 1, steps <= 2 * waves ? 1 : steps / waves);
-  const dim3 grid(static_cast<uint32_t>(units * split.count)), block(64 * waves);
+  const dim3 grid(GridOf(units * split.count, 64 * waves, "Attention is too large")), block(64 * waves);
   if (vec) hipLaunchKernelGGL((AttendF32StepKernel<DP, 16>), grid, block, 0, stream, a, k, v, split.count, split.partial);
   else hipLaunchKernelGGL((AttendF32StepKernel<DP, 4>), grid, block, 0, stream, a, k, v, split.count, split.partial);
   Check(hipGetLastError(), "AttendF32StepKernel launch");

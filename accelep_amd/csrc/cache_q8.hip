@@ -19,7 +19,8 @@ constexpr int kHeld = 8;  // items of a unit a thread holds in registers
 // reciprocal is off by 2^-17 at most, so its nearest integer is the quotient's unless it lies within
 // 2^-16 of the middle between two (one wave in 64 has such a value). There the remainder x - r s tells,
 // since the fma forms it with one rounding and near s / 2, where it matters, without any (x and r s are
-// multiples of half an ulp of s there).
+// multiples of half an ulp of s there). A scale below 2^-126 is itself rounded to few bits, so that its
+// codes may pass 127: they stay there.
 struct Coder {
   float s, half, inv, pre;
   __device__ __forceinline__ explicit Coder(float scale) {
@@ -35,7 +36,7 @@ struct Coder {
     const float ae = fabsf(e);
     const int32_t n = static_cast<int32_t>(r);
     const bool off = ae > half || (ae == half && (n & 1) != 0);
-    return n + (off && inv != 0.f ? (e < 0.f ? -1 : 1) : 0);
+    return min(max(n + (off && inv != 0.f ? (e < 0.f ? -1 : 1) : 0), -127), 127);
   }
   // The codes of x[0 .. kN) in the bytes of a word. 3 * 2^22 + r holds r in its low bits.
   template <int kN>
@@ -50,7 +51,7 @@ struct Coder {
       bits[e] = __float_as_uint(m);
       off = fmaxf(off, fabsf(fmaf(x, inv, kMagic - m)));
     }
-    if (__any(!(off < 0.5f - 0x1p-16f)) || !(inv > 0.f)) {
+    if (__any(!(off < 0.5f - 0x1p-16f)) || !(inv > 0.f) || pre != 1.f) {
 #pragma unroll
       for (int e = 0; e < kN; ++e) bits[e] = static_cast<uint32_t>(Exact(x0[e]));
     }
@@ -233,7 +234,14 @@ void LaunchAppendCacheQ8(const float* k, const float* v, const Q8Cache& cache, i
   a.position = static_cast<int32_t>(position);
   const int64_t blocks = ((position + seq - 1) >> cache.block_shift) - (position >> cache.block_shift) + 1;
   const int64_t units = blocks * cache.kv_heads * 2;
-  if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "AppendCache is too large");
+  constexpr int64_t kMostUnits = int64_t(1) << 23;  // a grid holds fewer than 2^32 threads
+  if (units > kMostUnits && blocks > 1) {  // whole blocks at a time
+    const int64_t first = std::max<int64_t>(1, kMostUnits / (cache.kv_heads * 2)) << cache.block_shift;
+    const int64_t rows = first - (position & ((int64_t(1) << cache.block_shift) - 1));
+    LaunchAppendCacheQ8(k, v, cache, rows, position, row_stride, stream);
+    LaunchAppendCacheQ8(k + rows * row_stride, v + rows * row_stride, cache, seq - rows, position + rows, row_stride, stream);
+    return;
+  }
   a.units = static_cast<uint32_t>(units);
   const bool vec = AlignedTo(k, 16) && AlignedTo(v, 16) && row_stride % 4 == 0 && cache.dim % 4 == 0 &&
                    AlignedTo(cache.k.code, 4) && AlignedTo(cache.v.code, 4);
@@ -242,7 +250,7 @@ void LaunchAppendCacheQ8(const float* k, const float* v, const Q8Cache& cache, i
   const int64_t rows = std::min<int64_t>(int64_t(1) << cache.block_shift, seq);
   const bool wide = rows * cache.dim > 64 * kHeld * (vec ? 4 : 1) ||
                     (units <= 256 && (int64_t(cache.dim) << cache.block_shift) > 2048);
-  const dim3 grid(static_cast<uint32_t>(wide ? units : (units + 3) / 4)), block(kThreads);
+  const dim3 grid(GridOf(wide ? units : (units + 3) / 4, kThreads, "AppendCache is too large")), block(kThreads);
   if (vec && wide) hipLaunchKernelGGL((AppendQ8Kernel<true, 4>), grid, block, 0, stream, a);
   else if (vec) hipLaunchKernelGGL((AppendQ8Kernel<true, 1>), grid, block, 0, stream, a);
   else if (wide) hipLaunchKernelGGL((AppendQ8Kernel<false, 4>), grid, block, 0, stream, a);
@@ -270,8 +278,7 @@ void LaunchReadCacheQ8(const Q8Cache& cache, int64_t first, int64_t count, float
   a.block_shift = cache.block_shift;
   a.items = count * a.kv_heads * a.per_head;
   const int64_t grid_x = (a.items + kThreads * kReadItems - 1) / (kThreads * kReadItems);
-  if (grid_x > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "the range is too large");
-  const dim3 grid(static_cast<uint32_t>(grid_x), static_cast<uint32_t>(planes)), block(kThreads);
+  const dim3 grid(GridOf(grid_x, kThreads * planes, "the range is too large"), static_cast<uint32_t>(planes)), block(kThreads);
   if (vec) hipLaunchKernelGGL(ReadQ8Kernel<true>, grid, block, 0, stream, a);
   else hipLaunchKernelGGL(ReadQ8Kernel<false>, grid, block, 0, stream, a);
   Check(hipGetLastError(), "ReadQ8Kernel launch");

@@ -457,6 +457,11 @@ constexpr size_t kDecodeSplitMaxBytesPerHead = 64 * (2 + 64) * sizeof(float);
 // Scratch bytes LaunchAttention needs for these sizes (0 when none).
 size_t AttentionWorkBytes(int64_t seq, int64_t heads, int64_t max_position, int64_t head_dim);
 size_t AttentionFlashWorkBytes(int64_t head_dim);
+// A grid of `groups` workgroups of `threads`: HIP launches fewer than 2^32 threads.
+inline uint32_t GridOf(int64_t groups, int64_t threads, const char* what) {
+  if (groups > 0xffffffffll / threads) Fail(ACCEL_HIP_INVALID_ARGUMENT, what);
+  return static_cast<uint32_t>(groups);
+}
 // ---- long contexts (rope_scaled.hip, cache_q8.hip, attention_q8.hip, attention_window.hip; the
 // entry points and their checks are in long_context.cc) ----
 struct RopeScaledArgs {

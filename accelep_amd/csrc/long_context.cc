@@ -234,6 +234,14 @@ ACCEL_HIP_API int accel_hip_append_cache_q8(AccelHipBuffer k, AccelHipBuffer v, 
     RequireAligned(k, sizeof(float), "AppendCache keys are not aligned");
     RequireAligned(v, sizeof(float), "AppendCache values are not aligned");
     if (seq == 0) return;
+    const size_t code_bytes = CheckedBytes(cache->capacity, row) / sizeof(float);
+    const size_t scale_bytes = CheckedBytes((cache->capacity - 1) / cache->block + 1, cache->kv_heads);
+    const struct { const AccelHipBuffer& buffer; size_t bytes; } parts[] = {
+        {cache->k, code_bytes}, {cache->v, code_bytes}, {cache->k_scale, scale_bytes}, {cache->v_scale, scale_bytes},
+        {k, bytes}, {v, bytes}};
+    for (int i = 0; i < 4; ++i)  // k and v may share rows
+      for (int j = i + 1; j < 6; ++j)
+        if (Overlap(parts[i].buffer, parts[i].bytes, parts[j].buffer, parts[j].bytes)) Invalid("AppendCache planes overlap");
     const int64_t b0 = position / cache->block;
     const size_t first = static_cast<size_t>(b0 * cache->block * row);
     const size_t codes = static_cast<size_t>(end * row) - first;
@@ -263,6 +271,7 @@ ACCEL_HIP_API int accel_hip_read_cache_q8(const AccelHipCacheQ8* cache, int64_t 
     float* k = checked(k_out, "cache key output is out of range");
     float* v = checked(v_out, "cache value output is out of range");
     if (k == nullptr && v == nullptr) return;
+    if (k != nullptr && v != nullptr && Overlap(k_out, bytes, v_out, bytes)) Invalid("cache outputs overlap");
     if (k != nullptr) NoteDeviceWrite(k, bytes);
     if (v != nullptr) NoteDeviceWrite(v, bytes);
     LaunchReadCacheQ8(c, first, count, k, v, Ctx().stream);
@@ -278,6 +287,10 @@ ACCEL_HIP_API int accel_hip_attention_q8(AccelHipBuffer q, const AccelHipCacheQ8
     const bool any = CheckedAttend(q, out, seq, position, heads, c.kv_heads, c.dim, row_stride, window, sinks, &a);
     if (position + seq > cache->capacity) Invalid("8-bit cache rows are out of range");
     if (!any) return;
+    const size_t out_bytes = CheckedBytes(seq, heads * c.dim);
+    const size_t codes = static_cast<size_t>(position + seq) * c.kv_heads * c.dim;
+    if (Overlap(out, out_bytes, cache->k, codes) || Overlap(out, out_bytes, cache->v, codes))
+      Invalid("Attention output overlaps the cache");
     NoteDeviceWrite(out.data, sizeof(float));
     LaunchAttentionQ8(a, c, Ctx().stream);
   });
@@ -296,6 +309,8 @@ ACCEL_HIP_API int accel_hip_attention_window(AccelHipBuffer q, AccelHipBuffer k,
     RequireAligned(k, sizeof(float), "Attention key is not aligned");
     RequireAligned(v, sizeof(float), "Attention value is not aligned");
     if (!any) return;
+    const size_t out_bytes = CheckedBytes(seq, heads * head_dim);
+    if (Overlap(out, out_bytes, k, bytes) || Overlap(out, out_bytes, v, bytes)) Invalid("Attention output overlaps the cache");
     NoteDeviceWrite(out.data, sizeof(float));
     LaunchAttentionWindow(a, static_cast<const float*>(k.data), static_cast<const float*>(v.data), Ctx().stream);
   });

@@ -279,26 +279,34 @@ typedef struct AccelHipCacheQ8 {
  * head_dim a row). Each touched block and head gets the scale max|x| / 127 of its new rows, or keeps
  * the scale it has where rows of the block before `position` need more; when it grows, those rows'
  * codes become the nearest code of code * old / new. A code is the nearest integer to x / scale (the
- * true quotient; ties to even). Rows of the block from position + seq on do not count any more. A
- * NaN or an infinity makes its block's scale of that head NaN, and all that is read of it, until the
- * block is written from its start. The planes must not overlap one another or k and v. */
+ * true quotient; ties to even), within -127 .. 127, where only a scale below 2^-126 leaves it. Rows of
+ * the block from position + seq on do not count any more. A NaN or an infinity makes its block's scale of
+ * that head NaN, and all that is read of it, until the block is written from its start. The planes may
+ * not overlap one another or k and v. */
 ACCEL_HIP_API int accel_hip_append_cache_q8(AccelHipBuffer k, AccelHipBuffer v, const AccelHipCacheQ8* cache,
                                             int64_t seq, int64_t position, int64_t row_stride);
 /* Rows [first, first + count) of the 8-bit cache as fp32 [count, kv_heads, head_dim], code * scale
- * rounded once. k_out or v_out without data leaves that plane out. */
+ * rounded once. k_out or v_out without data leaves that plane out; they may not overlap. */
 ACCEL_HIP_API int accel_hip_read_cache_q8(const AccelHipCacheQ8* cache, int64_t first, int64_t count,
                                           AccelHipBuffer k_out, AccelHipBuffer v_out);
 /* Attention (as accel_hip_attention: causal, grouped heads, 1 / sqrt(head_dim)) over the 8-bit cache,
  * whose rows up to position + seq are written. With window > 0 the row at p sees the keys t <= p with
  * t > p - window or t < sinks; with window 0 every t <= p. q's rows are row_stride apart, out is dense
- * and may not overlap q. Rounding: queries and softmax weights enter the products with 22 bits (a
- * query relative to its row's largest value, a weight to the largest), sums are fp32. */
+ * and may not overlap q or the cache. head_dim is at most 256, kv_heads * head_dim at most 2^24.
+ * Rounding: queries and softmax weights enter the products with 22 bits (a query relative to its row's
+ * largest value, a weight to the largest), sums are fp32. A row whose query is not finite, or that sees a
+ * scale that is not finite, is NaN. Inside a capture whose workspace was not grown before (by the same
+ * call, once), the key range is not divided over workgroups. */
 ACCEL_HIP_API int accel_hip_attention_q8(AccelHipBuffer q, const AccelHipCacheQ8* cache, AccelHipBuffer out,
                                          int64_t seq, int64_t position, int64_t heads, int64_t row_stride,
                                          int64_t window, int64_t sinks);
 /* Attention over an fp32 cache k, v [>= position + seq, kv_heads, head_dim] with a sliding window: the
  * row at p sees the keys t <= p with t > p - window or t < sinks (window 0: every t <= p). Keys that no
- * row sees are not read. q's rows are row_stride apart, out is dense and may not overlap q. */
+ * row sees count for nothing, NaN included. q's rows are row_stride apart, out is dense and may not
+ * overlap q, k or v. Sizes, captures and queries as above. Rounding: with many rows (16 and more of a key
+ * head, over a long range) queries, keys and values enter the products with 22 bits of their row's
+ * largest value and weights with 22 bits of the largest; otherwise in fp32. A key or value that is not
+ * finite makes the rows that see it NaN. */
 ACCEL_HIP_API int accel_hip_attention_window(AccelHipBuffer q, AccelHipBuffer k, AccelHipBuffer v, AccelHipBuffer out,
                                              int64_t seq, int64_t position, int64_t heads, int64_t kv_heads,
                                              int64_t head_dim, int64_t row_stride, int64_t window, int64_t sinks);

@@ -61,7 +61,8 @@ class Cache:
                 kept = self.codes[n][begin:lo]
                 with np.errstate(invalid="ignore", divide="ignore"):
                     again = nearest(kept * old.astype(np.float64)[None, :, None] / now.astype(np.float64)[None, :, None])
-                    code = nearest(new / now.astype(np.float64)[None, :, None])
+                    # (a scale below 2^-126 has few bits: its codes may pass 127 and stay there)
+                    code = np.clip(nearest(new / now.astype(np.float64)[None, :, None]), -127, 127)
                 grows = now > old
                 self.codes[n][begin:lo] = np.where(grows[None, :, None], again, kept)
                 self.codes[n][lo:hi] = np.nan_to_num(np.where((now > 0)[None, :, None], code, 0))

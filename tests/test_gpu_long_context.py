@@ -97,6 +97,53 @@ def test_rope_from_memory_that_is_not_aligned_to_16_bytes():
     assert_within(got[1:].reshape(3, 2, 64), want, bound, floor=0)
 
 
+@pytest.mark.parametrize("layout", [capi.ROPE_HALF, capi.ROPE_INTERLEAVED])
+def test_rope_of_more_rows_than_a_grid_holds(layout):
+    """2^23 rows and some: workgroups take several. The last rows are compared."""
+    r = np.random.default_rng(7)
+    rows = (1 << 23) + 1001
+    x = np.tile(r.standard_normal((1001, 2)).astype(np.float32), (rows // 1001 + 1, 1))[:rows].reshape(rows, 1, 2)
+    f = np.array([0.001])
+    got = rope_call(dev(x), f, rows, 1, 2, 2, layout, out=dev(np.zeros_like(x)))
+    for at in (slice(0, 50), slice((1 << 23) - 50, (1 << 23) + 50), slice(rows - 50, rows)):
+        want, bound = rotated(x[at], f, np.arange(rows)[at], layout, 1.0)
+        assert_within(got[at], want, bound, floor=0)
+
+
+def test_append_of_more_blocks_than_a_grid_holds():
+    """2^23 units and some, from inside a block: the launches meet at a block's border."""
+    r = np.random.default_rng(15)
+    kv, dim, block, position = 64, 1, 4, 2
+    seq = (1 << 23) // (kv * 2) * block + 9
+    cache = Cache(position + seq, kv, dim, block)
+    first = [r.standard_normal((position, kv, dim)).astype(np.float32) for _ in "kv"]
+    append_call(cache, *first, 0)
+    cache.append(*first, 0)
+    x = np.tile(r.standard_normal((1003, kv, dim)).astype(np.float32), (seq // 1003 + 1, 1, 1))[:seq]
+    append_call(cache, x, -x, position)
+    codes, scale = cache.on_device()
+    whole = np.zeros((scale["k"].shape[0] * block, kv), np.float32)
+    whole[:position], whole[position:position + seq] = first[0][..., 0], x[..., 0]
+    need = (np.abs(whole.reshape(-1, block, kv).astype(np.float64)).max(axis=1) / 127).astype(np.float32)
+    np.testing.assert_array_equal(scale["k"], need)
+    by_row = np.repeat(need, block, axis=0)[position:position + seq].astype(np.float64)
+    np.testing.assert_array_equal(codes["k"][position:, :, 0], np.rint(x[..., 0] / by_row))
+    np.testing.assert_array_equal(codes["v"][position:, :, 0], np.rint(-x[..., 0] / np.repeat(scale["v"], block, axis=0)[position:position + seq]
+                                                                       .astype(np.float64)))
+
+
+def test_attention_of_nothing():
+    L = lib()
+    cache = Cache(16, 2, 64, 4)
+    out = dev(np.full(64, 7.0, np.float32))
+    for seq, heads in ((0, 4), (3, 0)):
+        check(L.accel_hip_attention_q8(out.buffer if seq == 0 else NONE, C.byref(cache.handle), out.buffer, seq, 5, heads, 0, 0, 0))
+        check(L.accel_hip_attention_window(NONE, cache.d_scale["k"].buffer if heads == 0 else NONE, NONE, NONE, 0, 0, heads, 2, 64, 0, 3, 1))
+    check(L.accel_hip_append_cache_q8(NONE, NONE, C.byref(cache.handle), 0, 16, 0))
+    check(L.accel_hip_read_cache_q8(C.byref(cache.handle), 16, 0, NONE, NONE))
+    assert (out.numpy() == 7.0).all()
+
+
 def test_rope_of_nothing():
     x = dev(np.zeros(64, np.float32))
     for seq, heads, dim in ((0, 2, 64), (3, 0, 64), (3, 2, 0)):
@@ -189,6 +236,25 @@ def test_codes_are_the_nearest_of_the_true_quotient(gain):
     assert_same_cache(cache)
 
 
+@pytest.mark.parametrize("dim", [64, 63])
+def test_codes_of_values_whose_scale_has_few_bits(dim):
+    """Multiples of 2^-149 up to 2^14: the scale is one of few, a code may want 190 and is 127."""
+    r = np.random.default_rng(31)
+    cache = Cache(64, 3, dim, 4)
+    top = np.float64(2.0) ** r.uniform(0, 14, (64, 3, 1)).round(2)
+    top[:4] = 190
+    top[4:8] = 63  # no scale at all
+    k, v = ((np.rint(top * r.uniform(-1, 1, (64, 3, dim))) * 2.0 ** -149).astype(np.float32) for _ in "kv")
+    k[0, :, 0] = 190 * 2.0 ** -149
+    append_call(cache, k, v, 0)
+    cache.append(k, v, 0)
+    codes, scale = cache.on_device()
+    for n in "kv":
+        np.testing.assert_array_equal(scale[n], cache.scale[n])
+        np.testing.assert_array_equal(codes[n], cache.codes[n])
+    assert codes["k"][0, 0, 0] == 127 and (codes["k"][4:8] == 0).all()
+
+
 def test_zeros_infinities_and_nans():
     cache = Cache(64, 2, 64, 16)
     r = np.random.default_rng(9)
@@ -236,6 +302,9 @@ SHAPES += [
     (700, 300, 64, 2, 64, 64, 500, 0), (300, 2000, 24, 8, 255, 8, 900, 5), (600, 900, 32, 32, 128, 64, 1, 0),
     (17, 30000, 32, 2, 128, 64, 0, 0), (2500, 100, 64, 8, 64, 64, 16, 300), (150, 3000, 32, 8, 1, 64, 0, 0),
 ]
+# Decode steps over long ranges, where a workgroup serves several key heads: four, three, two and one of them.
+SHAPES += [(1, 70000, 8, 4, 128, 64, 0, 0), (1, 100000, 9, 3, 64, 32, 0, 0), (2, 150000, 4, 2, 64, 64, 0, 0),
+           (1, 40000, 8, 4, 256, 16, 0, 0), (1, 60000, 10, 5, 80, 64, 59000, 4), (3, 90000, 4, 4, 100, 64, 0, 0)]
 IDS = ["-".join(map(str, s)) for s in SHAPES]
 
 

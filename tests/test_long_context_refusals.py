@@ -87,6 +87,35 @@ def test_append_and_read_refuse_rows_out_of_range():
     refused(read(0, 4, v=buf(4)), "value output")
 
 
+def test_append_and_read_refuse_memory_that_is_written_twice():
+    L = lib()
+    k, v = buf(4 * 4 * 128), buf(4 * 4 * 128, 1 << 28)
+    for name, other in (("v", buf(1 << 20, (1 << 30) + 100)), ("k_scale", buf(1 << 20, (1 << 30) + 4)),
+                        ("v_scale", buf(1 << 20, 3 << 30)), ("v", buf(1 << 20, 1 << 28)), ("k_scale", buf(1 << 20, 1 << 20))):
+        refused(L.accel_hip_append_cache_q8(k, v, C.byref(cache(**{name: other})), 4, 0, 0), "planes overlap")
+    refused(L.accel_hip_append_cache_q8(buf(1 << 20, (2 << 30) + 4), v, C.byref(cache()), 4, 0, 0), "planes overlap")
+    refused(L.accel_hip_read_cache_q8(C.byref(cache()), 0, 4, k, k), "outputs overlap")
+    refused(L.accel_hip_read_cache_q8(C.byref(cache()), 0, 4, k, buf(1 << 20, (1 << 20) + 4 * 4 * 128 - 4)), "outputs overlap")
+
+
+def test_attention_refuses_to_write_into_the_keys_and_values():
+    L, c = lib(), cache()
+    q = buf(4 * 3 * 4 * 64)
+    for at in (1 << 30, (2 << 30) + 3 * 128 - 4):
+        refused(L.accel_hip_attention_q8(q, C.byref(c), buf(1 << 20, at), 3, 0, 4, 0, 0, 0), "overlaps the cache")
+    k, v = buf(4 * 128 * 2 * 64, 1 << 30), buf(4 * 128 * 2 * 64, 2 << 30)
+    for at in (1 << 30, (2 << 30) + 4 * 3 * 128 - 4):
+        refused(L.accel_hip_attention_window(q, k, v, buf(1 << 20, at), 3, 0, 4, 2, 64, 0, 0, 0), "overlaps the cache")
+
+
+def test_attention_refuses_key_rows_past_its_offsets():
+    L, wide = lib(), (1 << 17) + 1  # heads of 128: 2^24 + 128
+    room, out = buf(1 << 40), buf(1 << 40, 1 << 50)
+    c = cache(1, wide, 128, 1, **{n: buf(1 << 40, (i + 2) << 50) for i, n in enumerate(("k", "v", "k_scale", "v_scale"))})
+    refused(L.accel_hip_attention_q8(room, C.byref(c), out, 1, 0, wide, 0, 0, 0), "too large")
+    refused(L.accel_hip_attention_window(room, c.k, c.v, out, 1, 0, wide, wide, 128, 0, 0, 0), "too large")
+
+
 def test_attention_refuses_what_does_not_fit():
     L, c = lib(), cache()
     q, out = buf(4 * 3 * 4 * 64), buf(4 * 3 * 4 * 64, 1 << 28)
