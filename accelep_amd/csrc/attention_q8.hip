@@ -16,8 +16,10 @@ constexpr int kStepKeys = 32;
 
 // One workgroup per (16 rows of up to 4 key heads, key range): wave w serves head w % hw of them, and the
 // waves of a head take its steps of 32 keys in turn, so that a workgroup reads a key row's heads together
-// (131072 keys of 8 heads of 128: a workgroup a head read them at 4.7 TB/s, 4 heads at 5.7).
-// Bound: the cache's bytes. Keys and values go from memory to registers, and there to f16: no LDS and
+// (131072 keys of 8 heads of 128, loads alone: a workgroup a head read them at 4.7 TB/s, 4 heads at 5.7).
+// Bound: the cache's bytes over a long range (131072 keys, 32 heads on 8 key heads of 128: 51.5 us, 5.2
+// TB/s, and 3.3 of the join); over a short one the chain of load, products, softmax and products of a
+// wave's few steps (2048 keys, 9 heads on 3 of 64: 5.2 us and 3.4 of the join). Keys and values go from memory to registers, and there to f16: no LDS and
 // no barrier in the loop. Lane (j, g) = (lane % 16, lane / 16). Per step
 //  * S^T = K Q^T on v_mfma_f32_16x16x32_f16: the A operand of instruction (c, half) are the codes
 //    64c + 16g + 8 half .. + 7 of key row j, so a lane loads 16 bytes of a key at a time;
@@ -287,7 +289,9 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
 }
 
 // A workgroup's threads are (row, key range, 16-byte piece), `lanes` ranges of a row at a time, up to 8
-// of a thread in flight at once: a round trip to what other workgroups left is all this costs.
+// of a thread in flight at once: a round trip to what other workgroups left is all this costs (3.3-5 us; the
+// last workgroup of a row to arrive joining them in the step kernel instead took 1-5 us more than this
+// launch, for its stores and loads past the XCDs' caches).
 constexpr int kJoinThreads = 512;
 constexpr int kJoinEach = 8;
 __global__ __launch_bounds__(kJoinThreads) void AttendJoinKernel(const float* ml, const float* o, float* out, int32_t rows,

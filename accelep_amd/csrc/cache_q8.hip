@@ -5,6 +5,11 @@
 // large. A unit holds its new rows in registers, takes their largest magnitude, forms the scale
 // (amax / 127, or the stored one where older rows of the block need more), and writes the codes: one
 // pass over the rows. Older rows of the block are only touched when the scale grows.
+//
+// Bound: the bytes, 5 a value each way. 4095 rows of 8 heads of 128: append 10.9 us, 42 MB at 3.9 TB/s
+// (the loads of a unit, then its largest, then its stores: a unit's phases follow one another, and a
+// reduction stands between); 32768 rows read back 52-58 us, 336 MB at 5.8-6.5 TB/s. One row: 3.3 and
+// 2.2 us, launch and two dependent round trips.
 #include <algorithm>
 
 #include "device_common.h"

@@ -5,7 +5,11 @@
 // The angle is formed in fp64, in half turns reduced to [-1, 1], so a position of any size costs
 // no accuracy: what the reduced angle's rounding to fp32 leaves over goes back in to first order
 // (sin(a + d) = sin a + d cos a). One workgroup per row (and part of its heads): its pairs' cos and
-// sin are computed once into LDS, then the heads stream through.
+// sin are computed once into LDS, then the heads stream through (their first loads are on the way
+// while the angles are formed).
+//
+// Bound: the bytes of the values, 8 each in a pass (4096 rows of 40 heads of 128, half of each turned:
+// 168 MB in 33-35 us, 4.8-5.1 TB/s, as a copy); a single row is a launch and one dependent load (2.1 us).
 #include <algorithm>
 
 #include "device_common.h"

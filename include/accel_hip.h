@@ -270,7 +270,7 @@ ACCEL_HIP_API int accel_hip_rope_scaled(AccelHipBuffer states, AccelHipBuffer ou
                                         float magnitude);
 /* A layer's KV cache in 8 bits: codes int8 [capacity, kv_heads, head_dim] and one fp32 scale for each
  * block of `block` tokens and head, [ceil(capacity / block), kv_heads], for keys and values. A value is
- * code * scale. block is a power of two up to 256, head_dim at most 256. */
+ * code * scale, and scales are not negative. block is a power of two up to 256, head_dim at most 256. */
 typedef struct AccelHipCacheQ8 {
   AccelHipBuffer k, v, k_scale, v_scale;
   int64_t capacity, kv_heads, head_dim, block;
