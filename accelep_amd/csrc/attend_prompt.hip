@@ -18,8 +18,8 @@
 // Bound: the matrix cores at the clock that they leave themselves (1.7-1.9 GHz under this load), with the
 // softmax and the split of its weights between their phases. 2048 rows from position 4097 on, 32 heads on
 // 8 of 128: 309 us, 172 GFLOP in two products, 1.11 PFLOP/s of f16; the matrix cores are busy 65 % of the
-// cycles. fp32, 4096 rows in a window of 1024: 231
-// us, 60 GFLOP in three products, 0.78 PFLOP/s; busy 41 %, since each tile of keys is also split there.
+// cycles. fp32, 4096 rows in a window of 1024: 231 us, 60 GFLOP in three products, 0.78 PFLOP/s; busy
+// 41 %, since each tile of keys is also split there.
 // Pieces of 8 codes, whose LDS writes have no bank conflicts (those of 16 have, 8 % of the cycles), took
 // 311 us; fp32 in workgroups of eight waves 225, which a variant of its own was not worth.
 #include "attend_common.h"
