@@ -4,6 +4,7 @@
 #pragma once
 
 #include <algorithm>
+#include <mutex>
 
 #include "device_common.h"
 
@@ -239,10 +240,12 @@ struct WaveParts {
 };
 
 // Into how many key ranges the rows of `units` workgroups are cut: up to per_cu workgroups per CU, at
-// most `most` ranges. Where the partial sums have no room the range stays whole.
+// most `most` ranges. Where the partial sums have no room the range stays whole. Their buffer serves these
+// calls alone, and is held until both launches are queued: calls from several threads take turns.
 struct AttendSplit {
   int32_t count = 1;
   AttendPartial partial{nullptr, nullptr};
+  std::unique_lock<std::mutex> held;
 };
 AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t per_cu, int64_t most);
 

@@ -386,9 +386,12 @@ AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t per_cu, int64
   const size_t ml_bytes = (static_cast<size_t>(parts) * 2 * sizeof(float) + 15) & ~size_t(15);
   const size_t bytes = ml_bytes + static_cast<size_t>(parts * PartialDims(a.dim)) * sizeof(float);
   AttendSplit split;
-  if (count == 1 || !ScratchReady(bytes, kTempFlags, 0)) return split;
+  if (count == 1) return split;
+  static std::mutex mu;
+  split.held = std::unique_lock<std::mutex>(mu);
+  if (!ScratchReady(0, kTempAttend, bytes)) return split;
   split.count = static_cast<int32_t>(count);
-  split.partial.ml = static_cast<float*>(Workspace(bytes));
+  split.partial.ml = static_cast<float*>(Temp(kTempAttend, bytes));
   split.partial.o = split.partial.ml + ml_bytes / sizeof(float);
   return split;
 }

@@ -58,7 +58,8 @@ enum TempSlot {
   kTempSplitA = 4,   // the bf16 GEMM's hi/mid/lo activation image
   kTempRowSums = 5,  // per-tile row sums of squares of a GEMM with a fused RMSNorm
   kTempGreedy = 6,   // the many-workgroup greedy pick's count and keys
-  kTempCount = 7
+  kTempAttend = 7,   // the parts of key ranges (attend_common.h)
+  kTempCount = 8
 };
 void* Temp(TempSlot slot, size_t bytes);
 // Bumped whenever the split-K workspace or a temporary buffer is replaced. A graph captured

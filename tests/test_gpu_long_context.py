@@ -4,6 +4,10 @@ against plain forms in 64 bits (long_context_helpers.py, which also says where e
 from __future__ import annotations
 
 import ctypes as C
+import subprocess
+import sys
+import threading
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -640,6 +644,99 @@ def test_captured_and_replayed():
             for got, want in zip(results(), eager):
                 np.testing.assert_array_equal(got, want)
         check(L.accel_hip_graph_destroy(graph))
+
+
+def test_calls_from_two_threads_keep_their_sums_apart():
+    """Both calls join key ranges in a second launch; the threads' launches meet on the one stream."""
+    r = np.random.default_rng(17)
+    L = lib()
+    jobs = []
+    for seq, heads, kv, dim, length in ((1, 32, 8, 128, 5000), (3, 9, 3, 64, 9000)):
+        cache = Cache(length, kv, dim, 64)
+        cache.fill(r, length)
+        q = dev(r.standard_normal((seq, heads, dim)).astype(np.float32))
+        kf, vf = (dev(cache.values(n)) for n in "kv")
+        outs = [[dev(np.zeros(q.shape, np.float32)) for _ in range(2)] for _ in range(40)]
+
+        def call(out, q=q, cache=cache, kf=kf, vf=vf, seq=seq, heads=heads, kv=kv, dim=dim, length=length):
+            check(L.accel_hip_attention_q8(q.buffer, C.byref(cache.handle), out[0].buffer, seq, length - seq, heads, 0, 0, 0))
+            check(L.accel_hip_attention_window(q.buffer, kf.buffer, vf.buffer, out[1].buffer, seq, length - seq, heads, kv, dim, 0,
+                                               4000, 4))
+
+        want = [dev(np.zeros(q.shape, np.float32)) for _ in range(2)]
+        call(want)
+        jobs.append((call, outs, [w.numpy() for w in want]))
+    failures = []
+
+    def run(call, outs):
+        try:
+            for out in outs:
+                call(out)
+        except BaseException as e:  # handed to the test's thread
+            failures.append(e)
+
+    threads = [threading.Thread(target=run, args=job[:2]) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
+    for _, outs, want in jobs:
+        for out in outs:
+            for got, w in zip(out, want):
+                np.testing.assert_array_equal(got.numpy(), w)
+
+
+FIRST_IN_A_CAPTURE = """
+import ctypes as C, sys
+sys.path[:0] = sys.argv[1:]
+import numpy as np
+from accelep_amd.capi import check, lib
+from hip_helpers import dev
+from long_context_helpers import Cache, assert_within, attend
+L = lib()
+check(L.accel_hip_init())
+r = np.random.default_rng(19)
+for seq in (1, 200):
+    length, heads, kv, dim = 3000, 6, 2, 64
+    cache = Cache(length, kv, dim, 64)
+    cache.fill(r, length)
+    x = r.standard_normal((seq, heads, dim)).astype(np.float32)
+    k, v = cache.values("k"), cache.values("v")
+    q, kf, vf = dev(x), dev(k), dev(v)
+    outs = [dev(np.zeros_like(x)) for _ in range(2)]
+    def step():
+        check(L.accel_hip_attention_q8(q.buffer, C.byref(cache.handle), outs[0].buffer, seq, length - seq, heads, 0, 0, 0))
+        check(L.accel_hip_attention_window(q.buffer, kf.buffer, vf.buffer, outs[1].buffer, seq, length - seq, heads, kv, dim, 0,
+                                           2000, 4))
+    check(L.accel_hip_capture_begin())
+    graph = C.c_void_p()
+    step()
+    check(L.accel_hip_capture_end(C.byref(graph)))
+    exact = [cache.codes[n].astype(np.float64) * np.repeat(cache.scale[n].astype(np.float64), 64, axis=0)[:length, :, None]
+             for n in "kv"]
+    wants = [attend(x, *exact, length - seq, 0, 0, value_scale=cache.value_scale(length)),
+             attend(x, k, v, length - seq, 2000, 4)]
+    for replay in range(3):
+        for o in outs:
+            o.upload(np.full(o.shape, -1.0, np.float32))
+        check(L.accel_hip_graph_launch(graph, 1))
+        for o, want in zip(outs, wants):
+            assert_within(o.numpy(), *want)
+    check(L.accel_hip_graph_destroy(graph))
+    step()
+    for o, want in zip(outs, wants):
+        assert_within(o.numpy(), *want)
+    print("held", seq, flush=True)
+"""
+
+
+def test_a_first_call_inside_a_capture():
+    """Before any eager call there is no room for the parts of a key range: it stays whole."""
+    here = Path(__file__).resolve().parent
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_A_CAPTURE, str(here), str(here.parent)], capture_output=True, text=True,
+                       timeout=100)
+    assert r.returncode == 0 and r.stdout.split() == ["held", "1", "held", "200"], r.stdout + r.stderr
 
 
 def test_frequencies_are_refused_in_a_capture():
