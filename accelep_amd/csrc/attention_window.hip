@@ -76,12 +76,8 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
       for (int c = 0; c < kC; ++c) vx[e][c] = piece(p, 64 * c + 4 * j);
     }
   };
-  int32_t u = begin + wave;
-  if (u < end) {
-    const int32_t t0 = range.Key(u);
-    load_k(t0);
-    load_v(t0);
-  }
+  // The queries are requested first: the first products wait for them and the keys, not for the values
+  // (a step over a window of 4096: 16.9 -> 16.5 us).
   f4 q[kI];
   {
     const float* p = a.q + s * a.q_stride + static_cast<int64_t>(head) * a.dim;
@@ -92,6 +88,13 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
       LoadQuery(a, p, 16 * i + 4 * g, vec, x);
       q[i] = f4{x[0], x[1], x[2], x[3]};
     }
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  int32_t u = begin + wave;
+  if (u < end) {
+    const int32_t t0 = range.Key(u);
+    load_k(t0);
+    load_v(t0);
   }
 
   float m = -INFINITY, l = 0.f;  // l: this lane's share of the row's sum
