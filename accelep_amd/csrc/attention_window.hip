@@ -12,6 +12,15 @@ constexpr int StepWaves(int dp) { return dp > 128 ? 4 : 8; }
 constexpr int kRows = 16;
 constexpr int kKeys = 16;  // of a wave's step
 
+// One argument, not five: less of the host's work for a launch (a step over a window of 4096: 16.5 -> 16.1 us).
+struct StepArgs {
+  AttendArgs a;
+  const float* k;
+  const float* v;
+  int32_t splits;
+  AttendPartial partial;
+};
+
 // One workgroup per (16 rows of a key head, key range); its waves take its steps of 16 keys in turn.
 // Bound: the bytes of the keys that are seen, and over a window the chain of a wave's one or two steps (4100
 // keys, 32 heads on 8 key heads of 128: 33.6 MB in 13.3 us, 2.5 TB/s). Both products run on v_mfma_f32_16x16x4f32, which takes
@@ -25,7 +34,11 @@ constexpr int kKeys = 16;  // of a wave's step
 // holds one (a test of the bits, uniform) has its values taken as zeros and its weights as NaN.
 template <int DP, int kLoad>
 __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
-    AttendArgs a, const float* k, const float* v, int32_t splits, AttendPartial partial) {
+    StepArgs args) {
+  const AttendArgs& a = args.a;
+  const float* k = args.k;
+  const float* v = args.v;
+  const int32_t splits = args.splits;
   const int32_t waves = static_cast<int32_t>(blockDim.x) / 64;
   constexpr int kI = DP / 16;  // 16-byte pieces of a key row per lane
   constexpr int kC = DP / 64;  // of a value row
@@ -192,7 +205,7 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
       *reinterpret_cast<f4*>(&parts.o[wave][j][64 * c + 16 * g + 4 * r]) =
           f4{acc[c][0][r], acc[c][1][r], acc[c][2][r], acc[c][3][r]};
   __syncthreads();
-  parts.Join(a, kv, 1, group, r0, rows, split, splits, partial);
+  parts.Join(a, kv, 1, group, r0, rows, split, splits, args.partial);
 }
 
 template <int DP>
@@ -207,8 +220,9 @@ void LaunchStep(const AttendArgs& a, const float* k, const float* v, bool vec, h
   const int32_t waves = units * steps < cus * kWaves ? 4 : kWaves;
   const AttendSplit split = SplitRange(a, units, 1, steps <= 2 * waves ? 1 : steps / waves);
   const dim3 grid(GridOf(units * split.count, 64 * waves, "Attention is too large")), block(64 * waves);
-  if (vec) hipLaunchKernelGGL((AttendF32StepKernel<DP, 16>), grid, block, 0, stream, a, k, v, split.count, split.partial);
-  else hipLaunchKernelGGL((AttendF32StepKernel<DP, 4>), grid, block, 0, stream, a, k, v, split.count, split.partial);
+  const StepArgs args{a, k, v, split.count, split.partial};
+  if (vec) hipLaunchKernelGGL((AttendF32StepKernel<DP, 16>), grid, block, 0, stream, args);
+  else hipLaunchKernelGGL((AttendF32StepKernel<DP, 4>), grid, block, 0, stream, args);
   Check(hipGetLastError(), "AttendF32StepKernel launch");
   if (split.count > 1) LaunchAttendJoin(a, split.partial, split.count, stream);
 }
