@@ -76,6 +76,19 @@ Q8Cache CheckedCache(const AccelHipCacheQ8* c) {
   return out;
 }
 
+// Whether b covers codes or scales of rows [first, end) of a checked cache; first < end.
+bool OverlapsRows(const AccelHipBuffer& b, size_t bytes, const AccelHipCacheQ8* c, int64_t first, int64_t end) {
+  const auto overlap = [&](const AccelHipBuffer& plane, int64_t from, int64_t to, size_t each) {
+    const AccelHipBuffer part{static_cast<char*>(plane.data) + static_cast<size_t>(from) * each, plane.bytes, 0};
+    return Overlap(b, bytes, part, static_cast<size_t>(to - from) * each);
+  };
+  const size_t code_row = static_cast<size_t>(c->kv_heads * c->head_dim);
+  const size_t scale_row = static_cast<size_t>(c->kv_heads) * sizeof(float);
+  const int64_t first_block = first / c->block, end_block = (end - 1) / c->block + 1;
+  return overlap(c->k, first, end, code_row) || overlap(c->v, first, end, code_row) ||
+         overlap(c->k_scale, first_block, end_block, scale_row) || overlap(c->v_scale, first_block, end_block, scale_row);
+}
+
 // Everything of the two attention calls but the cache. False: nothing to do.
 bool CheckedAttend(const AccelHipBuffer& q, const AccelHipBuffer& out, int64_t seq, int64_t position, int64_t heads,
                    int64_t kv_heads, int64_t dim, int64_t row_stride, int64_t window, int64_t sinks, AttendArgs* a) {
@@ -288,9 +301,7 @@ ACCEL_HIP_API int accel_hip_attention_q8(AccelHipBuffer q, const AccelHipCacheQ8
     if (position + seq > cache->capacity) Invalid("8-bit cache rows are out of range");
     if (!any) return;
     const size_t out_bytes = CheckedBytes(seq, heads * c.dim);
-    const size_t codes = static_cast<size_t>(position + seq) * c.kv_heads * c.dim;
-    if (Overlap(out, out_bytes, cache->k, codes) || Overlap(out, out_bytes, cache->v, codes))
-      Invalid("Attention output overlaps the cache");
+    if (OverlapsRows(out, out_bytes, cache, 0, position + seq)) Invalid("Attention output overlaps the cache");
     NoteDeviceWrite(out.data, sizeof(float));
     LaunchAttentionQ8(a, c, Ctx().stream);
   });
