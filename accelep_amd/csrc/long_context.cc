@@ -76,17 +76,15 @@ Q8Cache CheckedCache(const AccelHipCacheQ8* c) {
   return out;
 }
 
-// Whether b covers codes or scales of rows [first, end) of a checked cache; first < end.
-bool OverlapsRows(const AccelHipBuffer& b, size_t bytes, const AccelHipCacheQ8* c, int64_t first, int64_t end) {
+// Whether b covers codes or scales of rows [first, end) of one plane of a checked cache; first < end.
+bool OverlapsRows(const AccelHipBuffer& b, size_t bytes, const AccelHipCacheQ8* c, const AccelHipBuffer& codes,
+                  const AccelHipBuffer& scales, int64_t first, int64_t end) {
   const auto overlap = [&](const AccelHipBuffer& plane, int64_t from, int64_t to, size_t each) {
     const AccelHipBuffer part{static_cast<char*>(plane.data) + static_cast<size_t>(from) * each, plane.bytes, 0};
     return Overlap(b, bytes, part, static_cast<size_t>(to - from) * each);
   };
-  const size_t code_row = static_cast<size_t>(c->kv_heads * c->head_dim);
-  const size_t scale_row = static_cast<size_t>(c->kv_heads) * sizeof(float);
-  const int64_t first_block = first / c->block, end_block = (end - 1) / c->block + 1;
-  return overlap(c->k, first, end, code_row) || overlap(c->v, first, end, code_row) ||
-         overlap(c->k_scale, first_block, end_block, scale_row) || overlap(c->v_scale, first_block, end_block, scale_row);
+  return overlap(codes, first, end, static_cast<size_t>(c->kv_heads * c->head_dim)) ||
+         overlap(scales, first / c->block, (end - 1) / c->block + 1, static_cast<size_t>(c->kv_heads) * sizeof(float));
 }
 
 // Everything of the two attention calls but the cache. False: nothing to do.
@@ -285,6 +283,12 @@ ACCEL_HIP_API int accel_hip_read_cache_q8(const AccelHipCacheQ8* cache, int64_t 
     float* v = checked(v_out, "cache value output is out of range");
     if (k == nullptr && v == nullptr) return;
     if (k != nullptr && v != nullptr && Overlap(k_out, bytes, v_out, bytes)) Invalid("cache outputs overlap");
+    for (const AccelHipBuffer& out : {k_out, v_out}) {
+      if (out.data == nullptr) continue;
+      if ((k != nullptr && OverlapsRows(out, bytes, cache, cache->k, cache->k_scale, first, end)) ||
+          (v != nullptr && OverlapsRows(out, bytes, cache, cache->v, cache->v_scale, first, end)))
+        Invalid("cache outputs overlap the cache");
+    }
     if (k != nullptr) NoteDeviceWrite(k, bytes);
     if (v != nullptr) NoteDeviceWrite(v, bytes);
     LaunchReadCacheQ8(c, first, count, k, v, Ctx().stream);
@@ -301,7 +305,9 @@ ACCEL_HIP_API int accel_hip_attention_q8(AccelHipBuffer q, const AccelHipCacheQ8
     if (position + seq > cache->capacity) Invalid("8-bit cache rows are out of range");
     if (!any) return;
     const size_t out_bytes = CheckedBytes(seq, heads * c.dim);
-    if (OverlapsRows(out, out_bytes, cache, 0, position + seq)) Invalid("Attention output overlaps the cache");
+    if (OverlapsRows(out, out_bytes, cache, cache->k, cache->k_scale, 0, position + seq) ||
+        OverlapsRows(out, out_bytes, cache, cache->v, cache->v_scale, 0, position + seq))
+      Invalid("Attention output overlaps the cache");
     NoteDeviceWrite(out.data, sizeof(float));
     LaunchAttentionQ8(a, c, Ctx().stream);
   });

@@ -286,7 +286,8 @@ typedef struct AccelHipCacheQ8 {
 ACCEL_HIP_API int accel_hip_append_cache_q8(AccelHipBuffer k, AccelHipBuffer v, const AccelHipCacheQ8* cache,
                                             int64_t seq, int64_t position, int64_t row_stride);
 /* Rows [first, first + count) of the 8-bit cache as fp32 [count, kv_heads, head_dim], code * scale
- * rounded once. k_out or v_out without data leaves that plane out; they may not overlap. */
+ * rounded once. k_out or v_out without data leaves that plane out; they may overlap neither one another
+ * nor the codes and scales that are read. */
 ACCEL_HIP_API int accel_hip_read_cache_q8(const AccelHipCacheQ8* cache, int64_t first, int64_t count,
                                           AccelHipBuffer k_out, AccelHipBuffer v_out);
 /* Attention (as accel_hip_attention: causal, grouped heads, 1 / sqrt(head_dim)) over the 8-bit cache,

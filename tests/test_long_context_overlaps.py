@@ -8,7 +8,7 @@ import ctypes as C
 import pytest
 
 from accelep_amd.capi import lib
-from test_long_context_refusals import buf, cache, refused
+from test_long_context_refusals import NONE, buf, cache, refused
 
 # cache(): 128 rows of 2 heads of 64 in blocks of 32; k, v, k_scale and v_scale lie at 1, 2, 3 and 4 GiB.
 GIB = 1 << 30
@@ -23,3 +23,20 @@ def test_attention_refuses_to_write_into_the_scales(plane, rows, used):
     for at in (0, 4 * (2 * used - 1), 4 - out_bytes):
         refused(L.accel_hip_attention_q8(q, C.byref(cache()), buf(out_bytes, plane * GIB + at), 1, rows - 1, 4, 0, 0, 0),
                 "overlaps the cache")
+
+
+@pytest.mark.parametrize("first,count", [(0, 4), (30, 5), (124, 4)])
+def test_a_read_refuses_to_write_into_what_it_reads(first, count):
+    """The codes and scales of the rows that are read, for either output, alone and together; a plane that is left out
+    is not read."""
+    L, c = lib(), cache()
+    bytes_out, code_row, blocks = 4 * count * 128, 128, (first // 32, (first + count - 1) // 32 + 1)
+    clear = buf(bytes_out)
+    for plane in "kv":
+        codes, scales = (1, 3) if plane == "k" else (2, 4)
+        for begin, size in ((codes * GIB + first * code_row, count * code_row),
+                            (scales * GIB + 8 * blocks[0], 8 * (blocks[1] - blocks[0]))):
+            for at in (begin, begin + size - 4, begin + 4 - bytes_out):
+                out = buf(bytes_out, at)
+                for k_out, v_out in ((out, clear), (clear, out), (out, NONE) if plane == "k" else (NONE, out)):
+                    refused(L.accel_hip_read_cache_q8(C.byref(c), first, count, k_out, v_out), "overlap the cache")
