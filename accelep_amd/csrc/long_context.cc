@@ -40,6 +40,14 @@ bool Overlap(const AccelHipBuffer& a, size_t a_bytes, const AccelHipBuffer& b, s
   return a_bytes > 0 && b_bytes > 0 && x < y + b_bytes && y < x + a_bytes;
 }
 
+// b against `rows` rows of `width` bytes, `stride` bytes apart: what lies between the rows is not theirs.
+bool OverlapsStrided(const AccelHipBuffer& b, size_t bytes, const AccelHipBuffer& to, int64_t rows, size_t stride, size_t width) {
+  if (rows == 0 || !Overlap(b, bytes, to, static_cast<size_t>(rows - 1) * stride + width)) return false;
+  if (b.data <= to.data) return true;
+  const size_t in_row = static_cast<size_t>(static_cast<const char*>(b.data) - static_cast<const char*>(to.data)) % stride;
+  return in_row < width || bytes > stride - in_row;
+}
+
 void RequireAligned(const AccelHipBuffer& b, size_t to, const char* what) {
   if (reinterpret_cast<uintptr_t>(b.data) % to != 0) Invalid(what);
 }
@@ -212,6 +220,12 @@ ACCEL_HIP_API int accel_hip_rope_scaled(AccelHipBuffer states, AccelHipBuffer ou
       RequireBytes(positions, CheckedIntBytes(seq), "Rope positions are out of range");
       RequireAligned(positions, sizeof(int32_t), "Rope positions are not aligned");
     }
+    // Other workgroups may still read them.
+    const size_t stride_bytes = static_cast<size_t>(stride) * sizeof(float), row_bytes = static_cast<size_t>(row) * sizeof(float);
+    if (OverlapsStrided(frequencies, static_cast<size_t>(rotary_dim / 2) * sizeof(double), out, seq, stride_bytes, row_bytes))
+      Invalid("Rope output overlaps the frequencies");
+    if (rotary_dim > 0 && OverlapsStrided(positions, CheckedIntBytes(seq), out, seq, stride_bytes, row_bytes))
+      Invalid("Rope output overlaps the positions");
     NoteDeviceWrite(out.data, bytes);
     RopeScaledArgs a;
     a.states = static_cast<const float*>(states.data);

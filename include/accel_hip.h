@@ -262,7 +262,7 @@ ACCEL_HIP_API int accel_hip_rope_frequencies(const AccelHipRopeScaling* scaling,
  * multiplies them with magnitude; the other dims come out as they are. states and out are rows of
  * n_heads * head_dim floats (and row_stride apart both; what lies behind a row's heads is left alone):
  * the query and key heads of a fused projection's rows turn in one call. out may be states itself, and
- * may not overlap it otherwise. position_s is position + s, or position + positions[s] where positions
+ * may not overlap it otherwise, nor the frequencies and positions. position_s is position + s, or position + positions[s] where positions
  * (int32 [seq]) has data. Angles are formed in 64 bits: position_s counts up to 2^32. */
 ACCEL_HIP_API int accel_hip_rope_scaled(AccelHipBuffer states, AccelHipBuffer out, AccelHipBuffer frequencies,
                                         AccelHipBuffer positions, int64_t seq, int64_t n_heads, int64_t head_dim,

@@ -40,3 +40,21 @@ def test_a_read_refuses_to_write_into_what_it_reads(first, count):
                 out = buf(bytes_out, at)
                 for k_out, v_out in ((out, clear), (clear, out), (out, NONE) if plane == "k" else (NONE, out)):
                     refused(L.accel_hip_read_cache_q8(C.byref(c), first, count, k_out, v_out), "overlap the cache")
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("stride", [0, 160])
+def test_rope_refuses_to_write_into_its_frequencies_and_positions(in_place, stride):
+    """3 rows of 2 heads of 64; 32 frequencies of 8 bytes and 3 positions of 4."""
+    L, out = lib(), buf(1 << 20, GIB)
+    x = out if in_place else buf(1 << 20, 2 * GIB)
+    row, apart = 4 * 128, 4 * (stride or 128)
+    f, p = buf(256, 3 * GIB), buf(12, 4 * GIB)
+
+    def rope(f=f, p=p, rotary=64):
+        return L.accel_hip_rope_scaled(x, out, f, p, 3, 2, 64, stride, rotary, 0, 0, 1.0)
+
+    for at in (0, 8, row - 8, apart, 2 * apart + row - 8, 8 - 256, apart + 8 - 256):
+        refused(rope(f=buf(256, GIB + at)), "overlaps the frequencies")
+    for at in (0, 4, row - 4, 2 * apart + row - 4, 4 - 12, 2 * apart + 4 - 12):
+        refused(rope(p=buf(12, GIB + at)), "overlaps the positions")
