@@ -7,7 +7,8 @@
   host/*.cc) over the C-ABI.
 * tests/cpp/bin/*: the C++ tests (tests/cpp/*.cc), linked against both, and
   libbpe_host.so (tests/cpp/lib/bpe_host.cc over csrc/tokenizer.cc, no HIP) for the CPU
-  tokenizer tests.
+  tokenizer tests, and libscratch_host.so (tests/cpp/lib/scratch_host.cc over csrc/context.cc,
+  with a HIP runtime of host memory) for the CPU tests of the workspaces.
 
     python -m accelep_amd.build          # or: python accelep_amd/build.py
 """
@@ -99,6 +100,13 @@ def _build_bpe_host() -> Path:
     return out
 
 
+def _build_scratch_host() -> Path:
+    out = CPP_TEST_BIN / "libscratch_host.so"
+    _run(["g++", *GXX_FLAGS, "-shared", "-Wl,-Bsymbolic", "-Wl,-z,defs", "-pthread", "-o", str(out),
+          str(CPP_TESTS / "lib" / "scratch_host.cc"), str(CSRC / "context.cc")])
+    return out
+
+
 def build(verbose: bool = False) -> Path:
     """Compiles every source and links the library. Always rebuilds."""
     BUILD.mkdir(exist_ok=True)
@@ -117,6 +125,7 @@ def build(verbose: bool = False) -> Path:
     with ThreadPoolExecutor(max_workers=max(1, min(len(tests), jobs))) as pool:
         list(pool.map(_build_cpp_test, tests))
     _build_bpe_host()
+    _build_scratch_host()
     if verbose:
         print(f"built {LIB}, {RUNTIME_LIB} and {len(tests)} C++ test programs")
     return LIB

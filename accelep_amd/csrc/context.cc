@@ -203,7 +203,8 @@ bool WorkspaceFits(size_t bytes) {
 }
 
 // Workspaces only grow. A replaced block goes to the deferred frees and the generation moves,
-// so a graph captured before the growth is refused rather than replayed into freed memory.
+// so a graph captured before the growth is refused rather than replayed into freed memory. The new
+// block is there first: where there is no memory for it, all stays as it was.
 void* Workspace(size_t bytes) {
   if (void* p = FromArena(bytes, "split-K workspace")) return p;
   Context& ctx = Ctx();
@@ -211,11 +212,12 @@ void* Workspace(size_t bytes) {
   if (bytes > ctx.workspace_bytes) {
     RefuseInCapture("growing the split-K workspace");
     Check(hipStreamSynchronize(ctx.stream), "hipStreamSynchronize");
-    if (ctx.workspace != nullptr) DeferFree(ctx.workspace);
-    ctx.workspace = nullptr;
-    BumpGeneration();
     const size_t grown = std::max(bytes, ctx.workspace_bytes * 2);
-    Check(hipMalloc(&ctx.workspace, grown), "hipMalloc(workspace)");
+    void* block = nullptr;
+    Check(hipMalloc(&block, grown), "hipMalloc(workspace)");
+    DeferFree(ctx.workspace);
+    BumpGeneration();
+    ctx.workspace = block;
     ctx.workspace_bytes = grown;
   }
   return ctx.workspace;
@@ -252,14 +254,17 @@ void* Temp(TempSlot slot, size_t bytes) {
   if (bytes > sizes[slot]) {
     RefuseInCapture("growing a temporary buffer");
     Check(hipStreamSynchronize(ctx.stream), "hipStreamSynchronize");
-    if (buffers[slot] != nullptr) DeferFree(buffers[slot]);
-    buffers[slot] = nullptr;
-    BumpGeneration();
     const size_t grown = std::max<size_t>(bytes, std::max<size_t>(sizes[slot] * 2, 256));
-    Check(hipMalloc(&buffers[slot], grown), "hipMalloc(temp)");
+    void* block = nullptr;
+    Check(hipMalloc(&block, grown), "hipMalloc(temp)");
     // On the library stream: a null-stream memset is not ordered against it (the stream is
     // non-blocking) and could land after a kernel that already wrote the new buffer.
-    Check(hipMemsetAsync(buffers[slot], 0, grown, ctx.stream), "hipMemsetAsync(temp)");
+    const hipError_t cleared = hipMemsetAsync(block, 0, grown, ctx.stream);
+    if (cleared != hipSuccess) DeferFree(block);
+    Check(cleared, "hipMemsetAsync(temp)");
+    DeferFree(buffers[slot]);
+    BumpGeneration();
+    buffers[slot] = block;
     sizes[slot] = grown;
   }
   return buffers[slot];

@@ -1,0 +1,61 @@
+"""The library's workspaces where the GPU has no memory left: context.cc over a HIP runtime of host memory
+(tests/cpp/lib/scratch_host.cc), so these tests need no GPU."""
+
+from __future__ import annotations
+
+import ctypes as C
+import shutil
+from pathlib import Path
+
+import pytest
+
+HOST_SO = Path(__file__).resolve().parent / "cpp" / "bin" / "libscratch_host.so"
+OK, BAD_ALLOC, TEMP_ATTEND = 0, 4, 7
+
+
+@pytest.fixture
+def host(tmp_path):
+    """The library anew: a copy of the file has state of its own."""
+    at = tmp_path / "libscratch_host.so"
+    shutil.copy(HOST_SO, at)
+    lib = C.CDLL(str(at))
+    lib.scratch_host_refuse_from.argtypes = [C.c_size_t]
+    lib.scratch_host_generation.restype = C.c_uint64
+    lib.scratch_host_block.argtypes, lib.scratch_host_block.restype = [C.c_void_p], C.c_size_t
+    return lib
+
+
+def temp(host, size):
+    out = C.c_void_p()
+    return host.scratch_host_temp(TEMP_ATTEND, C.c_size_t(size), C.byref(out)), out.value
+
+
+def workspace(host, size):
+    out = C.c_void_p()
+    return host.scratch_host_workspace(C.c_size_t(size), C.byref(out)), out.value
+
+
+@pytest.mark.parametrize("get", [temp, workspace])
+def test_a_workspace_that_cannot_grow_stays_as_it_was(host, get):
+    rc, first = get(host, 1000)
+    assert rc == OK and host.scratch_host_block(first) >= 1000
+    generation = host.scratch_host_generation()
+    host.scratch_host_refuse_from(1500)
+    assert get(host, 5000)[0] == BAD_ALLOC
+    for size in (1000, 10):  # what fits is served from memory that is there
+        rc, again = get(host, size)
+        assert rc == OK and again == first and host.scratch_host_block(again) >= size
+    assert host.scratch_host_generation() == generation  # captured graphs still point to it
+    host.scratch_host_refuse_from(1 << 62)
+    rc, grown = get(host, 5000)
+    assert rc == OK and host.scratch_host_block(grown) >= 5000 and host.scratch_host_generation() > generation
+
+
+@pytest.mark.parametrize("get", [temp, workspace])
+def test_a_first_workspace_that_there_is_no_memory_for(host, get):
+    host.scratch_host_refuse_from(1)
+    assert get(host, 1000)[0] == BAD_ALLOC
+    assert get(host, 10)[0] == BAD_ALLOC
+    host.scratch_host_refuse_from(1 << 62)
+    rc, p = get(host, 10)
+    assert rc == OK and host.scratch_host_block(p) >= 10
