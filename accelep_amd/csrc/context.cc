@@ -109,6 +109,7 @@ void ClearLastError() { g_error.clear(); }
 
 void Check(hipError_t status, const char* what) {
   if (status != hipSuccess) {
+    (void)hipGetLastError();  // reported here, and not by the next kernel launch's check again
     Fail(status == hipErrorOutOfMemory ? ACCEL_HIP_BAD_ALLOC : ACCEL_HIP_RUNTIME_ERROR,
          std::string(what) + ": " + hipGetErrorString(status));
   }
@@ -347,10 +348,14 @@ ACCEL_HIP_API int accel_hip_allocate(size_t bytes, AccelHipBuffer* out) {
     if (ptr == nullptr) {
       hipError_t st = hipMalloc(&ptr, block);
       if (st == hipErrorOutOfMemory) {
+        (void)hipGetLastError();
         accel_hip_trim();
         st = hipMalloc(&ptr, block);
       }
-      if (st != hipSuccess || ptr == nullptr) throw std::bad_alloc();
+      if (st != hipSuccess || ptr == nullptr) {
+        (void)hipGetLastError();
+        throw std::bad_alloc();
+      }
     }
     Check(hipMemsetAsync(ptr, 0, block, ctx.stream), "hipMemsetAsync");
     const uint64_t id = g_next_id.fetch_add(1, std::memory_order_relaxed);

@@ -59,3 +59,18 @@ def test_a_first_workspace_that_there_is_no_memory_for(host, get):
     host.scratch_host_refuse_from(1 << 62)
     rc, p = get(host, 10)
     assert rc == OK and host.scratch_host_block(p) >= 10
+
+
+@pytest.mark.parametrize("get", [temp, workspace])
+def test_a_failed_allocation_is_reported_once(host, get):
+    """Kernel launches ask HIP for the thread's last error: a reported one may not be there any more."""
+    host.scratch_host_refuse_from(1)
+    assert get(host, 1000)[0] == BAD_ALLOC
+    assert host.scratch_host_last_error() == 0
+
+
+def test_a_failed_device_allocation_is_reported_once(host):
+    out = (C.c_uint64 * 3)()
+    host.scratch_host_refuse_from(1)
+    assert host.accel_hip_allocate(C.c_size_t(1000), out) == BAD_ALLOC
+    assert host.scratch_host_last_error() == 0
