@@ -7,8 +7,8 @@
   host/*.cc) over the C-ABI.
 * tests/cpp/bin/*: the C++ tests (tests/cpp/*.cc), linked against both, and
   libbpe_host.so (tests/cpp/lib/bpe_host.cc over csrc/tokenizer.cc, no HIP) for the CPU
-  tokenizer tests, and libscratch_host.so (tests/cpp/lib/scratch_host.cc over csrc/context.cc,
-  with a HIP runtime of host memory) for the CPU tests of the workspaces.
+  tokenizer tests, and libscratch_host.so (tests/cpp/lib/scratch_host.cc over csrc/context.cc
+  and attend_split.cc, with a HIP runtime of host memory) for the CPU tests of the workspaces.
 
     python -m accelep_amd.build          # or: python accelep_amd/build.py
 """
@@ -103,7 +103,7 @@ def _build_bpe_host() -> Path:
 def _build_scratch_host() -> Path:
     out = CPP_TEST_BIN / "libscratch_host.so"
     _run(["g++", *GXX_FLAGS, "-shared", "-Wl,-Bsymbolic", "-Wl,-z,defs", "-pthread", "-o", str(out),
-          str(CPP_TESTS / "lib" / "scratch_host.cc"), str(CSRC / "context.cc")])
+          str(CPP_TESTS / "lib" / "scratch_host.cc"), str(CSRC / "context.cc"), str(CSRC / "attend_split.cc")])
     return out
 
 

@@ -4,8 +4,8 @@
 #pragma once
 
 #include <algorithm>
-#include <mutex>
 
+#include "attend_split.h"
 #include "device_common.h"
 
 namespace accel_hip {
@@ -178,14 +178,6 @@ __device__ __forceinline__ bool QueryVec(const AttendArgs& a) {  // uniform
   return a.dim % 4 == 0 && a.q_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
 }
 
-// Partial results of key ranges: of each (row, range) the reference m and the sum l, and the weighted
-// sum of PartialDims(dim) floats, 16-byte aligned.
-inline __host__ __device__ int32_t PartialDims(int32_t dim) { return (dim + 3) & ~3; }
-struct AttendPartial {
-  float* ml;  // [rows][splits][2]
-  float* o;   // [rows][splits][PartialDims]
-};
-
 // The results of a workgroup's waves for kRows rows meet in LDS. Wave w serves head w % heads of the
 // workgroup's `heads` key heads and has every (waves / heads)-th step of the key range: each row's joined
 // (m, l, sum) goes to `partial`, or with one key range the quotient to the output.
@@ -238,16 +230,6 @@ struct WaveParts {
     }
   }
 };
-
-// Into how many key ranges the rows of `units` workgroups are cut: up to per_cu workgroups per CU, at
-// most `most` ranges. Where the partial sums have no room the range stays whole. Their buffer serves these
-// calls alone, and is held until both launches are queued: calls from several threads take turns.
-struct AttendSplit {
-  int32_t count = 1;
-  AttendPartial partial{nullptr, nullptr};
-  std::unique_lock<std::mutex> held;
-};
-AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t per_cu, int64_t most);
 
 // Joins the key ranges of each row into the output (attention_q8.hip).
 void LaunchAttendJoin(const AttendArgs& a, const AttendPartial& partial, int32_t splits, hipStream_t stream);

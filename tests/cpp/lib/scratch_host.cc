@@ -1,4 +1,4 @@
-// The library's process state (accelep_amd/csrc/context.cc) over a HIP runtime of host memory, for the CPU
+// The library's process state (accelep_amd/csrc/context.cc) and the division of key ranges (attend_split.cc) over a HIP runtime of host memory, for the CPU
 // tests of what happens when an allocation fails. TEST INFRASTRUCTURE ONLY: the functions below stand in for
 // the HIP runtime's and the kernel files'. A failed call leaves its error for hipGetLastError, as HIP does.
 #include <hip/hip_runtime_api.h>
@@ -8,6 +8,7 @@
 #include <map>
 #include <mutex>
 
+#include "attend_split.h"
 #include "common.h"
 #include "host_util.h"
 
@@ -134,4 +135,18 @@ HOST_API int scratch_host_temp(int slot, size_t bytes, void** out) {
 }
 HOST_API int scratch_host_workspace(size_t bytes, void** out) {
   return Guard([&] { *out = Workspace(bytes); });
+}
+// Into how many ranges an attention call of one row of `heads` heads of `dim` is cut.
+HOST_API int scratch_host_split(int heads, int dim, int64_t most, int* count) {
+  return Guard([&] {
+    AttendArgs a{};
+    a.seq = 1;
+    a.heads = heads;
+    a.kv_heads = 1;
+    a.dim = dim;
+    const AttendSplit split = SplitRange(a, 1, 1, most);
+    *count = split.count;
+    const size_t bytes = static_cast<size_t>(split.count) * heads * (2 + PartialDims(dim)) * sizeof(float);
+    if (split.count > 1 && scratch_host_block(split.partial.ml) < bytes) Fail(ACCEL_HIP_LOGIC_ERROR, "the parts have no room");
+  });
 }

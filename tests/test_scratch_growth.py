@@ -1,4 +1,4 @@
-"""The library's workspaces where the GPU has no memory left: context.cc over a HIP runtime of host memory
+"""The library's workspaces where the GPU has no memory left: context.cc and attend_split.cc over a HIP runtime of host memory
 (tests/cpp/lib/scratch_host.cc), so these tests need no GPU."""
 
 from __future__ import annotations
@@ -74,3 +74,19 @@ def test_a_failed_device_allocation_is_reported_once(host):
     host.scratch_host_refuse_from(1)
     assert host.accel_hip_allocate(C.c_size_t(1000), out) == BAD_ALLOC
     assert host.scratch_host_last_error() == 0
+
+
+def split(host, most, heads=32, dim=128):
+    count = C.c_int()
+    return host.scratch_host_split(heads, dim, C.c_int64(most), C.byref(count)), count.value
+
+
+def test_a_key_range_whose_parts_have_no_memory_stays_whole(host):
+    assert split(host, 8) == (OK, 8)
+    host.scratch_host_refuse_from(1)
+    assert split(host, 4) == (OK, 4)  # room that is there
+    assert split(host, 200) == (OK, 1)
+    assert split(host, 8) == (OK, 8)
+    assert host.scratch_host_last_error() == 0
+    host.scratch_host_refuse_from(1 << 62)
+    assert split(host, 200) == (OK, 200)
