@@ -12,8 +12,7 @@ AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t per_cu, int64
   const size_t bytes = ml_bytes + static_cast<size_t>(parts * PartialDims(a.dim)) * sizeof(float);
   AttendSplit split;
   if (count == 1) return split;
-  static std::mutex mu;
-  split.held = std::unique_lock<std::mutex>(mu);
+  split.held = std::unique_lock<std::mutex>(AttendPartsMutex());
   if (!ScratchReady(0, kTempAttend, bytes)) return split;
   try {
     split.partial.ml = static_cast<float*>(Temp(kTempAttend, bytes));

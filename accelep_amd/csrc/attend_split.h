@@ -18,7 +18,7 @@ struct AttendPartial {
 // Into how many key ranges the rows of `units` workgroups are cut: up to per_cu workgroups per CU, at
 // most `most` ranges. Where the partial sums have no room (no memory is left, or a capture runs and the
 // buffer is too small) the range stays whole. Their buffer serves these calls alone, and is held until both
-// launches are queued: calls from several threads take turns.
+// launches are queued: calls from several threads, and replays of graphs, take turns.
 struct AttendSplit {
   int32_t count = 1;
   AttendPartial partial{nullptr, nullptr};

@@ -6,6 +6,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -62,6 +63,9 @@ enum TempSlot {
   kTempCount = 8
 };
 void* Temp(TempSlot slot, size_t bytes);
+// Held while launches that use the kTempAttend parts are queued: by an attention call from before it asks for
+// them until its join is queued, and by a graph's replay, whose kernels may use them too.
+std::mutex& AttendPartsMutex();
 // Bumped whenever the split-K workspace or a temporary buffer is replaced. A graph captured
 // under an older value may point into a replaced block: accel_hip_graph_launch refuses it.
 uint64_t Generation();

@@ -229,6 +229,11 @@ void* g_temp[kTempCount] = {};
 size_t g_temp_bytes[kTempCount] = {};
 }  // namespace
 
+std::mutex& AttendPartsMutex() {
+  static std::mutex mu;
+  return mu;
+}
+
 bool ScratchReady(size_t workspace_bytes, TempSlot slot, size_t temp_bytes) {
   if (const Arena* arena = g_arena; arena != nullptr) {
     const size_t start = (arena->used + 255) & ~size_t(255);
@@ -563,6 +568,8 @@ ACCEL_HIP_API int accel_hip_graph_launch(void* graph_exec, int32_t times) {
     if (graph_exec == nullptr) Fail(ACCEL_HIP_INVALID_ARGUMENT, "null graph");
     Context& ctx = Ctx();
     const GraphHandle* g = static_cast<const GraphHandle*>(graph_exec);
+    // Before the check: the parts do not move until the launches are queued.
+    std::lock_guard<std::mutex> parts(AttendPartsMutex());
     if (!GraphIsCurrent(g))
       Fail(ACCEL_HIP_RUNTIME_ERROR,
            "stale HIP graph: device memory it points into (a staged weight copy, the split-K workspace or a "

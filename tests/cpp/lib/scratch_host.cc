@@ -136,6 +136,20 @@ HOST_API int scratch_host_temp(int slot, size_t bytes, void** out) {
 HOST_API int scratch_host_workspace(size_t bytes, void** out) {
   return Guard([&] { *out = Workspace(bytes); });
 }
+// The parts of key ranges, held by this thread until the release.
+namespace {
+AttendSplit g_held;
+}
+HOST_API int scratch_host_hold_parts() {
+  return Guard([&] {
+    AttendArgs a{};
+    a.seq = a.heads = a.kv_heads = 1;
+    a.dim = 64;
+    g_held = SplitRange(a, 1, 1, 8);
+    if (g_held.count != 8) Fail(ACCEL_HIP_LOGIC_ERROR, "the range is whole");
+  });
+}
+HOST_API void scratch_host_release_parts() { g_held = AttendSplit{}; }
 // Into how many ranges an attention call of one row of `heads` heads of `dim` is cut.
 HOST_API int scratch_host_split(int heads, int dim, int64_t most, int* count) {
   return Guard([&] {

@@ -5,12 +5,13 @@ from __future__ import annotations
 
 import ctypes as C
 import shutil
+import threading
 from pathlib import Path
 
 import pytest
 
 HOST_SO = Path(__file__).resolve().parent / "cpp" / "bin" / "libscratch_host.so"
-OK, BAD_ALLOC, TEMP_ATTEND = 0, 4, 7
+OK, BAD_ALLOC, RUNTIME_ERROR, TEMP_ATTEND = 0, 4, 5, 7
 
 
 @pytest.fixture
@@ -90,3 +91,40 @@ def test_a_key_range_whose_parts_have_no_memory_stays_whole(host):
     assert host.scratch_host_last_error() == 0
     host.scratch_host_refuse_from(1 << 62)
     assert split(host, 200) == (OK, 200)
+
+
+def test_a_graph_waits_for_the_parts_that_another_thread_uses(host):
+    """A captured attention call writes its parts to the same memory: a replay may not come between another thread's
+    two launches."""
+    graph = C.c_void_p()
+    assert host.scratch_host_hold_parts() == OK
+    host.scratch_host_release_parts()
+    assert host.accel_hip_capture_begin() == OK and host.accel_hip_capture_end(C.byref(graph)) == OK
+    launched = []
+    other = threading.Thread(target=lambda: launched.append(host.accel_hip_graph_launch(graph, 2)))
+    assert host.scratch_host_hold_parts() == OK
+    other.start()
+    other.join(0.3)
+    waited = not launched
+    host.scratch_host_release_parts()
+    other.join(10)
+    assert waited and launched == [OK]
+    assert host.accel_hip_graph_destroy(graph) == OK
+
+
+def test_a_graph_is_refused_once_the_parts_moved(host):
+    """Also where they move while the replay waits for them."""
+    graph = C.c_void_p()
+    assert split(host, 8) == (OK, 8)
+    assert host.accel_hip_capture_begin() == OK and host.accel_hip_capture_end(C.byref(graph)) == OK
+    assert host.accel_hip_graph_launch(graph, 1) == OK
+    launched = []
+    other = threading.Thread(target=lambda: launched.append(host.accel_hip_graph_launch(graph, 1)))
+    assert host.scratch_host_hold_parts() == OK
+    other.start()
+    other.join(0.3)
+    rc = temp(host, 1 << 24)[0]
+    host.scratch_host_release_parts()
+    other.join(10)
+    assert rc == OK and launched == [RUNTIME_ERROR]
+    assert host.accel_hip_graph_destroy(graph) == OK
