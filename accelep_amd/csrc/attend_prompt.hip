@@ -214,7 +214,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
 
   // ---- the rows' queries ----
   h8 qh[kSteps], ql[kSteps];
-  float row_factor;
+  float row_back;  // a power of two: takes the row's scale out of its scores again
   {
     const float* q = a.q + s * a.q_stride + static_cast<int64_t>(head) * a.dim;
     const bool vec = QueryVec(a);
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
     top = max(top, XorLane<32>(top));
     const bool bad = top >= 0x7f800000u;
     const float scale = RowScale(top);
-    row_factor = a.factor / scale;  // by a power of two
+    row_back = 1.f / scale;
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
       h2 hi[4], lo[4];
@@ -295,11 +295,11 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
           for (int r4 = 0; r4 < 4; ++r4) {
             const f4 f = *reinterpret_cast<const f4*>(&sk[buf][32 * h + 8 * r4 + 4 * g]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) st[h][4 * r4 + e] *= f[e];
+            for (int e = 0; e < 4; ++e) st[h][4 * r4 + e] *= f[e] * row_back;  // the scales first: they may be far from 1
           }
       }
-      float c = row_factor;
-      if (one_scale) c *= kF32 ? 1.f / kCommonScale : ks;
+      float c = a.factor;
+      if (one_scale) c *= row_back * (kF32 ? 1.f / kCommonScale : ks);
       if (!whole) {
 #pragma unroll
         for (int h = 0; h < kSub; ++h)

@@ -100,7 +100,7 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
   }
   // The row's queries: piece (c, half) of dims 64c + 16g + 8 half .. + 7.
   h8 qh[kC][2], ql[kC][2];
-  float row_factor;
+  float row_back;  // a power of two: takes the row's scale out of its scores again
   {
     float x[kC][16];
     const float* q = a.q + s * a.q_stride + static_cast<int64_t>(head) * a.dim;
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
     top = max(top, XorLane<32>(top));
     const bool bad = top >= 0x7f800000u;  // no finite row: all of it NaN
     const float scale = RowScale(top);
-    row_factor = a.factor / scale;  // by a power of two
+    row_back = 1.f / scale;
 #pragma unroll
     for (int i = 0; i < kC; ++i)
 #pragma unroll
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
       for (int e = 0; e < kEach; ++e) {
         // A value scale that is not finite makes the scores NaN, and a weight of 0 stays one.
         const bool finite = fabsf(vs[h][e]) < INFINITY;
-        factor[h][e] = finite ? row_factor * ks[h][e] : NAN;
+        factor[h][e] = finite ? row_back * ks[h][e] * a.factor : NAN;
         value[h][e] = finite ? vs[h][e] : 0.f;
       }
     if (next >= 0) {

@@ -1,0 +1,81 @@
+"""Attention over keys and values near the ends of fp32's range: what is finite in 64 bits and fits fp32 comes out so."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from long_context_helpers import Cache, assert_within, attend, attention_q8_call, attention_window_call, check, lib
+
+pytestmark = pytest.mark.gpu
+
+Q8, F32 = 6 << 20, 3 << 20  # pairs of rows and keys from which the kernel of many rows is taken
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    check(lib().accel_hip_init())
+    yield
+
+
+def takes_many_rows(pairs, seq, position, heads, kv_heads, window=0, sinks=0):
+    """The library's choice of kernel, from the sizes."""
+    group, end = heads // kv_heads, position + seq
+    rows = seq * group
+    keys = end if window == 0 or window >= end else min(end, window + min(seq, (14 + group) // group + 1) + 32)
+    steps = -(-keys // 32) + (0 if window == 0 or window >= end else -(-min(sinks, end) // 32))
+    each = steps * 32 * kv_heads
+    return rows > 16 and -(-rows // 16) * 16 >= -(-pairs // each)
+
+
+def many(q, copies, pairs, position, kv_heads, window=0, sinks=0):
+    """`copies` of each query head: one for the kernel of few rows, more for the one of many."""
+    out = np.repeat(q, copies, axis=1)
+    assert takes_many_rows(pairs, q.shape[0], position, out.shape[1], kv_heads, window, sinks) == (copies > 1)
+    return out
+
+
+# (seq, length, copies): few rows over a range in one part and in several; many rows, the same.
+SIZES = [(3, 50, 1), (2, 9000, 1), (17, 30000, 16), (200, 600, 512)]
+SIZE_IDS = ["few", "few-long", "many-divided", "many"]
+
+
+@pytest.mark.parametrize("seq,length,copies", SIZES, ids=SIZE_IDS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (33, 4)])
+@pytest.mark.parametrize("large", [100, 119])
+def test_window_attention_of_large_keys_and_small_queries(seq, length, copies, window, sinks, large):
+    """Keys of 2^large and more with queries that make ordinary scores of them: rows of scales of their own."""
+    r = np.random.default_rng(41)
+    position = length - seq
+    while copies > 1 and not takes_many_rows(F32, seq, position, 2 * copies, 2, window, sinks):
+        copies *= 2  # a window is short
+    q, k, v = (r.standard_normal(s).astype(np.float32) for s in ((seq, 2, 64), (length, 2, 64), (length, 2, 64)))
+    q *= np.float32(2.0 ** -large)
+    k *= (2.0 ** (large + r.integers(-2, 5, (length, 2, 1)))).astype(np.float32)
+    some = np.unique(np.r_[0:seq:7, seq - 1])
+    want, bound = attend(q, k, v, position, window, sinks, some)
+    got = attention_window_call(many(q, copies, F32, position, 2, window, sinks), k, v, position, window, sinks)
+    assert_within(got[some, ::copies], want, bound)
+
+
+@pytest.mark.parametrize("seq,length,copies", SIZES, ids=SIZE_IDS)
+@pytest.mark.parametrize("block", [1, 16, 64])
+@pytest.mark.parametrize("large", [100, 119])
+def test_attention_q8_of_large_keys_and_small_queries(seq, length, copies, block, large):
+    r = np.random.default_rng(42)
+    position = length - seq
+    cache = Cache(length, 2, 64, block)
+    cache.fill(r, length)
+    cache.scale["k"] *= np.float32(2.0 ** large)
+    cache.upload()
+    q = (r.standard_normal((seq, 2, 64)) * 2.0 ** -large).astype(np.float32)
+    some = np.unique(np.r_[0:seq:7, seq - 1])
+    want, bound = attend(q, cache.values("k"), cache.values("v"), position, 0, 0, some, cache.value_scale(length))
+    got = attention_q8_call(many(q, copies, Q8, position, 2), cache, position)
+    assert_within(got[some, ::copies], want, bound)
+
+
+def large_values(r, shape, signs):
+    """Between a third and nearly all of the largest float."""
+    x = r.uniform(1.2e38, 3.3e38, shape)
+    return (x * r.choice([-1.0, 1.0], shape) if signs else x).astype(np.float32)
