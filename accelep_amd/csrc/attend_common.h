@@ -87,6 +87,8 @@ __device__ __forceinline__ h8 Join(h2 a, h2 b, h2 c, h2 d) { return h8{a[0], a[1
 // 2^power, with top * 2^power kept in [2^3, 2^15): a weight then has 22 bits down to 2^-6 of the largest
 // and is off by 2^-28 of that below, whatever the scales, and a key that a row does not see has no say.
 constexpr int32_t kPowerMax = 127;
+// From this power on the sum of up to 2^31 keys is less than 2^100 when the power is taken out.
+constexpr int32_t kFarPower = -40;
 __device__ __forceinline__ int32_t WeightPower(float top, int32_t power) {
   const float at = ldexpf(top, power);
   if (at < 0x1p15f && (at >= 8.f || !(top > 0.f))) return power;
@@ -178,6 +180,12 @@ __device__ __forceinline__ bool QueryVec(const AttendArgs& a) {  // uniform
   return a.dim % 4 == 0 && a.q_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
 }
 
+// A part of a row's keys leaves (m, l, o): its reference, the sum of its weights, and the sum o of weight *
+// value. Where that sum may pass the largest float (its quotient does not) it is held times 2^-64, and l is
+// negative as a sign of it.
+constexpr int32_t kFarShift = 64;
+constexpr float kFarDown = 0x1p-64f, kFarUp = 0x1p64f;
+
 // The results of a workgroup's waves for kRows rows meet in LDS. Wave w serves head w % heads of the
 // workgroup's `heads` key heads and has every (waves / heads)-th step of the key range: each row's joined
 // (m, l, sum) goes to `partial`, or with one key range the quotient to the output.
@@ -200,12 +208,29 @@ struct WaveParts {
       float big = -INFINITY;
       for (int32_t w = h; w < waves; w += heads) big = fmaxf(big, m[w][rl]);
       const float base = big == -INFINITY ? 0.f : big;
-      float total = 0.f;
+      float total = 0.f, low = 0.f;
       f4 x = f4{0.f, 0.f, 0.f, 0.f};
       for (int32_t w = h; w < waves; w += heads) {
         const float wt = __builtin_amdgcn_exp2f(m[w][rl] - base);
+        low = fminf(low, l[w][rl]);
         total += wt * l[w][rl];
         x += wt * *reinterpret_cast<const f4*>(&o[w][rl][d]);
+      }
+      float up = 1.f;
+      if (low < 0.f) {  // some parts are held times 2^-64: the sum is then too, unless they count for little
+        float most = 0.f;
+        for (int32_t w = h; w < waves; w += heads)
+          if (l[w][rl] < 0.f) most = fmaxf(most, __builtin_amdgcn_exp2f(m[w][rl] - base));
+        const bool far = most >= 0x1p-60f;
+        total = 0.f;
+        x = f4{0.f, 0.f, 0.f, 0.f};
+        for (int32_t w = h; w < waves; w += heads) {
+          const float wt = __builtin_amdgcn_exp2f(m[w][rl] - base);
+          const bool held = l[w][rl] < 0.f;
+          total += wt * fabsf(l[w][rl]);
+          x += wt * (held == far ? 1.f : far ? kFarDown : kFarUp) * *reinterpret_cast<const f4*>(&o[w][rl][d]);
+        }
+        if (far) up = kFarUp;
       }
       const int32_t s = (r0 + rl) / group;
       const int64_t out_row = static_cast<int64_t>(s) * a.heads + (kv0 + h) * group + (r0 + rl - s * group);
@@ -213,12 +238,12 @@ struct WaveParts {
         const int64_t at = out_row * splits + split;
         if (d == 0) {
           partial.ml[2 * at] = big;
-          partial.ml[2 * at + 1] = total;
+          partial.ml[2 * at + 1] = up == 1.f ? total : -total;
         }
         *reinterpret_cast<f4*>(partial.o + at * PartialDims(a.dim) + d) = x;
       } else {
         float* dst = a.out + out_row * a.dim + d;
-        const f4 y = f4{__fdiv_rn(x[0], total), __fdiv_rn(x[1], total), __fdiv_rn(x[2], total), __fdiv_rn(x[3], total)};
+        const f4 y = f4{__fdiv_rn(x[0], total), __fdiv_rn(x[1], total), __fdiv_rn(x[2], total), __fdiv_rn(x[3], total)} * up;
         if (vec) {
           *reinterpret_cast<f4*>(dst) = y;
         } else {

@@ -418,6 +418,9 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   // acc[t][r] is O^T[dim 32t + 8 (r / 4) + 4g + r % 4][row j].
   l = l + XorLane<32>(l);
   if (w0 + j >= rows) return;
+  const bool far = power < kFarPower;
+  const int32_t down = far ? -power - kFarShift : -power;
+  const float up = far ? kFarUp : 1.f;
   const int64_t out_row = static_cast<int64_t>(s) * a.heads + head;
   float* dst = a.out + out_row * a.dim;
   bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
@@ -427,7 +430,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
     vec = true;
     if (g == 0) {
       b.partial.ml[2 * at] = m;
-      b.partial.ml[2 * at + 1] = l;
+      b.partial.ml[2 * at + 1] = far ? -l : l;
     }
   }
 #pragma unroll
@@ -438,8 +441,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       f4 o;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        o[e] = ldexpf(acc[t][4 * r4 + e], -power);
-        if (b.splits == 1) o[e] = __fdiv_rn(o[e], l);
+        o[e] = ldexpf(acc[t][4 * r4 + e], down);
+        if (b.splits == 1) o[e] = __fdiv_rn(o[e], l) * up;
       }
       if (vec) {
         if (d < a.dim) *reinterpret_cast<f4*>(dst + d) = o;

@@ -7,8 +7,8 @@
 
 namespace accel_hip {
 
-// Partial results of key ranges: of each (row, range) the reference m and the sum l, and the weighted
-// sum of PartialDims(dim) floats, 16-byte aligned.
+// Partial results of key ranges: of each (row, range) the reference m and the sum l, and the weighted sum o
+// of PartialDims(dim) floats, 16-byte aligned (attend_common.h says how l and o are held).
 constexpr int32_t PartialDims(int32_t dim) { return (dim + 3) & ~3; }
 struct AttendPartial {
   float* ml;  // [rows][splits][2]

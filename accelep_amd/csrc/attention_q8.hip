@@ -272,15 +272,16 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
   // acc[t][r] is O^T[dim DP / 16 (4g + r) + t][row j]; the waves' parts meet in LDS.
   l = l + XorLane<16>(l);
   l = l + XorLane<32>(l);
+  const bool far = power < kFarPower;
   if (g == 0) {
     parts.m[wave][j] = m;
-    parts.l[wave][j] = l;
+    parts.l[wave][j] = far ? -l : l;
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int t = 0; t < kTiles; t += 4) {
-      const int32_t down = -power;
+      const int32_t down = far ? -power - kFarShift : -power;
       *reinterpret_cast<f4*>(&parts.o[wave][j][kTiles * (4 * g + r) + t]) =
           f4{ldexpf(acc[t][r], down), ldexpf(acc[t + 1][r], down), ldexpf(acc[t + 2][r], down), ldexpf(acc[t + 3][r], down)};
     }
@@ -310,7 +311,7 @@ __global__ __launch_bounds__(kJoinThreads) void AttendJoinKernel(const float* ml
   const bool active = local < kJoinThreads / per_row && row < rows;
   ml += static_cast<int64_t>(row) * splits * 2;
   o += static_cast<int64_t>(row) * splits * dims + 4 * piece;
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, low = 0.f;
   f4 sum = f4{0.f, 0.f, 0.f, 0.f};
   if (active) {
     for (int c0 = of; c0 < splits; c0 += lanes * kJoinEach) {
@@ -334,13 +335,14 @@ __global__ __launch_bounds__(kJoinThreads) void AttendJoinKernel(const float* ml
       for (int i = 0; i < kJoinEach; ++i) {
         if (c0 + i * lanes >= splits) break;
         const float w = __builtin_amdgcn_exp2f(y[i].x - base);
+        low = fminf(low, y[i].y);
         l += w * y[i].y;
         sum += w * x[i];
       }
       m = big;
     }
     part_m[threadIdx.x] = m;
-    part_l[threadIdx.x] = l;
+    part_l[threadIdx.x] = low < 0.f ? -1.f : l;
     part_o[threadIdx.x] = sum;
   }
   __syncthreads();
@@ -350,14 +352,30 @@ __global__ __launch_bounds__(kJoinThreads) void AttendJoinKernel(const float* ml
   for (int i = 0; i < lanes; ++i) big = fmaxf(big, part_m[first + i * pieces]);
   const float base = big == -INFINITY ? 0.f : big;
   float total = 0.f;
+  low = 0.f;
   sum = f4{0.f, 0.f, 0.f, 0.f};
   for (int i = 0; i < lanes; ++i) {
     const float w = __builtin_amdgcn_exp2f(part_m[first + i * pieces] - base);
+    low = fminf(low, part_l[first + i * pieces]);
     total += w * part_l[first + i * pieces];
     sum += w * part_o[first + i * pieces];
   }
+  f4 far = f4{0.f, 0.f, 0.f, 0.f};
+  if (low < 0.f) {  // some parts are held times 2^-64: their sum is one of its own
+    total = 0.f;
+    sum = far;
+    for (int c = 0; c < splits; ++c) {
+      const float w = __builtin_amdgcn_exp2f(ml[2 * c] - base);
+      const f4 x = w * *reinterpret_cast<const f4*>(o + static_cast<int64_t>(c) * dims);
+      total += w * fabsf(ml[2 * c + 1]);
+      if (ml[2 * c + 1] < 0.f) far += x;
+      else sum += x;
+    }
+  }
   float* dst = out + static_cast<int64_t>(row) * dim + 4 * piece;
-  const f4 y = f4{__fdiv_rn(sum[0], total), __fdiv_rn(sum[1], total), __fdiv_rn(sum[2], total), __fdiv_rn(sum[3], total)};
+  f4 y = f4{__fdiv_rn(sum[0], total), __fdiv_rn(sum[1], total), __fdiv_rn(sum[2], total), __fdiv_rn(sum[3], total)};
+  if (low < 0.f)
+    y += f4{__fdiv_rn(far[0], total), __fdiv_rn(far[1], total), __fdiv_rn(far[2], total), __fdiv_rn(far[3], total)} * kFarUp;
   if (vec) {
     *reinterpret_cast<f4*>(dst) = y;
   } else {

@@ -79,3 +79,37 @@ def large_values(r, shape, signs):
     """Between a third and nearly all of the largest float."""
     x = r.uniform(1.2e38, 3.3e38, shape)
     return (x * r.choice([-1.0, 1.0], shape) if signs else x).astype(np.float32)
+
+
+@pytest.mark.parametrize("seq,length,copies", SIZES[2:], ids=SIZE_IDS[2:])
+@pytest.mark.parametrize("dim", [64, 100, 128, 256])
+@pytest.mark.parametrize("signs", [False, True])
+def test_window_attention_of_values_near_the_largest_float(seq, length, copies, dim, signs):
+    """The sum over the keys of weight times value passes the largest float, its quotient does not."""
+    r = np.random.default_rng(43)
+    position = length - seq
+    q, k = (r.standard_normal(s).astype(np.float32) for s in ((seq, 2, dim), (length, 2, dim)))
+    v = large_values(r, (length, 2, dim), signs)
+    some = np.unique(np.r_[0:seq:13, seq - 1])
+    want, bound = attend(q, k, v, position, 0, 0, some)
+    got = attention_window_call(many(q, copies, F32, position, 2), k, v, position)
+    assert_within(got[some, ::copies], want, bound)
+
+
+@pytest.mark.parametrize("seq,length,copies", SIZES[:1], ids=SIZE_IDS[:1])
+@pytest.mark.parametrize("block", [1, 4, 16, 64])
+@pytest.mark.parametrize("dim", [64, 100, 128, 256])
+def test_attention_q8_of_values_near_the_largest_float(seq, length, copies, block, dim):
+    r = np.random.default_rng(44)
+    position = length - seq
+    cache = Cache(length, 2, dim, block)
+    cache.fill(r, length)
+    cache.codes["v"][:] = r.integers(80, 128, cache.codes["v"].shape)
+    cache.codes["v"][:, :, ::5] *= -1
+    cache.scale["v"][:] = r.uniform(1.3e36, 2.6e36, cache.scale["v"].shape)
+    cache.upload()
+    q = r.standard_normal((seq, 2, dim)).astype(np.float32)
+    some = np.unique(np.r_[0:seq:13, seq - 1])
+    want, bound = attend(q, cache.values("k"), cache.values("v"), position, 0, 0, some, cache.value_scale(length))
+    got = attention_q8_call(many(q, copies, Q8, position, 2), cache, position)
+    assert_within(got[some, ::copies], want, bound)
