@@ -96,6 +96,11 @@ __device__ __forceinline__ int32_t WeightPower(float top, int32_t power) {
   return min(6 - e, kPowerMax);
 }
 
+// By how much a score may pass the reference before it moves, in log2 units: p then stays within 2^8. Where a
+// value scale is near the largest float (they reach 2^121) p times it has to stay in range.
+constexpr float kLargeScale = 0x1p112f;
+__device__ __forceinline__ float Slack(bool large_scale) { return large_scale ? 0.f : 8.f; }
+
 // Codes are read through buffer descriptors whose bounds are the range's last key row: rows past it read
 // as 0, with no address to clamp. Dims past a head's read whatever lies there, a code of the next head or
 // 0, which meets a query of 0, or as a value makes a dim that is not stored.

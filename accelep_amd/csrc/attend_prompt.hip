@@ -60,7 +60,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   __shared__ __align__(16) _Float16 vt[2][kParts][kKeys][kVStride];
   __shared__ __align__(16) float sk[2][kKeys];
   __shared__ __align__(16) float sv[2][kKeys];
-  __shared__ int odd[3];  // fp32: the tile has rows of scales of their own
+  __shared__ int odd[3];  // fp32: the tile has rows of scales of their own; codes: it has a large value scale
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -207,6 +207,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       if (!kUniform && tid < kKeys) {
         sk[buf][tid] = ks_next;
         sv[buf][tid] = vs_next;
+        if (vs_next >= kLargeScale) odd[slot] = 1;
       }
     }
   };
@@ -257,7 +258,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
     const int buf = (u - begin) & 1;
     const int32_t t0 = range.Key(u);
     __syncthreads();
-    if (kF32 && tid == 0) odd[(u + 2 - begin) % 3] = 0;  // next written behind the next barrier
+    if (!kUniform && tid == 0) odd[(u + 2 - begin) % 3] = 0;  // next written behind the next barrier
     if (u + 1 < end) fetch(range.Key(u + 1));
     __builtin_amdgcn_sched_barrier(0);
     const int32_t last = t0 + kKeys - 1;
@@ -314,9 +315,11 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[h][r]);
       mx = fmaxf(mx, XorLane<32>(mx)) * c;
-      // The reference moves only when a score passes it by 2^8, so the sums are seldom scaled.
+      // The reference moves only when a score passes it by 8, so the sums are seldom scaled. (fp32 rows'
+      // powers of two stay below 2^115, and a weight of 2^8 times that in range.)
+      const float slack = Slack(kF32 ? false : kUniform ? vs >= kLargeScale : odd[(u - begin) % 3] != 0);
       const float m_old = m;
-      if (mx > m + 8.f) m = mx;
+      if (mx > m + slack) m = mx;
       const float base = m == -INFINITY ? 0.f : m;
       const float corr = __builtin_amdgcn_exp2f(m_old - base);
       float sum = 0.f;

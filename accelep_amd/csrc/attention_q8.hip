@@ -170,13 +170,19 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
         factor[h][e] = finite ? row_back * ks[h][e] * a.factor : NAN;
         value[h][e] = finite ? vs[h][e] : 0.f;
       }
+    float largest = 0.f;
+#pragma unroll
+    for (int h = 0; h < kGroups; ++h)
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) largest = fmaxf(largest, value[h][e]);
+    const float slack = Slack(__any(largest >= kLargeScale));
     if (next >= 0) {
       load_k(next);
       load_scales(c.k.scale, next, ks);
     }
     __builtin_amdgcn_sched_barrier(0);
-    // Scores, and the row's largest. The reference m moves only when a score passes it by 2^8, so the
-    // sums are seldom scaled.
+    // Scores, and the row's largest. The reference m moves only when a score passes it by 8, so the sums
+    // are seldom scaled.
     const bool whole = range.Whole(a, t0);  // a row past the last may see what it likes
     float p[8];
     float mx = -INFINITY;
@@ -192,7 +198,7 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
     mx = fmaxf(mx, XorLane<16>(mx));
     mx = fmaxf(mx, XorLane<32>(mx));
     const float m_old = m;
-    if (mx > m + 8.f) m = mx;
+    if (mx > m + slack) m = mx;
     const float base = m == -INFINITY ? 0.f : m;
     const float corr = __builtin_amdgcn_exp2f(m_old - base);
     float sum = 0.f;

@@ -96,7 +96,7 @@ def test_window_attention_of_values_near_the_largest_float(seq, length, copies, 
     assert_within(got[some, ::copies], want, bound)
 
 
-@pytest.mark.parametrize("seq,length,copies", SIZES[:1], ids=SIZE_IDS[:1])
+@pytest.mark.parametrize("seq,length,copies", SIZES, ids=SIZE_IDS)
 @pytest.mark.parametrize("block", [1, 4, 16, 64])
 @pytest.mark.parametrize("dim", [64, 100, 128, 256])
 def test_attention_q8_of_values_near_the_largest_float(seq, length, copies, block, dim):
@@ -112,4 +112,30 @@ def test_attention_q8_of_values_near_the_largest_float(seq, length, copies, bloc
     some = np.unique(np.r_[0:seq:13, seq - 1])
     want, bound = attend(q, cache.values("k"), cache.values("v"), position, 0, 0, some, cache.value_scale(length))
     got = attention_q8_call(many(q, copies, Q8, position, 2), cache, position)
+    assert_within(got[some, ::copies], want, bound)
+
+
+@pytest.mark.parametrize("seq,length,copies", SIZES[1:], ids=SIZE_IDS[1:])
+@pytest.mark.parametrize("block", [1, 4, 16, 64])
+@pytest.mark.parametrize("rise", [2.0, 5.0])
+@pytest.mark.parametrize("first", [1.0, 2.0 ** -90])
+def test_attention_q8_of_large_values_behind_keys_of_lower_scores(seq, length, copies, block, rise, first):
+    """Scores rise by less than 8 in log2 units halfway, so the weights behind pass 1; the values there are near the
+    largest float, and before ordinary ones (or 2^-90 times those). Over many parts only one of them has the rise."""
+    r = np.random.default_rng(45)
+    position = length - seq
+    cache = Cache(length, 1, 64, block)
+    cache.fill(r, length)
+    middle = length // 2 // 64 * 64 - 64
+    cache.codes["k"][:, 0, 0] = 1
+    cache.codes["k"][middle:, 0, 0] = 127
+    cache.scale["k"][:] = 1 / 127
+    cache.scale["v"][:] = first * r.uniform(0.5, 1, cache.scale["v"].shape) / 64
+    cache.scale["v"][middle // block:] = r.uniform(1.3e36, 2.6e36, cache.scale["v"][middle // block:].shape)
+    cache.upload()
+    q = (r.standard_normal((seq, 2, 64)) / 64).astype(np.float32)
+    q[:, :, 0] = 8 * rise * 127 / 126
+    some = np.unique(np.r_[0:seq:13, seq - 1])
+    want, bound = attend(q, cache.values("k"), cache.values("v"), position, 0, 0, some, cache.value_scale(length))
+    got = attention_q8_call(many(q, copies, Q8, position, 1), cache, position)
     assert_within(got[some, ::copies], want, bound)
