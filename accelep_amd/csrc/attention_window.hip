@@ -11,6 +11,7 @@ namespace {
 constexpr int StepWaves(int dp) { return dp > 128 ? 4 : 8; }
 constexpr int kRows = 16;
 constexpr int kKeys = 16;  // of a wave's step
+constexpr uint32_t kLargeBits = (127 + 96) << 23;  // 2^96
 
 // One argument, not five: less of the host's work for a launch (a step over a window of 4096: 16.5 -> 16.1 us).
 struct StepArgs {
@@ -31,7 +32,9 @@ struct StepArgs {
 //    instruction s is key 4g + s, the A operand of dim tile (c, t) float t of the 16 bytes at
 //    V[key][64c + 4j].
 // A key or value row that is not finite would reach rows that do not see it, as 0 * NaN: a step that
-// holds one (a test of the bits, uniform) has its values taken as zeros and its weights as NaN.
+// holds one (a test of the bits, uniform) has its values taken as zeros and its weights as NaN. The same test
+// finds values from 2^96 on, whose sum over the keys may pass the largest float: a row that gives one of them a
+// weight holds its sum times 2^-64 until that weight is next to nothing beside later ones.
 template <int DP, int kLoad>
 __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
     StepArgs args) {
@@ -111,6 +114,7 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
   }
 
   float m = -INFINITY, l = 0.f;  // l: this lane's share of the row's sum
+  float shift = 1.f, share = 0.f;  // the weighted sum's power of two, and the largest weight now of a large value
   f4 acc[kC][4];
 #pragma unroll
   for (int c = 0; c < kC; ++c)
@@ -141,13 +145,14 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
 #pragma unroll
         for (int t = 0; t < 4; ++t) vtop[e] = max(vtop[e], FloatBits(vx[e][c][t]) & 0x7fffffffu);
     }
-    uint32_t bad = 0;  // of the lane's keys 4g + e
-    if (__any(max(max(vtop[0], vtop[1]), max(vtop[2], vtop[3])) >= 0x7f800000u) || bad_keys != 0) {
+    uint32_t bad = 0, large = 0;  // of the lane's keys 4g + e
+    if (__any(max(max(vtop[0], vtop[1]), max(vtop[2], vtop[3])) >= kLargeBits) || bad_keys != 0) {
       const uint32_t keys16 = static_cast<uint32_t>(bad_keys | bad_keys >> 16 | bad_keys >> 32 | bad_keys >> 48) & 0xffffu;
       bad = keys16 >> (4 * g) & 15u;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint64_t lanes = __ballot(vtop[e] >= 0x7f800000u);
+        if ((__ballot(vtop[e] >= kLargeBits) >> (16 * g) & 0xffffu) != 0) large |= 1u << e;
         if ((lanes >> (16 * g) & 0xffffu) != 0) {
           bad |= 1u << e;
 #pragma unroll
@@ -176,12 +181,31 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
     }
     l = l * corr + sum;
     m = m_new;
-    if (__any(corr != 1.f)) {
+    float again = corr;
+    share *= corr;
+    if (shift != 1.f && share < 0x1p-40f) {  // little is left of the large values
+      again *= kFarUp;
+      shift = 1.f;
+    }
+    if (__any(large != 0)) {
+      bool weighs = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) weighs = weighs || ((large >> e & 1) != 0 && p[e] > 0.f);
+      const uint64_t lanes = __ballot(weighs);
+      if (((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) >> j & 1) != 0) {
+        share = 1.f;
+        again *= shift == 1.f ? kFarDown : 1.f;
+        shift = kFarDown;
+      }
+    }
+    if (__any(again != 1.f)) {
 #pragma unroll
       for (int c = 0; c < kC; ++c)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) acc[c][t] *= corr;
+        for (int t = 0; t < 4; ++t) acc[c][t] *= again;
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p[e] *= shift;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -196,7 +220,7 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
   l = l + XorLane<32>(l);
   if (g == 0) {
     parts.m[wave][j] = m;
-    parts.l[wave][j] = l;
+    parts.l[wave][j] = shift == 1.f ? l : -l;
   }
 #pragma unroll
   for (int c = 0; c < kC; ++c)

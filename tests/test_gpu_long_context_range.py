@@ -81,7 +81,7 @@ def large_values(r, shape, signs):
     return (x * r.choice([-1.0, 1.0], shape) if signs else x).astype(np.float32)
 
 
-@pytest.mark.parametrize("seq,length,copies", SIZES[2:], ids=SIZE_IDS[2:])
+@pytest.mark.parametrize("seq,length,copies", SIZES, ids=SIZE_IDS)
 @pytest.mark.parametrize("dim", [64, 100, 128, 256])
 @pytest.mark.parametrize("signs", [False, True])
 def test_window_attention_of_values_near_the_largest_float(seq, length, copies, dim, signs):
@@ -139,3 +139,54 @@ def test_attention_q8_of_large_values_behind_keys_of_lower_scores(seq, length, c
     want, bound = attend(q, cache.values("k"), cache.values("v"), position, 0, 0, some, cache.value_scale(length))
     got = attention_q8_call(many(q, copies, Q8, position, 1), cache, position)
     assert_within(got[some, ::copies], want, bound)
+
+
+@pytest.mark.parametrize("seq,heads,length", [(1, 2, 70), (7, 4, 300), (16, 2, 5000)])
+@pytest.mark.parametrize("small", [1.0, 2.0 ** -100])
+def test_rows_of_one_tile_that_see_large_values_and_that_do_not(seq, heads, length, small):
+    """A window of 5: the key before the last rows' own holds values near the largest float; rows that do not see it
+    keep the bits of theirs, those that do have a finite quotient."""
+    r = np.random.default_rng(46)
+    position = length - seq
+    q, k, v = (r.standard_normal(s).astype(np.float32) for s in ((seq, heads, 64), (length, 2, 64), (length, 2, 64)))
+    v *= np.float32(small)
+    for t in sorted({length - 2, position + seq // 2, max(0, position - 3)}):
+        vv = v.copy()
+        vv[t] = large_values(r, (2, 64), True)
+        want, bound = attend(q, k, vv, position, 5, 1)
+        got = attention_window_call(q, k, vv, position, 5, 1)
+        assert_within(got, want, bound, floor=0)
+
+
+def test_small_values_beside_a_large_one_that_counts_for_nothing():
+    """A visible key whose values are near the largest float and whose weight is e^-100 of the others'."""
+    r = np.random.default_rng(47)
+    for seq, length in ((1, 60), (3, 4000)):
+        q, k, v = (r.standard_normal(s).astype(np.float32) for s in ((seq, 2, 64), (length, 1, 64), (length, 1, 64)))
+        q /= 8
+        q[:, :, 0] = 400
+        k[:, 0, 0] = 1
+        for t in (0, length // 2, length - seq):
+            kk, vv = k.copy(), v.copy()
+            kk[t, 0, 0] = -1
+            vv[t] = large_values(r, (1, 64), True)
+            want, bound = attend(q, kk, vv, length - seq, 0, 0)
+            assert_within(attention_window_call(q, kk, vv, length - seq), want, bound)
+
+
+@pytest.mark.parametrize("seq,heads,kv_heads,copies", [(1, 128, 128, 1), (2, 4, 1, 1), (40, 2, 1, 256)])
+@pytest.mark.parametrize("rise", [200.0, 4000.0])
+@pytest.mark.parametrize("small", [1.0, 2.0 ** -100])
+def test_small_values_behind_large_ones_whose_weights_vanish(seq, heads, kv_heads, copies, rise, small):
+    """The first keys' values are near the largest float; scores rise by `rise` over 4000 keys, so what they gave
+    the sum fades, slowly or at once, and only the last keys count."""
+    r = np.random.default_rng(48)
+    length = 4000
+    q, k, v = (r.standard_normal(s).astype(np.float32) for s in ((seq, heads, 64), (length, kv_heads, 64), (length, kv_heads, 64)))
+    v *= np.float32(small)
+    v[:200] = large_values(r, (200, kv_heads, 64), True)
+    q[:, :, 0] = 8
+    k[:, :, 0] = np.linspace(0, rise, length)[:, None]
+    want, bound = attend(q, k, v, length - seq, 0, 0)
+    got = attention_window_call(many(q, copies, F32, length - seq, kv_heads), k, v, length - seq)
+    assert_within(got[:, ::copies], want, bound, floor=0)
