@@ -5,34 +5,16 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from long_context_dispatch import F32, Q8, many, takes_many_rows
 from long_context_helpers import Cache, assert_within, attend, attention_q8_call, attention_window_call, check, lib
 
 pytestmark = pytest.mark.gpu
-
-Q8, F32 = 6 << 20, 3 << 20  # pairs of rows and keys from which the kernel of many rows is taken
 
 
 @pytest.fixture(scope="module", autouse=True)
 def device():
     check(lib().accel_hip_init())
     yield
-
-
-def takes_many_rows(pairs, seq, position, heads, kv_heads, window=0, sinks=0):
-    """The library's choice of kernel, from the sizes."""
-    group, end = heads // kv_heads, position + seq
-    rows = seq * group
-    keys = end if window == 0 or window >= end else min(end, window + min(seq, (14 + group) // group + 1) + 32)
-    steps = -(-keys // 32) + (0 if window == 0 or window >= end else -(-min(sinks, end) // 32))
-    each = steps * 32 * kv_heads
-    return rows > 16 and -(-rows // 16) * 16 >= -(-pairs // each)
-
-
-def many(q, copies, pairs, position, kv_heads, window=0, sinks=0):
-    """`copies` of each query head: one for the kernel of few rows, more for the one of many."""
-    out = np.repeat(q, copies, axis=1)
-    assert takes_many_rows(pairs, q.shape[0], position, out.shape[1], kv_heads, window, sinks) == (copies > 1)
-    return out
 
 
 # (seq, length, copies): few rows over a range in one part and in several; many rows, the same.
