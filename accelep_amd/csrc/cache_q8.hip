@@ -3,8 +3,8 @@
 //
 // Append: each touched (block, head, plane) is one unit of one wave, or of one workgroup where it is
 // large. A unit holds its new rows in registers, takes their largest magnitude, forms the scale
-// (amax / 127, or the stored one where older rows of the block need more), and writes the codes: one
-// pass over the rows. Older rows of the block are only touched when the scale grows.
+// (amax / 127, or the stored one where that is larger and the block has older rows), and writes the codes:
+// one pass over the rows. Older rows of the block are only touched when the scale grows.
 //
 // Bound: the bytes, 5 a value each way. 4095 rows of 8 heads of 128: append 10.9 us, 42 MB at 3.9 TB/s
 // (the loads of a unit, then its largest, then its stores: a unit's phases follow one another, and a

@@ -276,9 +276,10 @@ typedef struct AccelHipCacheQ8 {
   int64_t capacity, kv_heads, head_dim, block;
 } AccelHipCacheQ8;
 /* AppendCache into the 8-bit cache: rows [position, position + seq) of k and v (fp32, kv_heads *
- * head_dim a row). Each touched block and head gets the scale max|x| / 127 of its new rows, or keeps
- * the scale it has where rows of the block before `position` need more; when it grows, those rows'
- * codes become the nearest code of code * old / new. A code is the nearest integer to x / scale (the
+ * head_dim a row). Each touched block and head gets the scale max|x| / 127 of its new rows. A block that has
+ * rows before `position` keeps the scale it has where that is larger, also where only rows from position on,
+ * written over now (a rejected draft), needed it; when it grows, the rows' codes before become the nearest
+ * code of code * old / new. A block written from its start is new. A code is the nearest integer to x / scale (the
  * true quotient; ties to even), within -127 .. 127, where only a scale below 2^-126 leaves it. Rows of
  * the block from position + seq on do not count any more. A NaN or an infinity makes its block's scale of
  * that head NaN, and all that is read of it, until the block is written from its start. The planes may
