@@ -49,9 +49,9 @@ __device__ __forceinline__ bool Sees(const AttendArgs& a, int32_t p, int32_t t) 
 __device__ __forceinline__ h2 PackRtz(float x, float y) {
   return __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
 }
-// x = hi + lo to 22 bits (each part 11, the first rounded towards zero): for |x| between 2^-3 and 2^15
-// the rest is below 2^-22 |x|, under that below 2^-25. Both products with exact f16 operands are exact
-// in the matrix core's fp32 sums.
+// x = hi + lo to 22 bits, each part 11 cut towards zero: for |x| between 2^-3 and 2^15 what is left, the last
+// two of x's 24 bits at most, is within 1.5 * 2^-22 |x|, under that below 2^-24 (the spacing of f16's
+// subnormal numbers). Both products with exact f16 operands are exact in the matrix core's fp32 sums.
 __device__ __forceinline__ void SplitF16(float x, float y, h2& hi, h2& lo) {
   hi = PackRtz(x, y);
   float rx, ry;  // x - hi[0], y - hi[1]: one instruction each, which the compiler makes two of
@@ -85,7 +85,7 @@ __device__ __forceinline__ h8 Join(h2 a, h2 b, h2 c, h2 d) { return h8{a[0], a[1
 // A row's softmax while its keys pass holds m, a reference for its scores in log2 units, l, the sum of
 // p = 2^(s - m), and `top`, the largest p * value scale so far. The weighted sum holds p * value scale *
 // 2^power, with top * 2^power kept in [2^3, 2^15): a weight then has 22 bits down to 2^-6 of the largest
-// and is off by 2^-28 of that below, whatever the scales, and a key that a row does not see has no say.
+// and is off by 2^-27 of that below, whatever the scales, and a key that a row does not see has no say.
 constexpr int32_t kPowerMax = 127;
 // From this power on the sum of up to 2^31 keys is less than 2^100 when the power is taken out.
 constexpr int32_t kFarPower = -40;
@@ -148,6 +148,10 @@ inline int64_t AttendRangeSteps(const AttendArgs& a, int64_t rows, int64_t step)
   const int64_t keys = std::min<int64_t>(end, int64_t(a.window) + queries + step);
   return (keys + step - 1) / step + (std::min<int64_t>(a.sinks, end) + step - 1) / step;
 }
+
+// Waves of a step workgroup at most: two a SIMD, one of head dim 256, whose sums and operands take more than
+// half of a SIMD's registers.
+constexpr int StepWaves(int dp) { return dp > 128 ? 4 : 8; }
 
 // Whether the rows are many enough for the tiles of keys to go through LDS: more than 16 of a key head,
 // and `pairs` of rows (in 16s) and keys. Below, the step kernels' spread over the CUs wins. 16 heads, 4 key

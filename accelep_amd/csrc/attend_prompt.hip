@@ -17,9 +17,11 @@
 //
 // Bound: the matrix cores at the clock that they leave themselves (1.7-1.9 GHz under this load), with the
 // softmax and the split of its weights between their phases. 2048 rows from position 4097 on, 32 heads on
-// 8 of 128: 309 us, 172 GFLOP in two products, 1.11 PFLOP/s of f16; the matrix cores are busy 65 % of the
-// cycles. fp32, 4096 rows in a window of 1024: 231 us, 60 GFLOP in three products, 0.78 PFLOP/s; busy
-// 41 %, since each tile of keys is also split there.
+// 8 of 128: 311 us, 172 GFLOP in two products, 1.11 PFLOP/s of f16; the matrix cores are busy 65 % of the
+// cycles. fp32, 4096 rows in a window of 1024: 236 us, 60 GFLOP in three products, 0.77 PFLOP/s; busy
+// 41 %, since each tile of keys is also split there, by every workgroup that reads it.
+// Dims are padded to 64, 128 or 256: the 8-bit case takes 301 us with heads of 80, 305 of 96, 708 of 192 and
+// 707 of 256 (197 of 64), where the registers of a wave no longer hold queries, sums and staging.
 // Pieces of 8 codes, whose LDS writes have no bank conflicts (those of 16 have, 8 % of the cycles), took
 // 311 us; fp32 in workgroups of eight waves 225, which a variant of its own was not worth.
 #include "attend_common.h"
@@ -93,7 +95,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   const auto fetch_plane = [&](const void* base, int32_t t0, uint4 (&x)[kChunks]) {
     if constexpr (kF32) {
       // A row past the range reads its last one, a piece past a head's dims its last: both are not used.
-      const float* p = static_cast<const float*>(base) + min(t0 + tid / 8, range.high - 1) * kv_row + static_cast<int64_t>(kv) * a.dim;
+      const float* p = static_cast<const float*>(base) + min(t0 + tid / 8, range.high - 1) * kv_row +
+                       static_cast<int64_t>(kv) * a.dim;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int d = 8 * (tid % 8 + 8 * (i / 2)) + 4 * (i % 2);
@@ -177,7 +180,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       for (int i = 0; i < kChunks; ++i) {
         const int key = (tid + i * kThreads) / (DP / 16);
         const int d = 16 * ((tid + i * kThreads) % (DP / 16));
-        const uint32_t x0 = x[i].x ^ 0x80808080u, x1 = x[i].y ^ 0x80808080u, x2 = x[i].z ^ 0x80808080u, x3 = x[i].w ^ 0x80808080u;
+        const uint32_t x0 = x[i].x ^ 0x80808080u, x1 = x[i].y ^ 0x80808080u;
+        const uint32_t x2 = x[i].z ^ 0x80808080u, x3 = x[i].w ^ 0x80808080u;
         h8* p = reinterpret_cast<h8*>(dst + key * stride + d);
         p[0] = Join(CodesLow(x0), CodesHigh(x0), CodesLow(x1), CodesHigh(x1));
         p[1] = Join(CodesLow(x2), CodesHigh(x2), CodesLow(x3), CodesHigh(x3));
@@ -483,7 +487,7 @@ void LaunchPromptOf(const AttendArgs& a, PromptArgs b, int load, hipStream_t str
   const int64_t tiles = (int64_t(a.seq) * group + kRows - 1) / kRows;
   const int64_t units = tiles * a.kv_heads;
   if (units > 0x7fffffff) Fail(ACCEL_HIP_INVALID_ARGUMENT, "Attention is too large");
-  const AttendSplit split = SplitRange(a, units, 1, AttendRangeSteps(a, kRows, kF32 ? 32 : 64) / 4);
+  const AttendSplit split = SplitRange(a, units, AttendRangeSteps(a, kRows, kF32 ? 32 : 64) / 4);
   b.splits = split.count;
   b.tiles = static_cast<int32_t>(tiles);
   b.partial = split.partial;

@@ -4,9 +4,9 @@
 
 namespace accel_hip {
 
-AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t per_cu, int64_t most) {
+AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t most) {
   const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
-  const int64_t count = std::max<int64_t>(1, std::min<int64_t>(per_cu * cus / units, most));
+  const int64_t count = std::max<int64_t>(1, std::min<int64_t>(cus / units, most));
   const int64_t parts = int64_t(a.seq) * a.heads * count;
   const size_t ml_bytes = (static_cast<size_t>(parts) * 2 * sizeof(float) + 15) & ~size_t(15);
   const size_t bytes = ml_bytes + static_cast<size_t>(parts * PartialDims(a.dim)) * sizeof(float);

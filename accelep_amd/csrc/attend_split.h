@@ -15,8 +15,8 @@ struct AttendPartial {
   float* o;   // [rows][splits][PartialDims]
 };
 
-// Into how many key ranges the rows of `units` workgroups are cut: up to per_cu workgroups per CU, at
-// most `most` ranges. Where the partial sums have no room (no memory is left, or a capture runs and the
+// Into how many key ranges the rows of `units` workgroups are cut: up to one workgroup per CU, at most
+// `most` ranges. Where the partial sums have no room (no memory is left, or a capture runs and the
 // buffer is too small) the range stays whole. Their buffer serves these calls alone, and is held until both
 // launches are queued: calls from several threads, and replays of graphs, take turns.
 struct AttendSplit {
@@ -24,6 +24,6 @@ struct AttendSplit {
   AttendPartial partial{nullptr, nullptr};
   std::unique_lock<std::mutex> held;
 };
-AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t per_cu, int64_t most);
+AttendSplit SplitRange(const AttendArgs& a, int64_t units, int64_t most);
 
 }  // namespace accel_hip

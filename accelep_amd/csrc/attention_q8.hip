@@ -9,18 +9,17 @@
 namespace accel_hip {
 namespace {
 
-// Waves of a step workgroup at most: what a CU's registers hold.
-constexpr int StepWaves(int dp) { return dp > 128 ? 4 : 8; }
 constexpr int kStepRows = 16;
 constexpr int kStepKeys = 32;
 
 // One workgroup per (16 rows of up to 4 key heads, key range): wave w serves head w % hw of them, and the
 // waves of a head take its steps of 32 keys in turn, so that a workgroup reads a key row's heads together
 // (131072 keys of 8 heads of 128, loads alone: a workgroup a head read them at 4.7 TB/s, 4 heads at 5.7).
-// Bound: the cache's bytes over a long range (131072 keys, 32 heads on 8 key heads of 128: 51.5 us, 5.2
-// TB/s, and 3.3 of the join); over a short one the chain of load, products, softmax and products of a
-// wave's few steps (2048 keys, 9 heads on 3 of 64: 5.2 us and 3.4 of the join). Keys and values go from memory to registers, and there to f16: no LDS and
-// no barrier in the loop. Lane (j, g) = (lane % 16, lane / 16). Per step
+// Bound: the cache's bytes over a long range (131072 keys, 32 heads on 8 key heads of 128: 52.3 us, 5.1
+// TB/s, and 5.5 of the join); over a short one the chain of load, products, softmax and products of a
+// wave's few steps (2048 keys, 9 heads on 3 of 64: 5.5 us and 3.6 of the join). Medians, as in all these
+// comments. Keys and values go from memory to registers, and there to f16: no LDS and no barrier in the
+// loop. Lane (j, g) = (lane % 16, lane / 16). Per step
 //  * S^T = K Q^T on v_mfma_f32_16x16x32_f16: the A operand of instruction (c, half) are the codes
 //    64c + 16g + 8 half .. + 7 of key row j, so a lane loads 16 bytes of a key at a time;
 //  * O^T += V^T P^T: S^T leaves lane (j, g) the scores of keys 4g .. 4g + 3 and 16 + 4g .. of row j,
@@ -296,7 +295,7 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
 }
 
 // A workgroup's threads are (row, key range, 16-byte piece), `lanes` ranges of a row at a time, up to 8
-// of a thread in flight at once: a round trip to what other workgroups left is all this costs (3.3-5 us; the
+// of a thread in flight at once: a round trip to what other workgroups left is all this costs (3.6-5.6 us; the
 // last workgroup of a row to arrive joining them in the step kernel instead took 1-5 us more than this
 // launch, for its stores and loads past the XCDs' caches).
 constexpr int kJoinThreads = 512;
@@ -398,8 +397,9 @@ void LaunchAttendJoin(const AttendArgs& a, const AttendPartial& partial, int32_t
   const int32_t pieces = PartialDims(a.dim) / 4;
   const int32_t lanes = std::min(splits, kJoinThreads / pieces);
   const int32_t per_group = kJoinThreads / (pieces * lanes);
-  hipLaunchKernelGGL(AttendJoinKernel, dim3(GridOf((int64_t(rows) + per_group - 1) / per_group, kJoinThreads, "Attention is too large")), dim3(kJoinThreads), 0,
-                     stream, partial.ml, partial.o, a.out, rows, splits, a.dim, lanes, vec);
+  const dim3 grid(GridOf((int64_t(rows) + per_group - 1) / per_group, kJoinThreads, "Attention is too large"));
+  hipLaunchKernelGGL(AttendJoinKernel, grid, dim3(kJoinThreads), 0, stream, partial.ml, partial.o, a.out, rows, splits,
+                     a.dim, lanes, vec);
   Check(hipGetLastError(), "AttendJoinKernel launch");
 }
 
@@ -420,9 +420,9 @@ void LaunchStep(const AttendArgs& a, const Q8Cache& c, hipStream_t stream) {
   // Steps that do not fill the CUs are spread one wave a SIMD (2048 keys, 9 heads of 64: 7.6 us in
   // workgroups of four waves, 9.0 of eight, 14.2 in one of sixteen a key head).
   const int32_t sw = hw == 1 && units * steps < cus * kWaves ? 4 : kWaves / hw;
-  const AttendSplit split = SplitRange(a, units, 1, steps <= 2 * sw ? 1 : steps / sw);
-  hipLaunchKernelGGL((AttendQ8StepKernel<DP, kLoad, kScales>), dim3(GridOf(units * split.count, 64 * hw * sw, "Attention is too large")),
-                     dim3(64 * hw * sw), 0, stream, a, c, hw, split.count, split.partial);
+  const AttendSplit split = SplitRange(a, units, steps <= 2 * sw ? 1 : steps / sw);
+  const dim3 grid(GridOf(units * split.count, 64 * hw * sw, "Attention is too large")), block(64 * hw * sw);
+  hipLaunchKernelGGL((AttendQ8StepKernel<DP, kLoad, kScales>), grid, block, 0, stream, a, c, hw, split.count, split.partial);
   Check(hipGetLastError(), "AttendQ8StepKernel launch");
   if (split.count > 1) LaunchAttendJoin(a, split.partial, split.count, stream);
 }
@@ -440,7 +440,8 @@ void LaunchStepOf(const AttendArgs& a, const Q8Cache& c, int load, hipStream_t s
 
 void LaunchAttentionQ8(const AttendArgs& a, const Q8Cache& c, hipStream_t stream) {
   const auto aligned = [&](size_t to) {
-    return a.dim % to == 0 && reinterpret_cast<uintptr_t>(c.k.code) % to == 0 && reinterpret_cast<uintptr_t>(c.v.code) % to == 0;
+    return a.dim % to == 0 && reinterpret_cast<uintptr_t>(c.k.code) % to == 0 &&
+           reinterpret_cast<uintptr_t>(c.v.code) % to == 0;
   };
   const int load = aligned(16) ? 16 : aligned(4) ? 4 : 1;
   if (AttendManyRows(a, kPromptPairsQ8)) LaunchAttendPromptQ8(a, c, load, stream);

@@ -7,8 +7,6 @@
 namespace accel_hip {
 namespace {
 
-// Waves of a workgroup: what a CU's registers hold.
-constexpr int StepWaves(int dp) { return dp > 128 ? 4 : 8; }
 constexpr int kRows = 16;
 constexpr int kKeys = 16;  // of a wave's step
 constexpr uint32_t kLargeBits = (127 + 96) << 23;  // 2^96
@@ -24,8 +22,9 @@ struct StepArgs {
 
 // One workgroup per (16 rows of a key head, key range); its waves take its steps of 16 keys in turn.
 // Bound: the bytes of the keys that are seen, and over a window the chain of a wave's one or two steps (4100
-// keys, 32 heads on 8 key heads of 128: 33.6 MB in 12.9 us, 2.6 TB/s). Both products run on v_mfma_f32_16x16x4f32, which takes
-// fp32 as it is, with every operand straight from memory. Lane (j, g) = (lane % 16, lane / 16):
+// keys, 32 heads on 8 key heads of 128: 33.6 MB in 13.2 us, 2.5 TB/s). Both products run on
+// v_mfma_f32_16x16x4f32, which takes fp32 as it is, with every operand straight from memory. Lane (j, g) =
+// (lane % 16, lane / 16):
 //  * S^T = K Q^T: k slot g of instruction (i, e) is dim 16i + 4g + e, so a lane loads 16 bytes of key
 //    row j at a time and a key row's pieces lie side by side;
 //  * O^T += V^T P^T: S^T leaves the lane the scores of keys 4g .. 4g + 3 of row j; k slot g of
@@ -242,7 +241,7 @@ void LaunchStep(const AttendArgs& a, const float* k, const float* v, bool vec, h
   // Steps that do not fill the CUs are spread one wave a SIMD.
   const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
   const int32_t waves = units * steps < cus * kWaves ? 4 : kWaves;
-  const AttendSplit split = SplitRange(a, units, 1, steps <= 2 * waves ? 1 : steps / waves);
+  const AttendSplit split = SplitRange(a, units, steps <= 2 * waves ? 1 : steps / waves);
   const dim3 grid(GridOf(units * split.count, 64 * waves, "Attention is too large")), block(64 * waves);
   const StepArgs args{a, k, v, split.count, split.partial};
   if (vec) hipLaunchKernelGGL((AttendF32StepKernel<DP, 16>), grid, block, 0, stream, args);

@@ -6,10 +6,10 @@
 // (amax / 127, or the stored one where that is larger and the block has older rows), and writes the codes:
 // one pass over the rows. Older rows of the block are only touched when the scale grows.
 //
-// Bound: the bytes, 5 a value each way. 4095 rows of 8 heads of 128: append 10.9 us, 42 MB at 3.9 TB/s
+// Bound: the bytes, 5 a value each way. 4095 rows of 8 heads of 128: append 11.3 us, 42 MB at 3.7 TB/s
 // (the loads of a unit, then its largest, then its stores: a unit's phases follow one another, and a
-// reduction stands between); 32768 rows read back 52-58 us, 336 MB at 5.8-6.5 TB/s. One row: 3.3 and
-// 2.2 us, launch and two dependent round trips.
+// reduction stands between); 32768 rows read back 58 us, 336 MB at 5.8 TB/s. One row: 3.4 and 2.3 us,
+// launch and two dependent round trips.
 #include <algorithm>
 
 #include "device_common.h"
@@ -94,7 +94,8 @@ __global__ __launch_bounds__(kThreads) void AppendQ8Kernel(AppendArgs a) {
   const int32_t head = static_cast<int32_t>(bh) - block * a.kv_heads;
   const int32_t begin = ((a.position >> a.block_shift) + block) << a.block_shift;  // the block's first row
   const int32_t lo = max(a.position, begin);
-  const int32_t hi = static_cast<int32_t>(min(static_cast<int64_t>(a.position) + a.seq, static_cast<int64_t>(begin) + (1 << a.block_shift)));
+  const int64_t block_end = static_cast<int64_t>(begin) + (1 << a.block_shift);
+  const int32_t hi = static_cast<int32_t>(min(static_cast<int64_t>(a.position) + a.seq, block_end));
   const int32_t per_row = a.dim / kDims;
   const int32_t items = (hi - lo) * per_row;
   const float* src = a.src[pl] + static_cast<int64_t>(lo - a.position) * a.row_stride + static_cast<int64_t>(head) * a.dim;
@@ -116,7 +117,8 @@ __global__ __launch_bounds__(kThreads) void AppendQ8Kernel(AppendArgs a) {
   uint32_t top = 0;
   if (held) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) x[i] = lane + i * kLanes < items ? load(lane + i * kLanes) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < kHeld; ++i)
+      x[i] = lane + i * kLanes < items ? load(lane + i * kLanes) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
   float old = 0.f;
   if (lo > begin && (kWaves == 1 || lane == 0)) old = *scale;

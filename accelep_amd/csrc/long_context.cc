@@ -41,7 +41,8 @@ bool Overlap(const AccelHipBuffer& a, size_t a_bytes, const AccelHipBuffer& b, s
 }
 
 // b against `rows` rows of `width` bytes, `stride` bytes apart: what lies between the rows is not theirs.
-bool OverlapsStrided(const AccelHipBuffer& b, size_t bytes, const AccelHipBuffer& to, int64_t rows, size_t stride, size_t width) {
+bool OverlapsStrided(const AccelHipBuffer& b, size_t bytes, const AccelHipBuffer& to, int64_t rows, size_t stride,
+                     size_t width) {
   if (rows == 0 || !Overlap(b, bytes, to, static_cast<size_t>(rows - 1) * stride + width)) return false;
   if (b.data <= to.data) return true;
   const size_t in_row = static_cast<size_t>(static_cast<const char*>(b.data) - static_cast<const char*>(to.data)) % stride;
@@ -221,8 +222,10 @@ ACCEL_HIP_API int accel_hip_rope_scaled(AccelHipBuffer states, AccelHipBuffer ou
       RequireAligned(positions, sizeof(int32_t), "Rope positions are not aligned");
     }
     // Other workgroups may still read them.
-    const size_t stride_bytes = static_cast<size_t>(stride) * sizeof(float), row_bytes = static_cast<size_t>(row) * sizeof(float);
-    if (OverlapsStrided(frequencies, static_cast<size_t>(rotary_dim / 2) * sizeof(double), out, seq, stride_bytes, row_bytes))
+    const size_t stride_bytes = static_cast<size_t>(stride) * sizeof(float);
+    const size_t row_bytes = static_cast<size_t>(row) * sizeof(float);
+    const size_t frequency_bytes = static_cast<size_t>(rotary_dim / 2) * sizeof(double);
+    if (OverlapsStrided(frequencies, frequency_bytes, out, seq, stride_bytes, row_bytes))
       Invalid("Rope output overlaps the frequencies");
     if (rotary_dim > 0 && OverlapsStrided(positions, CheckedIntBytes(seq), out, seq, stride_bytes, row_bytes))
       Invalid("Rope output overlaps the positions");
@@ -341,7 +344,8 @@ ACCEL_HIP_API int accel_hip_attention_window(AccelHipBuffer q, AccelHipBuffer k,
     RequireAligned(v, sizeof(float), "Attention value is not aligned");
     if (!any) return;
     const size_t out_bytes = CheckedBytes(seq, heads * head_dim);
-    if (Overlap(out, out_bytes, k, bytes) || Overlap(out, out_bytes, v, bytes)) Invalid("Attention output overlaps the cache");
+    if (Overlap(out, out_bytes, k, bytes) || Overlap(out, out_bytes, v, bytes))
+      Invalid("Attention output overlaps the cache");
     NoteDeviceWrite(out.data, sizeof(float));
     LaunchAttentionWindow(a, static_cast<const float*>(k.data), static_cast<const float*>(v.data), Ctx().stream);
   });

@@ -2,14 +2,15 @@
 // for pair i of a head at position p, a = p * f_i, m the magnitude; pairs are dims (i, i + r/2) or
 // (2i, 2i + 1), dims from r on come out unchanged.
 //
-// The angle is formed in fp64, in half turns reduced to [-1, 1], so a position of any size costs
-// no accuracy: what the reduced angle's rounding to fp32 leaves over goes back in to first order
-// (sin(a + d) = sin a + d cos a). One workgroup per row (and part of its heads): its pairs' cos and
-// sin are computed once into LDS, then the heads stream through (their first loads are on the way
-// while the angles are formed).
+// The angle is formed in fp64, in half turns reduced to [-1, 1]. The product of position and frequency and the
+// change to half turns each round by 2^-53 of it: within 2^-24 radians together up to 2^27 radians, within 2^-20
+// at 2^31. What the reduced angle's rounding to fp32 leaves over goes back in to first order
+// (sin(a + d) = sin a + d cos a); cos and sin themselves are fp32. One workgroup per row (and part of its
+// heads): its pairs' cos and sin are computed once into LDS, then the heads stream through (their first loads
+// are on the way while the angles are formed).
 //
 // Bound: the bytes of the values, 8 each in a pass (4096 rows of 40 heads of 128, half of each turned:
-// 168 MB in 33-35 us, 4.8-5.1 TB/s, as a copy); a single row is a launch and one dependent load (2.1 us).
+// 168 MB in 35 us, 4.8 TB/s, nearly a copy's rate); a single row is a launch and one dependent load (2.2 us).
 #include <algorithm>
 
 #include "device_common.h"

@@ -262,8 +262,9 @@ ACCEL_HIP_API int accel_hip_rope_frequencies(const AccelHipRopeScaling* scaling,
  * multiplies them with magnitude; the other dims come out as they are. states and out are rows of
  * n_heads * head_dim floats (and row_stride apart both; what lies behind a row's heads is left alone):
  * the query and key heads of a fused projection's rows turn in one call. out may be states itself, and
- * may not overlap it otherwise, nor the frequencies and positions. position_s is position + s, or position + positions[s] where positions
- * (int32 [seq]) has data. Angles are formed in 64 bits: position_s counts up to 2^32. */
+ * may not overlap it otherwise, nor the frequencies and positions. position_s is position + s, or position +
+ * positions[s] where positions (int32 [seq]) has data; it counts up to 2^32. Angles are formed in 64 bits
+ * (within 2^-24 radians up to 2^27 of them, within 2^-20 at 2^31), their cos and sin in fp32. */
 ACCEL_HIP_API int accel_hip_rope_scaled(AccelHipBuffer states, AccelHipBuffer out, AccelHipBuffer frequencies,
                                         AccelHipBuffer positions, int64_t seq, int64_t n_heads, int64_t head_dim,
                                         int64_t row_stride, int64_t rotary_dim, int32_t layout, int64_t position,
@@ -276,14 +277,14 @@ typedef struct AccelHipCacheQ8 {
   int64_t capacity, kv_heads, head_dim, block;
 } AccelHipCacheQ8;
 /* AppendCache into the 8-bit cache: rows [position, position + seq) of k and v (fp32, kv_heads *
- * head_dim a row). Each touched block and head gets the scale max|x| / 127 of its new rows. A block that has
- * rows before `position` keeps the scale it has where that is larger, also where only rows from position on,
- * written over now (a rejected draft), needed it; when it grows, the rows' codes before become the nearest
- * code of code * old / new. A block written from its start is new. A code is the nearest integer to x / scale (the
- * true quotient; ties to even), within -127 .. 127, where only a scale below 2^-126 leaves it. Rows of
- * the block from position + seq on do not count any more. A NaN or an infinity makes its block's scale of
- * that head NaN, and all that is read of it, until the block is written from its start. The planes may
- * not overlap one another or k and v. */
+ * head_dim a row). Each touched block and head gets the scale max|x| / 127 of its new rows. A block that
+ * has rows before `position` keeps the scale it has where that is larger, also where only rows that are
+ * written over now (a rejected draft) needed it; when it grows, the codes of the rows before become the
+ * nearest code of code * old / new. A block written from its start is new. A code is the nearest integer to
+ * x / scale (the true quotient; ties to even), within -127 .. 127, where only a scale below 2^-126 leaves
+ * it. Rows of the block from position + seq on do not count any more. A NaN or an infinity makes its block's
+ * scale of that head NaN, and all that is read of it, until the block is written from its start. The planes
+ * may not overlap one another or k and v. */
 ACCEL_HIP_API int accel_hip_append_cache_q8(AccelHipBuffer k, AccelHipBuffer v, const AccelHipCacheQ8* cache,
                                             int64_t seq, int64_t position, int64_t row_stride);
 /* Rows [first, first + count) of the 8-bit cache as fp32 [count, kv_heads, head_dim], code * scale
@@ -305,8 +306,8 @@ ACCEL_HIP_API int accel_hip_attention_q8(AccelHipBuffer q, const AccelHipCacheQ8
 /* Attention over an fp32 cache k, v [>= position + seq, kv_heads, head_dim] with a sliding window: the
  * row at p sees the keys t <= p with t > p - window or t < sinks (window 0: every t <= p). Keys that no
  * row sees count for nothing, NaN included. q's rows are row_stride apart, out is dense and may not
- * overlap q, k or v. Sizes, captures and queries as above. Rounding: with many rows (16 and more of a key
- * head, over a long range) queries, keys and values enter the products with 22 bits of their row's
+ * overlap q, k or v. Sizes, captures and queries as above. Rounding: with many rows (more than 16 of a
+ * key head, over a long range) queries, keys and values enter the products with 22 bits of their row's
  * largest value and weights with 22 bits of the largest; otherwise in fp32. A key or value that is not
  * finite makes the rows that see it NaN. */
 ACCEL_HIP_API int accel_hip_attention_window(AccelHipBuffer q, AccelHipBuffer k, AccelHipBuffer v, AccelHipBuffer out,

@@ -145,7 +145,7 @@ HOST_API int scratch_host_hold_parts() {
     AttendArgs a{};
     a.seq = a.heads = a.kv_heads = 1;
     a.dim = 64;
-    g_held = SplitRange(a, 1, 1, 8);
+    g_held = SplitRange(a, 1, 8);
     if (g_held.count != 8) Fail(ACCEL_HIP_LOGIC_ERROR, "the range is whole");
   });
 }
@@ -158,7 +158,7 @@ HOST_API int scratch_host_split(int heads, int dim, int64_t most, int* count) {
     a.heads = heads;
     a.kv_heads = 1;
     a.dim = dim;
-    const AttendSplit split = SplitRange(a, 1, 1, most);
+    const AttendSplit split = SplitRange(a, 1, most);
     *count = split.count;
     const size_t bytes = static_cast<size_t>(split.count) * heads * (2 + PartialDims(dim)) * sizeof(float);
     if (split.count > 1 && scratch_host_block(split.partial.ml) < bytes) Fail(ACCEL_HIP_LOGIC_ERROR, "the parts have no room");
