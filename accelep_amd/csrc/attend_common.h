@@ -101,6 +101,11 @@ __device__ __forceinline__ int32_t WeightPower(float top, int32_t power) {
 constexpr float kLargeScale = 0x1p112f;
 __device__ __forceinline__ float Slack(bool large_scale) { return large_scale ? 0.f : 8.f; }
 
+// The exponent s - m is one fma of the unrounded product s, and the reference m a rounded one: their distance,
+// up to 2^-24 |m|, counts for nothing until it is as large as the exponents that matter. From here on s is
+// rounded as m was, so that the largest key's exponent is 0.
+constexpr float kFarScore = 0x1p20f;
+
 // Codes are read through buffer descriptors whose bounds are the range's last key row: rows past it read
 // as 0, with no address to clamp. Dims past a head's read whatever lies there, a code of the next head or
 // 0, which meets a query of 0, or as a value makes a dim that is not stored.

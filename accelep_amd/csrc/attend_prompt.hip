@@ -326,12 +326,20 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       if (mx > m + slack) m = mx;
       const float base = m == -INFINITY ? 0.f : m;
       const float corr = __builtin_amdgcn_exp2f(m_old - base);
-      float sum = 0.f;
+      float sum = 0.f, below = base;
+      if (__any(fabsf(base) >= kFarScore)) {
+#pragma unroll
+        for (int h = 0; h < kSub; ++h)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) st[h][r] = st[h][r] * c - base;
+        c = 1.f;
+        below = 0.f;
+      }
 #pragma unroll
       for (int h = 0; h < kSub; ++h)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          st[h][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[h][r], c, -base));
+          st[h][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[h][r], c, -below));
           sum += st[h][r];
         }
       l = l * corr + sum;

@@ -201,10 +201,11 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
     const float base = m == -INFINITY ? 0.f : m;
     const float corr = __builtin_amdgcn_exp2f(m_old - base);
     float sum = 0.f;
+    const bool far_scores = __any(fabsf(base) >= kFarScore);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       // The product once more, unrounded: near the reference little is left of it.
-      const float x = __builtin_fmaf(st[e >> 2][e & 3], factor[(e >> 2) % kGroups][(e & 3) % kEach], -base);
+      const float x = far_scores ? p[e] - base : __builtin_fmaf(st[e >> 2][e & 3], factor[(e >> 2) % kGroups][(e & 3) % kEach], -base);
       p[e] = __builtin_amdgcn_exp2f(whole || p[e] != -INFINITY ? x : -INFINITY);
       sum += p[e];
     }

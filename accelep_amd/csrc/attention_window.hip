@@ -173,9 +173,10 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
     const float base = m_new == -INFINITY ? 0.f : m_new;
     const float corr = __builtin_amdgcn_exp2f(m - base);
     float sum = 0.f;
+    const bool far_scores = __any(fabsf(base) >= kFarScore);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st0[e], a.factor, -base));
+      p[e] = __builtin_amdgcn_exp2f(far_scores ? st0[e] * a.factor - base : __builtin_fmaf(st0[e], a.factor, -base));
       sum += p[e];
     }
     l = l * corr + sum;

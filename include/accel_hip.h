@@ -298,7 +298,7 @@ ACCEL_HIP_API int accel_hip_read_cache_q8(const AccelHipCacheQ8* cache, int64_t 
  * and may not overlap q or the cache. head_dim is at most 256, kv_heads * head_dim at most 2^24.
  * Rounding: queries and softmax weights enter the products with 22 bits (a query relative to its row's
  * largest value, a weight to the largest), sums are fp32. A row whose query is not finite, or that sees a
- * scale that is not finite, is NaN. Inside a capture whose workspace was not grown before (by the same
+ * scale that is not finite or a score past the largest float, is NaN. Inside a capture whose workspace was not grown before (by the same
  * call, once), the key range is not divided over workgroups. */
 ACCEL_HIP_API int accel_hip_attention_q8(AccelHipBuffer q, const AccelHipCacheQ8* cache, AccelHipBuffer out,
                                          int64_t seq, int64_t position, int64_t heads, int64_t row_stride,
@@ -309,7 +309,7 @@ ACCEL_HIP_API int accel_hip_attention_q8(AccelHipBuffer q, const AccelHipCacheQ8
  * overlap q, k or v. Sizes, captures and queries as above. Rounding: with many rows (more than 16 of a
  * key head, over a long range) queries, keys and values enter the products with 22 bits of their row's
  * largest value and weights with 22 bits of the largest; otherwise in fp32. A key or value that is not
- * finite makes the rows that see it NaN. */
+ * finite makes the rows that see it NaN, and so does a score past the largest float. */
 ACCEL_HIP_API int accel_hip_attention_window(AccelHipBuffer q, AccelHipBuffer k, AccelHipBuffer v, AccelHipBuffer out,
                                              int64_t seq, int64_t position, int64_t heads, int64_t kv_heads,
                                              int64_t head_dim, int64_t row_stride, int64_t window, int64_t sinks);

@@ -6,7 +6,8 @@ import numpy as np
 import pytest
 
 from long_context_dispatch import F32, Q8, many, takes_many_rows
-from long_context_helpers import Cache, assert_within, attend, attention_q8_call, attention_window_call, check, lib
+from long_context_helpers import (Cache, assert_within, attend, attention_q8_call, attention_window_call, check, lib,
+                                  sees)
 
 pytestmark = pytest.mark.gpu
 
@@ -172,3 +173,53 @@ def test_small_values_behind_large_ones_whose_weights_vanish(seq, heads, kv_head
     want, bound = attend(q, k, v, length - seq, 0, 0)
     got = attention_window_call(many(q, copies, F32, length - seq, kv_heads), k, v, length - seq)
     assert_within(got[:, ::copies], want, bound, floor=0)
+
+
+def winners(q, k, position, window=0, sinks=0):
+    """Of each row and head the visible key of the largest score, and whether no rounding of scores can change it: the
+    next score is further below than all they may be off by (2^-14 of the largest sum of |q k|), and 2^10 besides."""
+    seq, heads, dim = q.shape
+    group = heads // k.shape[1]
+    seen = sees(position, seq, len(k), window, sinks)
+    best, sure = np.zeros((seq, heads), int), np.zeros((seq, heads), bool)
+    for h in range(heads):
+        kk, qq = k[:, h // group].astype(np.float64), q[:, h].astype(np.float64)
+        x = np.where(seen, qq @ kk.T / np.sqrt(dim), -np.inf)
+        off = (np.where(seen, np.abs(qq) @ np.abs(kk).T, 0) / np.sqrt(dim)).max(axis=1) * 2.0 ** -14
+        best[:, h] = x.argmax(axis=1)
+        top = np.sort(x, axis=1)[:, -2:]
+        sure[:, h] = top[:, 1] - top[:, 0] > off + 1024
+    return best, sure
+
+
+@pytest.mark.parametrize("seq,length,copies", [(40, 40, 1), (300, 300, 1), *SIZES, (600, 600, 128)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (33, 4)])
+@pytest.mark.parametrize("large", [20, 30, 60, 115])
+@pytest.mark.parametrize("block", [None, 1, 16, 64])
+def test_scores_so_far_apart_that_one_key_wins(seq, length, copies, window, sinks, large, block):
+    """Visible keys of 2^large with ordinary queries: each row's output is the values of its winner, whose score may be
+    far below zero too (the first rows see one key)."""
+    r = np.random.default_rng(49)
+    position = length - seq
+    pairs = F32 if block is None else Q8
+    while copies > 1 and not takes_many_rows(pairs, seq, position, 2 * copies, 2, window, sinks):
+        copies *= 2
+    q = r.standard_normal((seq, 2, 64)).astype(np.float32)
+    if block is None:
+        k, v = (r.standard_normal((length, 2, 64)).astype(np.float32) for _ in "kv")
+        k *= np.float32(2.0 ** large)
+        got = attention_window_call(many(q, copies, pairs, position, 2, window, sinks), k, v, position, window, sinks)
+    else:
+        cache = Cache(length, 2, 64, block)
+        cache.fill(r, length)
+        cache.scale["k"] *= np.float32(2.0 ** large)
+        cache.upload()
+        k, v = cache.values("k"), cache.values("v")
+        got = attention_q8_call(many(q, copies, pairs, position, 2, window, sinks), cache, position, window, sinks)
+    best, sure = winners(q, k, position, window, sinks)
+    assert sure.mean() > 0.9
+    for h in range(2):
+        want = v[best[:, h], h].astype(np.float64)
+        # a weight and its values are cut by 1.5 * 2^-22 each (values of the row's largest) and the quotient rounds
+        bound = 4 * 2.0 ** -22 * np.abs(want).max(axis=1, keepdims=True)
+        assert_within(got[sure[:, h], h * copies], want[sure[:, h]], np.broadcast_to(bound, want.shape)[sure[:, h]], floor=0)
