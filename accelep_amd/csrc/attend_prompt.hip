@@ -17,11 +17,11 @@
 //
 // Bound: the matrix cores at the clock that they leave themselves (1.7-1.9 GHz under this load), with the
 // softmax and the split of its weights between their phases. 2048 rows from position 4097 on, 32 heads on
-// 8 of 128: 311 us, 172 GFLOP in two products, 1.11 PFLOP/s of f16; the matrix cores are busy 65 % of the
-// cycles. fp32, 4096 rows in a window of 1024: 236 us, 60 GFLOP in three products, 0.77 PFLOP/s; busy
+// 8 of 128: 316 us, 172 GFLOP in two products, 1.09 PFLOP/s of f16; the matrix cores are busy 64 % of the
+// cycles. fp32, 4096 rows in a window of 1024: 234 us, 60 GFLOP in three products, 0.77 PFLOP/s; busy
 // 41 %, since each tile of keys is also split there, by every workgroup that reads it.
-// Dims are padded to 64, 128 or 256: the 8-bit case takes 301 us with heads of 80, 305 of 96, 708 of 192 and
-// 707 of 256 (197 of 64), where the registers of a wave no longer hold queries, sums and staging.
+// Dims are padded to 64, 128 or 256: the 8-bit case takes 306 us with heads of 80, 310 of 96, 713 of 192 and
+// 711 of 256 (198 of 64), where the registers of a wave no longer hold queries, sums and staging.
 // Pieces of 8 codes, whose LDS writes have no bank conflicts (those of 16 have, 8 % of the cycles), took
 // 311 us; fp32 in workgroups of eight waves 225, which a variant of its own was not worth.
 #include "attend_common.h"
@@ -33,6 +33,8 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kWaveRows = 32;
 constexpr float kCommonScale = 0x1p9f;
+constexpr float kFarKey = 0x1p90f;  // scores are below 2^37 before the scales
+constexpr float kBackFirst = 0x1p60f;
 constexpr uint32_t kCommonLow = 121u << 23, kCommonHigh = 133u << 23;  // bits of 2^-6 and 2^6
 constexpr int kRows = kWaves * kWaveRows;
 typedef short s4 __attribute__((ext_vector_type(4)));
@@ -46,10 +48,14 @@ struct PromptArgs {
   AttendPartial partial;
 };
 
+// What the registers are shared out for. Head dim 64 fits three waves at 16-byte loads, and needs to be held to
+// it with a scale per key (blocks of 16, 1024 rows: 42.3 us, with 173 registers and two waves 42.6).
+constexpr int WavesPerSimd(int dp, int load) { return dp > 128 ? 1 : dp > 64 || load < 16 ? 2 : 3; }
+
 // kF32: an fp32 cache. kLoad: bytes that may be loaded at once (16, 4 or 1; 16 or 4 for fp32).
 // kUniform: a block holds whole tiles, one scale each.
 template <int DP, bool kF32, int kLoad, bool kUniform>
-__global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel(AttendArgs a, PromptArgs b) {
+__global__ __launch_bounds__(kThreads, WavesPerSimd(DP, kLoad)) void AttendPromptKernel(AttendArgs a, PromptArgs b) {
   constexpr int kParts = kF32 ? 2 : 1;
   constexpr int kKeys = kF32 ? 32 : 64;
   constexpr int kSub = kKeys / 32;
@@ -62,7 +68,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   __shared__ __align__(16) _Float16 vt[2][kParts][kKeys][kVStride];
   __shared__ __align__(16) float sk[2][kKeys];
   __shared__ __align__(16) float sv[2][kKeys];
-  __shared__ int odd[3];  // fp32: the tile has rows of scales of their own; codes: it has a large value scale
+  __shared__ int odd[3];  // fp32: the tile has rows of scales of their own
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -91,7 +97,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
 
   // ---- staging: a thread's pieces of the next tile, from memory to registers and on to LDS ----
   uint4 kreg[kChunks], vreg[kChunks];
-  float ks_next = 0.f, vs_next = 0.f;
+  float ks_next = 0.f, vs_next = 0.f;  // each wave has the scales of all the tile's keys
+  bool marked_next = false;            // and a large one among them
   const auto fetch_plane = [&](const void* base, int32_t t0, uint4 (&x)[kChunks]) {
     if constexpr (kF32) {
       // A row past the range reads its last one, a piece past a head's dims its last: both are not used.
@@ -208,10 +215,10 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       }
     } else {
       move_nan(ks_next, vs_next);
+      marked_next = __any(ks_next >= kFarKey || vs_next >= kLargeScale);
       if (!kUniform && tid < kKeys) {
         sk[buf][tid] = ks_next;
         sv[buf][tid] = vs_next;
-        if (vs_next >= kLargeScale) odd[slot] = 1;
       }
     }
   };
@@ -258,11 +265,12 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
   __syncthreads();
   if (begin < end) put(0, 0);
   float ks = ks_next, vs = vs_next;
+  bool marked = marked_next;
   for (int32_t u = begin; u < end; ++u) {
     const int buf = (u - begin) & 1;
     const int32_t t0 = range.Key(u);
     __syncthreads();
-    if (!kUniform && tid == 0) odd[(u + 2 - begin) % 3] = 0;  // next written behind the next barrier
+    if (kF32 && tid == 0) odd[(u + 2 - begin) % 3] = 0;  // next written behind the next barrier
     if (u + 1 < end) fetch(range.Key(u + 1));
     __builtin_amdgcn_sched_barrier(0);
     const int32_t last = t0 + kKeys - 1;
@@ -293,18 +301,30 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       }
       __builtin_amdgcn_s_setprio(0);
       const bool one_scale = kUniform || (kF32 && odd[(u - begin) % 3] == 0);  // uniform
-      if (!one_scale) {
+      float c = a.factor;
+      if (one_scale) {
+        c *= row_back * (kF32 ? 1.f / kCommonScale : ks);
+      } else {
+        if (kF32 || marked) {
+          // A key's scale could carry the product past the range: the row's scale out first, as far as that
+          // itself cannot.
+          c *= row_back > kBackFirst ? row_back / kBackFirst : 1.f;
+#pragma unroll
+          for (int h = 0; h < kSub; ++h)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[h][r] *= fminf(row_back, kBackFirst);
+        } else {
+          c *= row_back;
+        }
 #pragma unroll
         for (int h = 0; h < kSub; ++h)
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
             const f4 f = *reinterpret_cast<const f4*>(&sk[buf][32 * h + 8 * r4 + 4 * g]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) st[h][4 * r4 + e] *= f[e] * row_back;  // the scales first: they may be far from 1
+            for (int e = 0; e < 4; ++e) st[h][4 * r4 + e] *= f[e];
           }
       }
-      float c = a.factor;
-      if (one_scale) c *= row_back * (kF32 ? 1.f / kCommonScale : ks);
       if (!whole) {
 #pragma unroll
         for (int h = 0; h < kSub; ++h)
@@ -321,7 +341,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       mx = fmaxf(mx, XorLane<32>(mx)) * c;
       // The reference moves only when a score passes it by 8, so the sums are seldom scaled. (fp32 rows'
       // powers of two stay below 2^115, and a weight of 2^8 times that in range.)
-      const float slack = Slack(kF32 ? false : kUniform ? vs >= kLargeScale : odd[(u - begin) % 3] != 0);
+      const float slack = Slack(!kF32 && marked);
       const float m_old = m;
       if (mx > m + slack) m = mx;
       const float base = m == -INFINITY ? 0.f : m;
@@ -427,6 +447,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void AttendPromptKernel
       put(buf ^ 1, (u + 1 - begin) % 3);
       ks = ks_next;
       vs = vs_next;
+      marked = marked_next;
     }
   }
 

@@ -16,8 +16,8 @@ constexpr int kStepKeys = 32;
 // waves of a head take its steps of 32 keys in turn, so that a workgroup reads a key row's heads together
 // (131072 keys of 8 heads of 128, loads alone: a workgroup a head read them at 4.7 TB/s, 4 heads at 5.7).
 // Bound: the cache's bytes over a long range (131072 keys, 32 heads on 8 key heads of 128: 52.3 us, 5.1
-// TB/s, and 5.5 of the join); over a short one the chain of load, products, softmax and products of a
-// wave's few steps (2048 keys, 9 heads on 3 of 64: 5.5 us and 3.6 of the join). Medians, as in all these
+// TB/s, and 5.4 of the join); over a short one the chain of load, products, softmax and products of a
+// wave's few steps (2048 keys, 9 heads on 3 of 64: 5.7 us and 3.7 of the join). Medians, as in all these
 // comments. Keys and values go from memory to registers, and there to f16: no LDS and no barrier in the
 // loop. Lane (j, g) = (lane % 16, lane / 16). Per step
 //  * S^T = K Q^T on v_mfma_f32_16x16x32_f16: the A operand of instruction (c, half) are the codes
@@ -205,7 +205,8 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       // The product once more, unrounded: near the reference little is left of it.
-      const float x = far_scores ? p[e] - base : __builtin_fmaf(st[e >> 2][e & 3], factor[(e >> 2) % kGroups][(e & 3) % kEach], -base);
+      const float f = factor[(e >> 2) % kGroups][(e & 3) % kEach];
+      const float x = far_scores ? p[e] - base : __builtin_fmaf(st[e >> 2][e & 3], f, -base);
       p[e] = __builtin_amdgcn_exp2f(whole || p[e] != -INFINITY ? x : -INFINITY);
       sum += p[e];
     }
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendQ8StepKernel(
 }
 
 // A workgroup's threads are (row, key range, 16-byte piece), `lanes` ranges of a row at a time, up to 8
-// of a thread in flight at once: a round trip to what other workgroups left is all this costs (3.6-5.6 us; the
+// of a thread in flight at once: a round trip to what other workgroups left is all this costs (3.7-5.7 us; the
 // last workgroup of a row to arrive joining them in the step kernel instead took 1-5 us more than this
 // launch, for its stores and loads past the XCDs' caches).
 constexpr int kJoinThreads = 512;

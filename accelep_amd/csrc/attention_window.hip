@@ -22,7 +22,7 @@ struct StepArgs {
 
 // One workgroup per (16 rows of a key head, key range); its waves take its steps of 16 keys in turn.
 // Bound: the bytes of the keys that are seen, and over a window the chain of a wave's one or two steps (4100
-// keys, 32 heads on 8 key heads of 128: 33.6 MB in 13.2 us, 2.5 TB/s). Both products run on
+// keys, 32 heads on 8 key heads of 128: 33.6 MB in 13.1 us, 2.6 TB/s). Both products run on
 // v_mfma_f32_16x16x4f32, which takes fp32 as it is, with every operand straight from memory. Lane (j, g) =
 // (lane % 16, lane / 16):
 //  * S^T = K Q^T: k slot g of instruction (i, e) is dim 16i + 4g + e, so a lane loads 16 bytes of key

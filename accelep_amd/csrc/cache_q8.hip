@@ -6,9 +6,9 @@
 // (amax / 127, or the stored one where that is larger and the block has older rows), and writes the codes:
 // one pass over the rows. Older rows of the block are only touched when the scale grows.
 //
-// Bound: the bytes, 5 a value each way. 4095 rows of 8 heads of 128: append 11.3 us, 42 MB at 3.7 TB/s
+// Bound: the bytes, 5 a value each way. 4095 rows of 8 heads of 128: append 11.0 us, 42 MB at 3.8 TB/s
 // (the loads of a unit, then its largest, then its stores: a unit's phases follow one another, and a
-// reduction stands between); 32768 rows read back 58 us, 336 MB at 5.8 TB/s. One row: 3.4 and 2.3 us,
+// reduction stands between); 32768 rows read back 59 us, 336 MB at 5.7 TB/s. One row: 3.7 and 2.2 us,
 // launch and two dependent round trips.
 #include <algorithm>
 

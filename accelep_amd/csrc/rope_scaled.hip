@@ -10,7 +10,7 @@
 // are on the way while the angles are formed).
 //
 // Bound: the bytes of the values, 8 each in a pass (4096 rows of 40 heads of 128, half of each turned:
-// 168 MB in 35 us, 4.8 TB/s, nearly a copy's rate); a single row is a launch and one dependent load (2.2 us).
+// 168 MB in 35 us, 4.8 TB/s, nearly a copy's rate); a single row is a launch and one dependent load (2.3 us).
 #include <algorithm>
 
 #include "device_common.h"

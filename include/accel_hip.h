@@ -298,8 +298,8 @@ ACCEL_HIP_API int accel_hip_read_cache_q8(const AccelHipCacheQ8* cache, int64_t 
  * and may not overlap q or the cache. head_dim is at most 256, kv_heads * head_dim at most 2^24.
  * Rounding: queries and softmax weights enter the products with 22 bits (a query relative to its row's
  * largest value, a weight to the largest), sums are fp32. A row whose query is not finite, or that sees a
- * scale that is not finite or a score past the largest float, is NaN. Inside a capture whose workspace was not grown before (by the same
- * call, once), the key range is not divided over workgroups. */
+ * scale that is not finite or a score past the largest float, is NaN. Inside a capture whose workspace was
+ * not grown before (by the same call, once), the key range is not divided over workgroups. */
 ACCEL_HIP_API int accel_hip_attention_q8(AccelHipBuffer q, const AccelHipCacheQ8* cache, AccelHipBuffer out,
                                          int64_t seq, int64_t position, int64_t heads, int64_t row_stride,
                                          int64_t window, int64_t sinks);
