@@ -65,6 +65,29 @@ class CacheQ8(C.Structure):
                 ("kv_heads", C.c_int64), ("head_dim", C.c_int64), ("block", C.c_int64)]
 
 
+CACHE_F32, CACHE_F16 = 0, 1
+
+
+class CachePaged(C.Structure):
+    """AccelHipCachePaged."""
+
+    _fields_ = [("k", Buffer), ("v", Buffer), ("type", C.c_int32), ("pages", C.c_int64), ("page", C.c_int64),
+                ("kv_heads", C.c_int64), ("head_dim", C.c_int64)]
+
+
+class Batch(C.Structure):
+    """AccelHipBatch."""
+
+    _fields_ = [("seen", Buffer), ("starts", Buffer), ("table", Buffer), ("requests", C.c_int64), ("rows", C.c_int64),
+                ("width", C.c_int64), ("longest", C.c_int64)]
+
+
+class PagePool(C.Structure):
+    """AccelHipPagePool."""
+
+    _fields_ = [("stack", Buffer), ("state", Buffer), ("pages", C.c_int64), ("page", C.c_int64)]
+
+
 WORK_FN = C.CFUNCTYPE(C.c_int, C.c_void_p)
 
 # name -> (restype, argtypes)
@@ -119,6 +142,13 @@ SIGNATURES = {
     "accel_hip_read_cache_q8": (C.c_int, [C.POINTER(CacheQ8), i64, i64, Buffer, Buffer]),
     "accel_hip_attention_q8": (C.c_int, [Buffer, C.POINTER(CacheQ8), Buffer, i64, i64, i64, i64, i64, i64]),
     "accel_hip_attention_window": (C.c_int, [Buffer, Buffer, Buffer, Buffer, i64, i64, i64, i64, i64, i64, i64, i64]),
+    "accel_hip_batch_tables": (C.c_int, [Buffer, Buffer, C.POINTER(PagePool), C.POINTER(Batch), Buffer, Buffer, Buffer,
+                                         Buffer]),
+    "accel_hip_release_pages": (C.c_int, [Buffer, Buffer, C.POINTER(PagePool), C.POINTER(Batch)]),
+    "accel_hip_append_paged": (C.c_int, [Buffer, Buffer, C.POINTER(CachePaged), Buffer, i64, i64]),
+    "accel_hip_attention_paged": (C.c_int, [Buffer, C.POINTER(CachePaged), C.POINTER(Batch), Buffer, i64, i64, i64]),
+    "accel_hip_attention_packed": (C.c_int, [Buffer, Buffer, Buffer, C.POINTER(Batch), Buffer, i64, i64, i64, i64, i64,
+                                             i64]),
     "accel_hip_time_ms": (C.c_double, [WORK_FN, C.c_void_p, C.c_int32]),
     "accel_hip_event_record": (C.c_int, [C.c_int32]),
     "accel_hip_event_elapsed_ms": (C.c_double, [C.c_int32, C.c_int32]),

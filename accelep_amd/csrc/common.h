@@ -506,6 +506,42 @@ struct AttendArgs {
 };
 void LaunchAttentionQ8(const AttendArgs& a, const Q8Cache& cache, hipStream_t stream);
 void LaunchAttentionWindow(const AttendArgs& a, const float* k, const float* v, hipStream_t stream);
+// ---- many requests from one cache (batch_tables.hip, cache_paged.hip, attend_batch*.hip; the entry points and
+// their checks are in batch.cc) ----
+struct BatchTablesArgs {
+  const int32_t *counts, *lengths, *stack, *state;
+  int32_t *starts, *seen, *table, *slots, *positions, *lengths_after, *state_after;
+  int32_t requests, rows, width, pages, page_shift;  // (width << page_shift) + rows < 2^31 - 256
+};
+void LaunchBatchTables(const BatchTablesArgs& a, hipStream_t stream);
+struct ReleasePagesArgs {
+  const int32_t* keep;
+  int32_t *lengths, *table, *stack, *state;
+  int32_t requests, width, pages, page_shift;
+};
+void LaunchReleasePages(const ReleasePagesArgs& a, hipStream_t stream);
+struct AppendPagedArgs {
+  const float* src[2];
+  void* dst[2];  // fp32 or f16 [slot_count, width]
+  const int32_t* slots;
+  int64_t row_stride;
+  int32_t rows, width, slot_count;
+  bool f16;
+};
+void LaunchAppendPaged(const AppendPagedArgs& a, hipStream_t stream);
+// Attention of a batch. paged: keys and values are pages of a cache, otherwise rows as the queries are.
+struct BatchAttendArgs {
+  const float* q;  // rows of heads * dim, q_stride apart
+  float* out;      // dense
+  const void *k, *v;  // fp32 or f16; a token's row is kv_heads * dim, kv_stride elements apart
+  const int32_t *starts, *seen, *table;  // seen and table: of a cache alone
+  int64_t q_stride, kv_stride;
+  int32_t requests, rows, width, pages, page_shift;  // (width << page_shift) + rows < 2^31 - 256
+  int32_t heads, kv_heads, dim, window, longest;     // window: kNoWindow for none; longest: of the rows, at most
+  float factor;  // log2(e) / sqrt(dim): scores in log2 units
+  bool f16, paged;
+};
+void LaunchAttendBatch(const BatchAttendArgs& a, hipStream_t stream);
 // rng_inout is a device word holding the xorshift32 state; index_dev offsets `chosen`.
 // greedy_work (at least GreedyWorkBytes(vocab) bytes, its first word zero and left zero by
 // each launch; launches sharing it must not overlap) lets a greedy pick run over many

@@ -12,33 +12,8 @@
 namespace accel_hip {
 namespace {
 
-constexpr int64_t kMaxHeadDim = 256;
 constexpr int64_t kMaxBlock = 256;
-constexpr int64_t kMaxRows = 0x7fffffff - 256;  // positions and row counts are 32-bit in the kernels
-constexpr int64_t kMaxKvRow = 1 << 24;           // and a step's offsets from its first key row
 constexpr double kTwoPi = 6.283185307179586476925286766559;
-constexpr double kLog2e = 1.4426950408889634073599246810019;
-
-void Invalid(const char* what) { Fail(ACCEL_HIP_INVALID_ARGUMENT, what); }
-
-// Floats of `rows` rows of `width`, row_stride apart (0: dense).
-int64_t Stride(int64_t row_stride, int64_t width, const char* what) {
-  if (row_stride != 0 && row_stride < width) Invalid(what);
-  return row_stride == 0 ? width : row_stride;
-}
-size_t StridedBytes(int64_t rows, int64_t stride, int64_t width) {
-  if (rows == 0 || width == 0) return 0;
-  const size_t before = CheckedBytes(rows - 1, stride);
-  const size_t last = CheckedBytes(width, 1);
-  if (before > SIZE_MAX - last) Fail(ACCEL_HIP_OVERFLOW, "matrix is too large");
-  return before + last;
-}
-
-bool Overlap(const AccelHipBuffer& a, size_t a_bytes, const AccelHipBuffer& b, size_t b_bytes) {
-  const char* x = static_cast<const char*>(a.data);
-  const char* y = static_cast<const char*>(b.data);
-  return a_bytes > 0 && b_bytes > 0 && x < y + b_bytes && y < x + a_bytes;
-}
 
 // b against `rows` rows of `width` bytes, `stride` bytes apart: what lies between the rows is not theirs.
 bool OverlapsStrided(const AccelHipBuffer& b, size_t bytes, const AccelHipBuffer& to, int64_t rows, size_t stride,
@@ -47,16 +22,6 @@ bool OverlapsStrided(const AccelHipBuffer& b, size_t bytes, const AccelHipBuffer
   if (b.data <= to.data) return true;
   const size_t in_row = static_cast<size_t>(static_cast<const char*>(b.data) - static_cast<const char*>(to.data)) % stride;
   return in_row < width || bytes > stride - in_row;
-}
-
-void RequireAligned(const AccelHipBuffer& b, size_t to, const char* what) {
-  if (reinterpret_cast<uintptr_t>(b.data) % to != 0) Invalid(what);
-}
-
-int64_t HeadRow(int64_t heads, int64_t dim) {
-  CheckedBytes(heads, dim);
-  if (heads > kMaxRows || dim > kMaxRows || heads * dim > kMaxRows) Fail(ACCEL_HIP_OVERFLOW, "matrix is too large");
-  return heads * dim;
 }
 
 // The cache's shape and room.
@@ -125,7 +90,7 @@ bool CheckedAttend(const AccelHipBuffer& q, const AccelHipBuffer& out, int64_t s
   a->dim = static_cast<int32_t>(dim);
   a->window = window == 0 || window >= seen ? kNoWindow : static_cast<int32_t>(window);
   a->sinks = static_cast<int32_t>(std::min(sinks, seen));
-  a->factor = dim > 0 ? static_cast<float>(kLog2e / std::sqrt(static_cast<double>(dim))) : 0.f;
+  a->factor = AttendFactor(dim);
   return out_bytes > 0;
 }
 

@@ -314,6 +314,77 @@ ACCEL_HIP_API int accel_hip_attention_window(AccelHipBuffer q, AccelHipBuffer k,
                                              int64_t seq, int64_t position, int64_t heads, int64_t kv_heads,
                                              int64_t head_dim, int64_t row_stride, int64_t window, int64_t sinks);
 
+/* ---- many requests from one cache --------------------------------------------------------
+ * No reference counterpart: what serves a batch of requests of different lengths. Keys and values lie in
+ * pages that any request may own; how long each request is stays in device memory, so that a captured step
+ * can be replayed while requests grow. Memory and stream as for long contexts above; exact products do not
+ * apply. int32 buffers are aligned to 4 bytes. */
+enum { ACCEL_HIP_CACHE_F32 = 0, ACCEL_HIP_CACHE_F16 = 1 };
+/* The pages of a layer: k and v are [pages, page, kv_heads, head_dim] of `type`. page is a power of two in
+ * 16 .. 256, head_dim at most 256. Slot s is row s % page of page s / page. */
+typedef struct AccelHipCachePaged {
+  AccelHipBuffer k, v;
+  int32_t type; /* ACCEL_HIP_CACHE_* */
+  int64_t pages, page, kv_heads, head_dim;
+} AccelHipCachePaged;
+/* One step of a batch. The new tokens of all requests are rows that lie one behind the other: those of
+ * request r are starts[r] .. starts[r + 1] - 1, its first token is its token seen[r]. table[r] are the pages
+ * of its tokens in order. rows is what there is room for; rows past starts[requests] are padding. longest is
+ * the most new rows of one request where the host knows it, otherwise 0: it chooses kernels, not results. */
+typedef struct AccelHipBatch {
+  AccelHipBuffer seen;   /* int32 [requests] */
+  AccelHipBuffer starts; /* int32 [requests + 1] */
+  AccelHipBuffer table;  /* int32 [requests, width] */
+  int64_t requests, rows, width, longest;
+} AccelHipBatch;
+/* The pages that no request owns: the first state[0] entries of `stack`, the last of them taken first. */
+typedef struct AccelHipPagePool {
+  AccelHipBuffer stack; /* int32 [pages] */
+  AccelHipBuffer state; /* int32 [2]: pages on the stack; requests that the last step had no page for */
+  int64_t pages, page;
+} AccelHipPagePool;
+/* The tables of one step. Request r has lengths[r] tokens in the cache and counts[r] new ones (below 0: 0; what
+ * is past `rows` does not count). Writes starts and seen (the lengths) of the batch; for the pages that the new
+ * tokens begin, in the order of the requests, the pages from the stack's end into the table; for each row its
+ * position and its slot (padding: 0 and -1); lengths_after (lengths + counts) and state_after, which may be
+ * `lengths` and the pool's state themselves. A request whose new pages are not all there, nor those of the requests
+ * before it, or do not fit its table row, takes none: its rows have slot -1, its missing entries become -1,
+ * its length stays, and it is counted in state_after[1]. Who needs no new page is always served. Other
+ * outputs may overlap neither one another nor the inputs. */
+ACCEL_HIP_API int accel_hip_batch_tables(AccelHipBuffer counts, AccelHipBuffer lengths, const AccelHipPagePool* pool,
+                                         const AccelHipBatch* batch, AccelHipBuffer slots, AccelHipBuffer positions,
+                                         AccelHipBuffer lengths_after, AccelHipBuffer state_after);
+/* Cuts requests short: a request with keep[r] (below 0: 0) less than lengths[r] keeps that many tokens (0: it has
+ * ended; drafts that were rejected go the same way). The pages past them, in the order of the requests and
+ * of their tokens, go onto the pool's stack, their table entries become -1 and lengths[r] becomes keep[r].
+ * Entries that are no page are left out. batch gives requests, width and the table; pool's state[1] stays. */
+ACCEL_HIP_API int accel_hip_release_pages(AccelHipBuffer keep, AccelHipBuffer lengths, const AccelHipPagePool* pool,
+                                          const AccelHipBatch* batch);
+/* Rows of k and v (fp32, kv_heads * head_dim a row, row_stride apart) into their slots (int32 [rows]),
+ * rounded to nearest even; past the largest f16 that is an infinity. Rows whose slot is outside the cache are
+ * left out. Two rows may not have the same slot. The planes may overlap neither one another nor k, v and slots. */
+ACCEL_HIP_API int accel_hip_append_paged(AccelHipBuffer k, AccelHipBuffer v, const AccelHipCachePaged* cache,
+                                         AccelHipBuffer slots, int64_t rows, int64_t row_stride);
+/* Causal grouped-query attention (1 / sqrt(head_dim)) of every request's new rows over its own tokens, whose
+ * keys and values, the new rows' too, are in the cache: the row at p sees the keys t <= p, with window > 0 those
+ * with t > p - window. q's rows are row_stride floats apart, out is dense and may not overlap q, the cache
+ * or the batch; padding rows of it stay as they were. Rounding: with an f16 cache, and with many rows
+ * (over fp32), queries, softmax weights and fp32 keys and values enter the products with 22 bits (of their row's
+ * largest value, the weights of the largest), otherwise with all; sums are fp32. A row whose query is not finite,
+ * that sees a key or value that is not, a score past the largest float, or a token without a page (an entry of
+ * the table that is none, a token past the table's width), is NaN; a value that no row sees has no say.
+ * Inside a capture whose workspace was not grown before (by the same call, once), key ranges are not divided
+ * over workgroups. */
+ACCEL_HIP_API int accel_hip_attention_paged(AccelHipBuffer q, const AccelHipCachePaged* cache, const AccelHipBatch* batch,
+                                            AccelHipBuffer out, int64_t heads, int64_t row_stride, int64_t window);
+/* The same over whole prompts that are not in a cache: the keys and values of request r are rows starts[r] ..
+ * starts[r + 1] - 1 of k and v (fp32, kv_heads * head_dim a row, kv_stride floats apart; 0: dense), and its
+ * positions begin at 0. seen, table and width of the batch are not read. q, k and v may be parts of the same rows. */
+ACCEL_HIP_API int accel_hip_attention_packed(AccelHipBuffer q, AccelHipBuffer k, AccelHipBuffer v,
+                                             const AccelHipBatch* batch, AccelHipBuffer out, int64_t heads,
+                                             int64_t kv_heads, int64_t head_dim, int64_t row_stride, int64_t kv_stride,
+                                             int64_t window);
+
 /* ---- timing ----------------------------------------------------------------------------- */
 /* Milliseconds between two HIP events recorded on the library's stream around `iters`
  * back-to-back calls of fn(user); returns < 0 on failure. Used by bench.py. */
