@@ -1,0 +1,231 @@
+// What the attention kernels over a batch of requests share: which part of the batch a workgroup has.
+//
+// How long the requests are is known on the device alone, so every workgroup reads the lengths, counts the steps
+// of all requests and finds its own part: no table of work is made ahead, and a captured launch follows
+// the lengths. A tile is kTileRows rows of a request and key head, row = query * group + head of the group; a step
+// is kStep keys. Ranges of keys have about (all steps) / target steps, so that a batch fills the CUs whatever
+// its lengths, and each part of a tile's range is an item.
+#pragma once
+
+#include "attend_common.h"
+
+namespace accel_hip {
+
+// How the work is divided. ranges 0: no key range is.
+struct BatchSplit {
+  int32_t few;        // the step kernel has the requests of up to `few` rows, the prompt kernel those of more
+  int32_t ranges;     // key ranges a key head that the tiles are cut to, about
+  int32_t min_steps;  // of a range
+  int32_t items;      // room for a key head's partial items: 2 * ranges at most (see FindWork)
+  AttendPartial partial;  // [kv_heads][items][tile rows]
+  int32_t* tiles;     // [tile][kTileInts]: the tiles whose ranges are divided, their count before them
+};
+constexpr int kTileInts = 8;  // first item, items, first row of the request in the batch, first row of the tile, its rows
+
+struct BatchItem {
+  int32_t request, start, seen, rows;  // rows: of the request and a key head
+  int32_t r0;                          // the tile's first
+  int32_t p_first, p_last;             // positions of the tile's rows
+  int32_t low, high;                   // its keys; low is a multiple of a step
+  int32_t begin, end;                  // steps of this item, the first at low
+  int32_t split, splits, partial;      // of the tile's range; where splits > 1, the item's place
+};
+
+// The requests' part of FindWork: shape of request r as this kernel sees it.
+template <int kTileRows, int kStep, bool kFew>
+struct BatchShape {
+  int32_t start, seen, rows, tiles, steps;  // steps: of one tile's range, at most
+  __device__ __forceinline__ BatchShape(const BatchAttendArgs& a, const BatchSplit& b, int32_t group, int32_t r) {
+    start = min(max(a.starts[r], 0), a.rows);
+    const int32_t n = min(max(a.starts[r + 1], start), a.rows) - start;
+    seen = a.paged ? min(max(a.seen[r], 0), a.width << a.page_shift) : 0;
+    rows = n * group;
+    if (kFew ? rows > b.few : rows <= b.few) rows = 0;
+    tiles = (rows + kTileRows - 1) / kTileRows;
+    const int32_t end = seen + n;
+    steps = (end + kStep - 1) / kStep;
+    if (a.window < min(end, 1 << 30)) steps = min(steps, (a.window + (kTileRows + group - 2) / group + 2 * kStep - 2) / kStep);
+    if (rows == 0) steps = 0;
+  }
+};
+
+// What a wave passes on to the others.
+template <int kThreads>
+struct BatchScan {
+  int64_t steps[kThreads / 64];
+  int32_t sums[kThreads / 64][3];
+  int32_t found[4];
+};
+
+// The item-th item of a key head's work; false: there are fewer, or it is empty. Uniform over the workgroup.
+// Items: a request's tiles are cut into `per` = ceil(steps / size) ranges each, size >= all steps / ranges. So all
+// items are at most ranges + all tiles, and those of divided tiles, whose steps / size is above 1, at most twice
+// their steps / size: 2 * ranges.
+template <int kThreads, int kTileRows, int kStep, bool kFew>
+__device__ __forceinline__ bool FindWork(const BatchAttendArgs& a, const BatchSplit& b, int32_t item, bool first_group,
+                                         BatchScan<kThreads>& shared, BatchItem* w) {
+  using Shape = BatchShape<kTileRows, kStep, kFew>;
+  constexpr int kWaves = kThreads / 64;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = tid >> 6;
+  const int32_t group = a.heads / a.kv_heads;
+  int64_t all = 0;
+  int32_t own_tiles = 0, own_steps = 0;  // of the first kThreads requests, which are looked at once
+  for (int32_t r = tid; r < a.requests; r += kThreads) {
+    const Shape x(a, b, group, r);
+    all += static_cast<int64_t>(x.tiles) * x.steps;
+    if (r == tid) {
+      own_tiles = x.tiles;
+      own_steps = x.steps;
+    }
+  }
+  constexpr int32_t kMostSteps = 0x3fffffff;
+  int32_t size = kMostSteps;
+  if (b.ranges > 0) {  // uniform
+    all = WaveButterfly(all, [](int64_t x, int64_t y) { return x + y; });
+    if (lane == 0) shared.steps[wave] = all;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) all += shared.steps[i];
+    size = static_cast<int32_t>(min(int64_t(kMostSteps), max(int64_t(b.min_steps), (all + b.ranges - 1) / b.ranges)));
+  }
+  int32_t before[3] = {0, 0, 0};  // items, items of divided tiles, divided tiles
+  bool here = false;
+  for (int32_t r0 = 0; r0 < a.requests; r0 += kThreads) {
+    int32_t tiles = 0, steps = 0;
+    if (r0 == 0) {
+      tiles = own_tiles;
+      steps = own_steps;
+    } else if (r0 + tid < a.requests) {
+      const Shape x(a, b, group, r0 + tid);
+      tiles = x.tiles;
+      steps = x.steps;
+    }
+    const int32_t per = (steps + size - 1) / size;
+    const int32_t own[3] = {tiles * per, per > 1 ? tiles * per : 0, per > 1 ? tiles : 0};
+    int32_t sum[3] = {own[0], own[1], own[2]};
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1)
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const int32_t x = __shfl_up(sum[i], off);
+        if (lane >= off) sum[i] += x;
+      }
+    if (lane == 63) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) shared.sums[wave][i] = sum[i];
+    }
+    __syncthreads();
+    int32_t total[3] = {0, 0, 0};
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v)
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const int32_t x = shared.sums[v][i];
+        if (v < wave) sum[i] += x;
+        total[i] += x;
+      }
+    const int32_t from = before[0] + sum[0] - own[0];
+    if (item >= from && item - from < own[0]) {
+      shared.found[0] = r0 + tid;
+      shared.found[1] = item - from;
+      shared.found[2] = before[1] + sum[1] - own[1];
+      shared.found[3] = before[2] + sum[2] - own[2];
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) before[i] += total[i];
+    __syncthreads();
+    here = item < before[0];
+    if (here && !(first_group && b.ranges > 0)) break;  // the first workgroup counts on
+  }
+  if (first_group && b.ranges > 0 && tid == 0) b.tiles[0] = before[2];
+  if (!here) return false;
+  const int32_t r = __builtin_amdgcn_readfirstlane(shared.found[0]);
+  const int32_t local = __builtin_amdgcn_readfirstlane(shared.found[1]);
+  const Shape x(a, b, group, r);
+  const int32_t per = (x.steps + size - 1) / size;
+  const int32_t at = local / per;
+  const int32_t tile = x.tiles - 1 - at;  // the rows with the most keys first
+  w->request = r;
+  w->start = x.start;
+  w->seen = x.seen;
+  w->rows = x.rows;
+  w->r0 = tile * kTileRows;
+  w->p_first = x.seen + w->r0 / group;
+  w->p_last = x.seen + (min(w->r0 + kTileRows, x.rows) - 1) / group;
+  w->low = a.window > w->p_first ? 0 : (w->p_first - a.window + 1) / kStep * kStep;
+  w->high = w->p_last + 1;
+  const int32_t steps = (w->high - w->low + kStep - 1) / kStep;
+  w->splits = min((steps + size - 1) / size, per);
+  w->split = local - at * per;
+  if (w->split >= w->splits) return false;
+  const int32_t each = (steps + w->splits - 1) / w->splits;
+  w->begin = min(steps, w->split * each);
+  w->end = min(steps, w->begin + each);
+  const int32_t first = __builtin_amdgcn_readfirstlane(shared.found[2]) + at * per;
+  w->partial = first + w->split;
+  if (per > 1 && w->split == 0 && static_cast<int32_t>(blockIdx.x) % a.kv_heads == 0 && tid == 0) {
+    int32_t* p = b.tiles + static_cast<int64_t>(kTileInts) * (1 + __builtin_amdgcn_readfirstlane(shared.found[3]) + at);
+    p[0] = first;
+    p[1] = w->splits;
+    p[2] = w->start;
+    p[3] = w->r0;
+    p[4] = min(kTileRows, x.rows - w->r0);
+  }
+  return true;
+}
+
+__device__ __forceinline__ bool SeesKey(const BatchAttendArgs& a, int32_t p, int32_t t) { return t <= p && t > p - a.window; }
+
+// Where row rl of the item's tile (rl < rows - r0) lies in the output, in rows of a head.
+__device__ __forceinline__ int64_t BatchOutRow(const BatchAttendArgs& a, int32_t start, int32_t r, int32_t group, int32_t kv) {
+  const int32_t s = r / group;
+  return static_cast<int64_t>(start + s) * a.heads + kv * group + (r - s * group);
+}
+
+// The page of the 16 tokens from t on, and whether there is one.
+struct BatchPages {
+  const int32_t* entries;
+  int32_t width, pages, shift;
+  __device__ __forceinline__ BatchPages(const BatchAttendArgs& a, int32_t request)
+      : entries(a.table + static_cast<int64_t>(request) * a.width), width(a.width), pages(a.pages), shift(a.page_shift) {}
+  __device__ __forceinline__ int32_t Entry(int32_t t) const {
+    const int32_t q = t >> shift;
+    return q < width ? entries[q] : -1;
+  }
+  __device__ __forceinline__ bool Is(int32_t entry) const { return entry >= 0 && entry < pages; }
+  // The slot of token t, on page `entry`, or on page 0 where that is none.
+  __device__ __forceinline__ int64_t Slot(int32_t entry, int32_t t) const {
+    return (static_cast<int64_t>(Is(entry) ? entry : 0) << shift) + (t & ((1 << shift) - 1));
+  }
+};
+
+// kN floats of a query row from dim d on, 0 past the row.
+template <int kN>
+__device__ __forceinline__ void LoadBatchQuery(const float* q, int32_t dim, int d, bool vec, float (&x)[kN]) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < kN / 4; ++i) {
+      const f4 y = d + 4 * i < dim ? *reinterpret_cast<const f4*>(q + d + 4 * i) : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = y[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) x[e] = d + e < dim ? q[d + e] : 0.f;
+  }
+}
+__device__ __forceinline__ bool BatchQueryVec(const BatchAttendArgs& a) {  // uniform
+  return a.dim % 4 == 0 && a.q_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
+}
+
+// Few rows of each request (attend_batch_step.hip), many (attend_batch_prompt.hip). Items: of a key head, at most.
+constexpr int kStepTileRows = 16, kPromptTileRows = 128;
+constexpr int StepKeys(bool f16) { return f16 ? 32 : 16; }
+constexpr int PromptKeys(bool f16) { return f16 ? 64 : 32; }
+void LaunchBatchStep(const BatchAttendArgs& a, const BatchSplit& b, int64_t items, bool vec, hipStream_t stream);
+void LaunchBatchPrompt(const BatchAttendArgs& a, const BatchSplit& b, int64_t items, bool vec, hipStream_t stream);
+
+}  // namespace accel_hip

@@ -1,84 +1,225 @@
-// Attention of a batch of requests, over the pages of a cache or over packed prompts.
-#include "attend_common.h"
+// Attention of a batch of requests, over the pages of a cache or over packed prompts: which kernels a call takes,
+// into how many key ranges, and the join of the ranges.
+#include "attend_batch.h"
 
 namespace accel_hip {
 namespace {
 
-// A wave a row and head: 64 keys at a time, a key a lane for the scores and some dims a lane for the sums.
-__global__ __launch_bounds__(64) void AttendBatchKernel(BatchAttendArgs a) {
-  __shared__ float query[256];
-  const int lane = threadIdx.x;
-  const int32_t row = static_cast<int32_t>(blockIdx.x / static_cast<uint32_t>(a.heads));
-  const int32_t head = static_cast<int32_t>(blockIdx.x - static_cast<uint32_t>(row) * a.heads);
-  const int32_t kv = head / (a.heads / a.kv_heads);
-  int32_t low = -1, high = a.requests;  // the last request whose rows begin at or before this one
-  while (high - low > 1) {
-    const int32_t mid = low + (high - low) / 2;
-    if (a.starts[mid] <= row) low = mid;
-    else high = mid;
-  }
-  if (low < 0 || row >= a.starts[low + 1]) return;
-  const int32_t r = low, start = max(a.starts[r], 0);
-  const int32_t p = (a.paged ? min(max(a.seen[r], 0), a.width << a.page_shift) : 0) + row - start;
-  const float* q = a.q + row * a.q_stride + static_cast<int64_t>(head) * a.dim;
-  bool bad = false;
-  for (int d = lane; d < a.dim; d += 64) {
-    query[d] = q[d];
-    bad = bad || !(fabsf(q[d]) < INFINITY);
-  }
-  __syncthreads();
-  const int32_t first = a.window == kNoWindow ? 0 : max(0, p - a.window + 1);
-  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  const auto value = [&](const void* x, int64_t at) {
-    return a.f16 ? static_cast<float>(static_cast<const _Float16*>(x)[at]) : static_cast<const float*>(x)[at];
-  };
-  for (int32_t t0 = first; t0 <= p; t0 += 64) {
-    const int32_t t = min(t0 + lane, p);
-    int64_t at = start + t;
-    if (a.paged) {
-      const int32_t q = t >> a.page_shift;
-      const int32_t page = q < a.width ? a.table[static_cast<int64_t>(r) * a.width + q] : -1;
-      const bool is = page >= 0 && page < a.pages;
-      bad = bad || !is;
-      at = is ? (static_cast<int64_t>(page) << a.page_shift) + (t & ((1 << a.page_shift) - 1)) : 0;
-    }
-    at = at * a.kv_stride + static_cast<int64_t>(kv) * a.dim;
-    float s = 0.f;
-    for (int d = 0; d < a.dim; ++d) {
-      const float k = value(a.k, at + d), v = value(a.v, at + d);
-      bad = bad || !(fabsf(k) < INFINITY) || !(fabsf(v) < INFINITY);
-      s = fmaf(query[d], k, s);
-    }
-    s = t0 + lane <= p ? s * a.factor : -INFINITY;
-    bad = bad || s == INFINITY;
-    const float m_new = fmaxf(m, WaveButterfly(s, [](float x, float y) { return fmaxf(x, y); }));
-    const float base = m_new == -INFINITY ? 0.f : m_new;
-    const float corr = exp2f(m - base), w = exp2f(s - base - 40.f);  // times 2^-40: sums of large values stay in range
-    l = l * corr + WaveButterfly(w, [](float x, float y) { return x + y; });
-    m = m_new;
+constexpr int kJoinThreads = 256;
+constexpr int kJoinRows = 4;  // of a workgroup and round
+constexpr int kJoinEach = 4;  // ranges in flight at once
+
+// A workgroup's threads are (row, key range, 16-byte piece). Workgroup (tile and key head, y) takes rows 4y .. 4y + 3
+// of each 4 * gridDim.y of a divided tile.
+__global__ __launch_bounds__(kJoinThreads) void BatchJoinKernel(BatchAttendArgs a, BatchSplit b, int32_t tile_rows, bool vec) {
+  __shared__ __align__(16) f4 part_o[kJoinThreads];
+  __shared__ float part_m[kJoinThreads];
+  __shared__ float part_l[kJoinThreads];
+  const int32_t kv = static_cast<int32_t>(blockIdx.x) % a.kv_heads;
+  const int32_t which = static_cast<int32_t>(blockIdx.x) / a.kv_heads;
+  if (which >= b.tiles[0]) return;
+  const int32_t* tile = b.tiles + static_cast<int64_t>(kTileInts) * (1 + which);
+  const int32_t first = tile[0], splits = tile[1], start = tile[2], r0 = tile[3], rows = tile[4];
+  if (splits == 1) return;
+  const int32_t group = a.heads / a.kv_heads;
+  const int dims = PartialDims(a.dim);
+  const int pieces = dims / 4;
+  const int lanes = min(splits, kJoinThreads / (kJoinRows * pieces));
+  const int per_row = pieces * lanes;
+  const int local = static_cast<int>(threadIdx.x) / per_row;
+  const int rest = static_cast<int>(threadIdx.x) - local * per_row;
+  const int of = rest / pieces;
+  const int piece = rest - of * pieces;
+  for (int32_t base_row = kJoinRows * static_cast<int32_t>(blockIdx.y); base_row < rows;
+       base_row += kJoinRows * static_cast<int32_t>(gridDim.y)) {
+    const int32_t rl = base_row + local;
+    const bool active = local < kJoinRows && rl < rows;
+    const int64_t at0 = (static_cast<int64_t>(kv) * b.items + first) * tile_rows + rl;  // the next range's: tile_rows on
+    const auto ml_of = [&](int c) {
+      return *reinterpret_cast<const float2*>(b.partial.ml + 2 * (at0 + static_cast<int64_t>(c) * tile_rows));
+    };
+    const auto o_of = [&](int c) {
+      return *reinterpret_cast<const f4*>(b.partial.o + (at0 + static_cast<int64_t>(c) * tile_rows) * dims + 4 * piece);
+    };
+    float m = -INFINITY, l = 0.f, low = 0.f;
+    f4 sum = f4{0.f, 0.f, 0.f, 0.f};
+    if (active) {
+      for (int c0 = of; c0 < splits; c0 += lanes * kJoinEach) {
+        float2 y[kJoinEach];
+        f4 x[kJoinEach];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] *= corr;
-    for (int e = 0; e < 64; ++e) {
-      const float we = __shfl(w, e);
-      const int64_t ae = __shfl(at, e);
+        for (int i = 0; i < kJoinEach; ++i) {
+          const int c = min(c0 + i * lanes, splits - 1);
+          y[i] = ml_of(c);
+          x[i] = o_of(c);
+        }
+        float big = m;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < a.dim) acc[i] = fmaf(we, value(a.v, ae + lane + 64 * i), acc[i]);
+        for (int i = 0; i < kJoinEach; ++i)
+          if (c0 + i * lanes < splits) big = fmaxf(big, y[i].x);
+        const float base = big == -INFINITY ? 0.f : big;
+        const float corr = __builtin_amdgcn_exp2f(m - base);
+        l *= corr;
+        sum *= corr;
+#pragma unroll
+        for (int i = 0; i < kJoinEach; ++i) {
+          if (c0 + i * lanes >= splits) break;
+          const float wt = __builtin_amdgcn_exp2f(y[i].x - base);
+          low = fminf(low, y[i].y);
+          l += wt * y[i].y;
+          sum += wt * x[i];
+        }
+        m = big;
+      }
+      part_m[threadIdx.x] = m;
+      part_l[threadIdx.x] = low < 0.f ? -1.f : l;
+      part_o[threadIdx.x] = sum;
     }
+    __syncthreads();
+    if (active && of == 0) {
+      const int at = threadIdx.x;
+      float big = -INFINITY;
+      for (int i = 0; i < lanes; ++i) big = fmaxf(big, part_m[at + i * pieces]);
+      const float base = big == -INFINITY ? 0.f : big;
+      float total = 0.f;
+      low = 0.f;
+      sum = f4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < lanes; ++i) {
+        const float wt = __builtin_amdgcn_exp2f(part_m[at + i * pieces] - base);
+        low = fminf(low, part_l[at + i * pieces]);
+        total += wt * part_l[at + i * pieces];
+        sum += wt * part_o[at + i * pieces];
+      }
+      f4 far = f4{0.f, 0.f, 0.f, 0.f};
+      if (low < 0.f) {  // some parts are held times 2^-64: their sum is one of its own
+        total = 0.f;
+        sum = far;
+        for (int c = 0; c < splits; ++c) {
+          const float2 y = ml_of(c);
+          const float wt = __builtin_amdgcn_exp2f(y.x - base);
+          const f4 x = wt * o_of(c);
+          total += wt * fabsf(y.y);
+          if (y.y < 0.f) far += x;
+          else sum += x;
+        }
+      }
+      float* dst = a.out + BatchOutRow(a, start, r0 + rl, group, kv) * a.dim + 4 * piece;
+      f4 y = f4{__fdiv_rn(sum[0], total), __fdiv_rn(sum[1], total), __fdiv_rn(sum[2], total), __fdiv_rn(sum[3], total)};
+      if (low < 0.f)
+        y += f4{__fdiv_rn(far[0], total), __fdiv_rn(far[1], total), __fdiv_rn(far[2], total), __fdiv_rn(far[3], total)} * kFarUp;
+      if (vec) {
+        *reinterpret_cast<f4*>(dst) = y;
+      } else {
+        for (int e = 0; e < 4; ++e)
+          if (4 * piece + e < a.dim) dst[e] = y[e];
+      }
+    }
+    __syncthreads();
   }
-  bad = __any(bad);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < a.dim)
-      a.out[(static_cast<int64_t>(row) * a.heads + head) * a.dim + lane + 64 * i] = bad ? NAN : __fdiv_rn(acc[i], l);
+}
+
+// One kernel's share of a call: the step kernel's (few rows) or the prompt kernel's.
+struct Share {
+  int32_t tile_rows, keys;
+  int64_t tiles;      // of a key head, at most
+  int64_t ranges;     // a key head's key ranges, about; 0: no range is divided
+  int64_t min_steps;  // of a range
+  int64_t items;      // a key head's partial items, at most
+  size_t ml_bytes, o_bytes, tile_bytes;
+};
+
+size_t Round16(size_t bytes) { return (bytes + 15) & ~size_t(15); }
+
+Share ShareOf(const BatchAttendArgs& a, int32_t tile_rows, int32_t keys, int64_t tiles, int64_t groups, int64_t min_steps) {
+  Share s{tile_rows, keys, tiles, 0, min_steps, 0, 0, 0, 0};
+  const int64_t most_keys = std::min<int64_t>(a.paged ? (int64_t(a.width) << a.page_shift) + a.longest : a.rows,
+                                              int64_t(a.window) + a.longest + 2 * keys);
+  const int64_t most_steps = (most_keys + keys - 1) / keys;
+  if (most_steps <= min_steps) return s;
+  s.ranges = std::max<int64_t>(1, groups / a.kv_heads);
+  s.items = std::min<int64_t>(2 * s.ranges, tiles * ((most_steps + min_steps - 1) / min_steps));
+  const size_t parts = static_cast<size_t>(s.items) * a.kv_heads * tile_rows;
+  s.ml_bytes = Round16(parts * 2 * sizeof(float));
+  s.o_bytes = Round16(parts * PartialDims(a.dim) * sizeof(float));
+  s.tile_bytes = static_cast<size_t>(std::min<int64_t>(s.items, tiles) + 1) * kTileInts * sizeof(int32_t);
+  return s;
+}
+
+size_t Bytes(const Share& s) { return s.ranges > 0 ? s.ml_bytes + s.o_bytes + s.tile_bytes : 0; }
+
+BatchSplit SplitOf(const Share& s, int32_t few, char* scratch) {
+  BatchSplit b{};
+  b.few = few;
+  b.min_steps = static_cast<int32_t>(s.min_steps);
+  if (s.ranges == 0 || scratch == nullptr) return b;
+  b.ranges = static_cast<int32_t>(s.ranges);
+  b.items = static_cast<int32_t>(s.items);
+  b.partial.ml = reinterpret_cast<float*>(scratch);
+  b.partial.o = reinterpret_cast<float*>(scratch + s.ml_bytes);
+  b.tiles = reinterpret_cast<int32_t*>(scratch + s.ml_bytes + s.o_bytes);
+  return b;
+}
+
+void LaunchJoin(const BatchAttendArgs& a, const BatchSplit& b, const Share& s, hipStream_t stream) {
+  if (b.ranges == 0) return;
+  const bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+  const int64_t rows = std::min<int64_t>(s.tile_rows, int64_t(a.longest) * (a.heads / a.kv_heads));
+  const int64_t row_groups = (rows + kJoinRows - 1) / kJoinRows;
+  const dim3 grid(GridOf(std::min<int64_t>(s.items, s.tiles) * a.kv_heads, kJoinThreads * row_groups, "Attention is too large"),
+                  static_cast<uint32_t>(row_groups));
+  hipLaunchKernelGGL(BatchJoinKernel, grid, dim3(kJoinThreads), 0, stream, a, b, s.tile_rows, vec);
+  Check(hipGetLastError(), "BatchJoinKernel launch");
 }
 
 }  // namespace
 
 void LaunchAttendBatch(const BatchAttendArgs& a, hipStream_t stream) {
-  const int64_t units = int64_t(a.rows) * a.heads;
-  hipLaunchKernelGGL(AttendBatchKernel, dim3(GridOf(units, 64, "Attention is too large")), dim3(64), 0, stream, a);
-  Check(hipGetLastError(), "AttendBatchKernel launch");
+  const int64_t cus = Ctx().cu_count > 0 ? Ctx().cu_count : 256;
+  const int64_t group = a.heads / a.kv_heads;
+  const int64_t all_rows = int64_t(a.rows) * group;
+  const int32_t align = a.f16 ? 8 : 4;
+  const bool vec = a.dim % align == 0 && a.kv_stride % align == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
+  // Requests of up to 16 rows of a key head are the step kernel's, larger ones the prompt kernel's. Where no request
+  // has more, the first has all (also one that is longer than `longest` says); packed prompts, whose short ones
+  // have few keys too, are the second's.
+  constexpr int32_t kAll = 0x7fffffff;
+  const bool steps_only = a.longest * group <= kStepTileRows;
+  const bool steps = steps_only || (a.paged && group <= kStepTileRows);
+  const int32_t few = steps_only ? kAll : steps ? kStepTileRows : 0;
+  Share step{}, prompt{};
+  if (steps) {
+    const int64_t tiles = std::min<int64_t>(a.requests, a.rows) + (steps_only ? all_rows / kStepTileRows : 0);
+    step = ShareOf(a, kStepTileRows, StepKeys(a.f16), tiles, 4 * cus, 8);
+  }
+  if (!steps_only) {
+    const int64_t tiles = all_rows / kPromptTileRows + std::min<int64_t>(a.requests, all_rows / (few + 1));
+    prompt = ShareOf(a, kPromptTileRows, PromptKeys(a.f16), tiles, 2 * cus, 4);
+  }
+  // Both kernels' parts lie in the same memory, one after the other. Where there is none the ranges stay whole.
+  std::unique_lock<std::mutex> held;
+  char* scratch = nullptr;
+  const size_t bytes = std::max(Bytes(step), Bytes(prompt));
+  if (bytes > 0) {
+    held = std::unique_lock<std::mutex>(AttendPartsMutex());
+    if (ScratchReady(0, kTempAttend, bytes)) {
+      try {
+        scratch = static_cast<char*>(Temp(kTempAttend, bytes));
+      } catch (const Error& e) {
+        if (e.code != ACCEL_HIP_BAD_ALLOC) throw;
+      }
+    }
+  }
+  if (steps) {
+    const BatchSplit b = SplitOf(step, few, scratch);
+    LaunchBatchStep(a, b, step.tiles + b.ranges, vec, stream);
+    LaunchJoin(a, b, step, stream);
+  }
+  if (!steps_only) {
+    const BatchSplit b = SplitOf(prompt, few, scratch);
+    LaunchBatchPrompt(a, b, prompt.tiles + b.ranges, vec, stream);
+    LaunchJoin(a, b, prompt, stream);
+  }
 }
 
 }  // namespace accel_hip
