@@ -16,7 +16,7 @@ struct BatchSplit {
   int32_t few;        // the step kernel has the requests of up to `few` rows, the prompt kernel those of more
   int32_t ranges;     // key ranges a key head that the tiles are cut to, about
   int32_t min_steps;  // of a range
-  int32_t items;      // room for a key head's partial items: 2 * ranges at most (see FindWork)
+  int32_t items;      // room for a key head's partial items: 4 * ranges at most (see FindWork)
   AttendPartial partial;  // [kv_heads][items][tile rows]
   int32_t* tiles;     // [tile][kTileInts]: the tiles whose ranges are divided, their count before them
 };
@@ -35,6 +35,7 @@ struct BatchItem {
 template <int kTileRows, int kStep, bool kFew>
 struct BatchShape {
   int32_t start, seen, rows, tiles, steps;  // steps: of one tile's range, at most
+  int64_t work;                             // of all tiles' ranges, half of tiles * steps at least
   __device__ __forceinline__ BatchShape(const BatchAttendArgs& a, const BatchSplit& b, int32_t group, int32_t r) {
     start = min(max(a.starts[r], 0), a.rows);
     const int32_t n = min(max(a.starts[r + 1], start), a.rows) - start;
@@ -46,6 +47,9 @@ struct BatchShape {
     steps = (end + kStep - 1) / kStep;
     if (a.window < min(end, 1 << 30)) steps = min(steps, (a.window + (kTileRows + group - 2) / group + 2 * kStep - 2) / kStep);
     if (rows == 0) steps = 0;
+    // The first tile's range ends at its own rows, and without a window those between grow evenly.
+    const int32_t first = min(steps, (seen + min(n, (kTileRows + group - 1) / group) + kStep - 1) / kStep);
+    work = (static_cast<int64_t>(tiles) * (a.window < end ? 2 * steps : first + steps) + 1) / 2;
   }
 };
 
@@ -57,12 +61,13 @@ struct BatchScan {
   int32_t found[4];
 };
 
-// The item-th item of a key head's work; false: there are fewer, or it is empty. Uniform over the workgroup.
-// Items: a request's tiles are cut into `per` = ceil(steps / size) ranges each, size >= all steps / ranges. So all
-// items are at most ranges + all tiles, and those of divided tiles, whose steps / size is above 1, at most twice
-// their steps / size: 2 * ranges.
+// The item-th item of a key head's work; false: there are fewer, or it is empty. Uniform over the workgroup. lead: of
+// the first key head, whose workgroups note the divided tiles.
+// Items: a request's tiles are cut into `per` = ceil(steps / size) ranges each, size >= all work / ranges. A request's
+// tiles * steps is at most twice its work, so all items are at most 2 * ranges + all tiles, and those of divided tiles,
+// whose steps / size is above 1, at most twice their steps / size: 4 * ranges. Divided tiles: 2 * ranges.
 template <int kThreads, int kTileRows, int kStep, bool kFew>
-__device__ __forceinline__ bool FindWork(const BatchAttendArgs& a, const BatchSplit& b, int32_t item, bool first_group,
+__device__ __forceinline__ bool FindWork(const BatchAttendArgs& a, const BatchSplit& b, int32_t item, bool lead,
                                          BatchScan<kThreads>& shared, BatchItem* w) {
   using Shape = BatchShape<kTileRows, kStep, kFew>;
   constexpr int kWaves = kThreads / 64;
@@ -70,11 +75,12 @@ __device__ __forceinline__ bool FindWork(const BatchAttendArgs& a, const BatchSp
   const int lane = tid & 63;
   const int wave = tid >> 6;
   const int32_t group = a.heads / a.kv_heads;
+  const bool first_group = lead && item == 0;
   int64_t all = 0;
   int32_t own_tiles = 0, own_steps = 0;  // of the first kThreads requests, which are looked at once
   for (int32_t r = tid; r < a.requests; r += kThreads) {
     const Shape x(a, b, group, r);
-    all += static_cast<int64_t>(x.tiles) * x.steps;
+    all += x.work;
     if (r == tid) {
       own_tiles = x.tiles;
       own_steps = x.steps;
@@ -148,26 +154,27 @@ __device__ __forceinline__ bool FindWork(const BatchAttendArgs& a, const BatchSp
   const int32_t per = (x.steps + size - 1) / size;
   const int32_t at = local / per;
   const int32_t tile = x.tiles - 1 - at;  // the rows with the most keys first
+  const auto uniform = [](int32_t x) { return __builtin_amdgcn_readfirstlane(x); };  // and in scalar registers
   w->request = r;
-  w->start = x.start;
-  w->seen = x.seen;
-  w->rows = x.rows;
-  w->r0 = tile * kTileRows;
-  w->p_first = x.seen + w->r0 / group;
-  w->p_last = x.seen + (min(w->r0 + kTileRows, x.rows) - 1) / group;
-  w->low = a.window > w->p_first ? 0 : (w->p_first - a.window + 1) / kStep * kStep;
+  w->start = uniform(x.start);
+  w->seen = uniform(x.seen);
+  w->rows = uniform(x.rows);
+  w->r0 = uniform(tile * kTileRows);
+  w->p_first = uniform(x.seen + w->r0 / group);
+  w->p_last = uniform(x.seen + (min(w->r0 + kTileRows, x.rows) - 1) / group);
+  w->low = uniform(a.window > w->p_first ? 0 : (w->p_first - a.window + 1) / kStep * kStep);
   w->high = w->p_last + 1;
   const int32_t steps = (w->high - w->low + kStep - 1) / kStep;
-  w->splits = min((steps + size - 1) / size, per);
-  w->split = local - at * per;
+  w->splits = uniform(min((steps + size - 1) / size, per));
+  w->split = uniform(local - at * per);
   if (w->split >= w->splits) return false;
-  const int32_t each = (steps + w->splits - 1) / w->splits;
+  const int32_t each = uniform((steps + w->splits - 1) / w->splits);
   w->begin = min(steps, w->split * each);
   w->end = min(steps, w->begin + each);
-  const int32_t first = __builtin_amdgcn_readfirstlane(shared.found[2]) + at * per;
+  const int32_t first = uniform(shared.found[2] + at * per);
   w->partial = first + w->split;
-  if (per > 1 && w->split == 0 && static_cast<int32_t>(blockIdx.x) % a.kv_heads == 0 && tid == 0) {
-    int32_t* p = b.tiles + static_cast<int64_t>(kTileInts) * (1 + __builtin_amdgcn_readfirstlane(shared.found[3]) + at);
+  if (per > 1 && w->split == 0 && lead && tid == 0) {
+    int32_t* p = b.tiles + static_cast<int64_t>(kTileInts) * (1 + uniform(shared.found[3] + at));
     p[0] = first;
     p[1] = w->splits;
     p[2] = w->start;
@@ -221,11 +228,20 @@ __device__ __forceinline__ bool BatchQueryVec(const BatchAttendArgs& a) {  // un
   return a.dim % 4 == 0 && a.q_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
 }
 
-// Few rows of each request (attend_batch_step.hip), many (attend_batch_prompt.hip). Items: of a key head, at most.
+constexpr int kBatchThreads = 256;
 constexpr int kStepTileRows = 16, kPromptTileRows = 128;
 constexpr int StepKeys(bool f16) { return f16 ? 32 : 16; }
 constexpr int PromptKeys(bool f16) { return f16 ? 64 : 32; }
-void LaunchBatchStep(const BatchAttendArgs& a, const BatchSplit& b, int64_t items, bool vec, hipStream_t stream);
-void LaunchBatchPrompt(const BatchAttendArgs& a, const BatchSplit& b, int64_t items, bool vec, hipStream_t stream);
+
+// A call's two shares: the tiles of requests with few rows and of those with many. groups: workgroups of each.
+struct BatchLaunch {
+  BatchAttendArgs a;
+  BatchSplit step, prompt;
+  uint32_t step_groups, prompt_groups;
+};
+// One of them alone (attend_batch_step.hip, attend_batch_prompt.hip), or both in one launch (attend_batch_mixed.hip).
+void LaunchBatchStep(const BatchLaunch& args, bool vec, hipStream_t stream);
+void LaunchBatchPrompt(const BatchLaunch& args, bool vec, hipStream_t stream);
+void LaunchBatchMixed(const BatchLaunch& args, bool vec, hipStream_t stream);
 
 }  // namespace accel_hip

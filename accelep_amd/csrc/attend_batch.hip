@@ -5,18 +5,22 @@
 namespace accel_hip {
 namespace {
 
-constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 4;  // of a workgroup and round
 constexpr int kJoinEach = 4;  // ranges in flight at once
 
 // A workgroup's threads are (row, key range, 16-byte piece). Workgroup (tile and key head, y) takes rows 4y .. 4y + 3
-// of each 4 * gridDim.y of a divided tile.
-__global__ __launch_bounds__(kJoinThreads) void BatchJoinKernel(BatchAttendArgs a, BatchSplit b, int32_t tile_rows, bool vec) {
-  __shared__ __align__(16) f4 part_o[kJoinThreads];
-  __shared__ float part_m[kJoinThreads];
-  __shared__ float part_l[kJoinThreads];
-  const int32_t kv = static_cast<int32_t>(blockIdx.x) % a.kv_heads;
-  const int32_t which = static_cast<int32_t>(blockIdx.x) / a.kv_heads;
+// of each 4 * gridDim.y of a divided tile; prompt_tiles: tiles and key heads of the prompt's share, which come first.
+__global__ __launch_bounds__(kBatchThreads) void BatchJoinKernel(BatchLaunch args, uint32_t prompt_tiles, bool vec) {
+  __shared__ __align__(16) f4 part_o[kBatchThreads];
+  __shared__ float part_m[kBatchThreads];
+  __shared__ float part_l[kBatchThreads];
+  const BatchAttendArgs& a = args.a;
+  const bool prompt = blockIdx.x < prompt_tiles;
+  const BatchSplit& b = prompt ? args.prompt : args.step;
+  const int32_t tile_rows = prompt ? kPromptTileRows : kStepTileRows;
+  const int32_t block = static_cast<int32_t>(blockIdx.x - (prompt ? 0 : prompt_tiles));
+  const int32_t kv = block % a.kv_heads;
+  const int32_t which = block / a.kv_heads;
   if (which >= b.tiles[0]) return;
   const int32_t* tile = b.tiles + static_cast<int64_t>(kTileInts) * (1 + which);
   const int32_t first = tile[0], splits = tile[1], start = tile[2], r0 = tile[3], rows = tile[4];
@@ -24,7 +28,7 @@ __global__ __launch_bounds__(kJoinThreads) void BatchJoinKernel(BatchAttendArgs 
   const int32_t group = a.heads / a.kv_heads;
   const int dims = PartialDims(a.dim);
   const int pieces = dims / 4;
-  const int lanes = min(splits, kJoinThreads / (kJoinRows * pieces));
+  const int lanes = min(splits, kBatchThreads / (kJoinRows * pieces));
   const int per_row = pieces * lanes;
   const int local = static_cast<int>(threadIdx.x) / per_row;
   const int rest = static_cast<int>(threadIdx.x) - local * per_row;
@@ -118,34 +122,35 @@ __global__ __launch_bounds__(kJoinThreads) void BatchJoinKernel(BatchAttendArgs 
   }
 }
 
-// One kernel's share of a call: the step kernel's (few rows) or the prompt kernel's.
+// One share of a call: the tiles of requests with few rows, or of those with many.
 struct Share {
-  int32_t tile_rows, keys;
+  int32_t tile_rows;
   int64_t tiles;      // of a key head, at most
   int64_t ranges;     // a key head's key ranges, about; 0: no range is divided
   int64_t min_steps;  // of a range
   int64_t items;      // a key head's partial items, at most
+  int64_t divided;    // a key head's divided tiles, at most
   size_t ml_bytes, o_bytes, tile_bytes;
+  size_t Bytes() const { return ml_bytes + o_bytes + tile_bytes; }
 };
 
 size_t Round16(size_t bytes) { return (bytes + 15) & ~size_t(15); }
 
 Share ShareOf(const BatchAttendArgs& a, int32_t tile_rows, int32_t keys, int64_t tiles, int64_t groups, int64_t min_steps) {
-  Share s{tile_rows, keys, tiles, 0, min_steps, 0, 0, 0, 0};
-  const int64_t most_keys = std::min<int64_t>(a.paged ? (int64_t(a.width) << a.page_shift) + a.longest : a.rows,
-                                              int64_t(a.window) + a.longest + 2 * keys);
+  Share s{tile_rows, tiles, 0, min_steps, 0, 0, 0, 0, 0};
+  const int64_t most_keys = std::min<int64_t>(a.paged ? (int64_t(a.width) << a.page_shift) + a.rows : a.rows,
+                                              int64_t(a.window) + tile_rows + 2 * keys);
   const int64_t most_steps = (most_keys + keys - 1) / keys;
   if (most_steps <= min_steps) return s;
   s.ranges = std::max<int64_t>(1, groups / a.kv_heads);
-  s.items = std::min<int64_t>(2 * s.ranges, tiles * ((most_steps + min_steps - 1) / min_steps));
+  s.items = std::min<int64_t>(4 * s.ranges, tiles * ((most_steps + min_steps - 1) / min_steps));
+  s.divided = std::min<int64_t>(2 * s.ranges, tiles);
   const size_t parts = static_cast<size_t>(s.items) * a.kv_heads * tile_rows;
   s.ml_bytes = Round16(parts * 2 * sizeof(float));
   s.o_bytes = Round16(parts * PartialDims(a.dim) * sizeof(float));
-  s.tile_bytes = static_cast<size_t>(std::min<int64_t>(s.items, tiles) + 1) * kTileInts * sizeof(int32_t);
+  s.tile_bytes = Round16(static_cast<size_t>(s.divided + 1) * kTileInts * sizeof(int32_t));
   return s;
 }
-
-size_t Bytes(const Share& s) { return s.ranges > 0 ? s.ml_bytes + s.o_bytes + s.tile_bytes : 0; }
 
 BatchSplit SplitOf(const Share& s, int32_t few, char* scratch) {
   BatchSplit b{};
@@ -160,14 +165,19 @@ BatchSplit SplitOf(const Share& s, int32_t few, char* scratch) {
   return b;
 }
 
-void LaunchJoin(const BatchAttendArgs& a, const BatchSplit& b, const Share& s, hipStream_t stream) {
-  if (b.ranges == 0) return;
+constexpr const char* kTooLarge = "Attention is too large";
+
+void LaunchJoin(const BatchLaunch& args, const Share& step, const Share& prompt, hipStream_t stream) {
+  const BatchAttendArgs& a = args.a;
+  const int64_t step_tiles = args.step.ranges > 0 ? step.divided * a.kv_heads : 0;
+  const int64_t prompt_tiles = args.prompt.ranges > 0 ? prompt.divided * a.kv_heads : 0;
+  if (step_tiles + prompt_tiles == 0) return;
   const bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
-  const int64_t rows = std::min<int64_t>(s.tile_rows, int64_t(a.longest) * (a.heads / a.kv_heads));
+  const int64_t rows = std::min<int64_t>(prompt_tiles > 0 ? kPromptTileRows : kStepTileRows,
+                                         int64_t(a.longest) * (a.heads / a.kv_heads));
   const int64_t row_groups = (rows + kJoinRows - 1) / kJoinRows;
-  const dim3 grid(GridOf(std::min<int64_t>(s.items, s.tiles) * a.kv_heads, kJoinThreads * row_groups, "Attention is too large"),
-                  static_cast<uint32_t>(row_groups));
-  hipLaunchKernelGGL(BatchJoinKernel, grid, dim3(kJoinThreads), 0, stream, a, b, s.tile_rows, vec);
+  const dim3 grid(GridOf(step_tiles + prompt_tiles, kBatchThreads * row_groups, kTooLarge), static_cast<uint32_t>(row_groups));
+  hipLaunchKernelGGL(BatchJoinKernel, grid, dim3(kBatchThreads), 0, stream, args, static_cast<uint32_t>(prompt_tiles), vec);
   Check(hipGetLastError(), "BatchJoinKernel launch");
 }
 
@@ -180,8 +190,8 @@ void LaunchAttendBatch(const BatchAttendArgs& a, hipStream_t stream) {
   const int32_t align = a.f16 ? 8 : 4;
   const bool vec = a.dim % align == 0 && a.kv_stride % align == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
-  // Requests of up to 16 rows of a key head are the step kernel's, larger ones the prompt kernel's. Where no request
-  // has more, the first has all (also one that is longer than `longest` says); packed prompts, whose short ones
+  // Requests of up to 16 rows of a key head are the step tiles', larger ones the prompt tiles'. Where no request
+  // has more, the first have all (also one that is longer than `longest` says); packed prompts, whose short ones
   // have few keys too, are the second's.
   constexpr int32_t kAll = 0x7fffffff;
   const bool steps_only = a.longest * group <= kStepTileRows;
@@ -196,10 +206,10 @@ void LaunchAttendBatch(const BatchAttendArgs& a, hipStream_t stream) {
     const int64_t tiles = all_rows / kPromptTileRows + std::min<int64_t>(a.requests, all_rows / (few + 1));
     prompt = ShareOf(a, kPromptTileRows, PromptKeys(a.f16), tiles, 2 * cus, 4);
   }
-  // Both kernels' parts lie in the same memory, one after the other. Where there is none the ranges stay whole.
+  // Where there is no memory for the parts the ranges stay whole.
   std::unique_lock<std::mutex> held;
   char* scratch = nullptr;
-  const size_t bytes = std::max(Bytes(step), Bytes(prompt));
+  const size_t bytes = step.Bytes() + prompt.Bytes();
   if (bytes > 0) {
     held = std::unique_lock<std::mutex>(AttendPartsMutex());
     if (ScratchReady(0, kTempAttend, bytes)) {
@@ -210,16 +220,15 @@ void LaunchAttendBatch(const BatchAttendArgs& a, hipStream_t stream) {
       }
     }
   }
-  if (steps) {
-    const BatchSplit b = SplitOf(step, few, scratch);
-    LaunchBatchStep(a, b, step.tiles + b.ranges, vec, stream);
-    LaunchJoin(a, b, step, stream);
-  }
-  if (!steps_only) {
-    const BatchSplit b = SplitOf(prompt, few, scratch);
-    LaunchBatchPrompt(a, b, prompt.tiles + b.ranges, vec, stream);
-    LaunchJoin(a, b, prompt, stream);
-  }
+  BatchLaunch args{a, SplitOf(step, few, scratch), SplitOf(prompt, few, scratch == nullptr ? nullptr : scratch + step.Bytes()), 0, 0};
+  // A key head's items are 2 * ranges and the tiles at most.
+  args.step_groups = steps ? GridOf((step.tiles + 2 * args.step.ranges) * a.kv_heads, kBatchThreads, kTooLarge) : 0;
+  args.prompt_groups = steps_only ? 0 : GridOf((prompt.tiles + 2 * args.prompt.ranges) * a.kv_heads, kBatchThreads, kTooLarge);
+  GridOf(int64_t(args.step_groups) + args.prompt_groups, kBatchThreads, kTooLarge);
+  if (steps_only) LaunchBatchStep(args, vec, stream);
+  else if (a.paged) LaunchBatchMixed(args, vec, stream);
+  else LaunchBatchPrompt(args, vec, stream);
+  LaunchJoin(args, step, prompt, stream);
 }
 
 }  // namespace accel_hip
