@@ -22,6 +22,21 @@ struct BatchSplit {
 };
 constexpr int kTileInts = 8;  // first item, items, first row of the request in the batch, first row of the tile, its rows
 
+__device__ __forceinline__ int32_t Quotient(int32_t x, const QuickDivisor& d) {
+  return static_cast<int32_t>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * d.mul >> d.shift);
+}
+
+// Sums over the lanes up to this one: shifts inside rows of 16, then the ends of the rows before.
+__device__ __forceinline__ int32_t WaveSums(int32_t x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
 struct BatchItem {
   int32_t request, start, seen, rows;  // rows: of the request and a key head
   int32_t r0;                          // the tile's first
@@ -34,21 +49,24 @@ struct BatchItem {
 // The requests' part of FindWork: shape of request r as this kernel sees it.
 template <int kTileRows, int kStep, bool kFew>
 struct BatchShape {
-  int32_t start, seen, rows, tiles, steps;  // steps: of one tile's range, at most
-  int64_t work;                             // of all tiles' ranges, half of tiles * steps at least
+  int32_t start = 0, seen = 0, rows = 0, tiles = 0, steps = 0;  // steps: of one tile's range, at most
+  int64_t work = 0;  // of all tiles' ranges, half of tiles * steps at least
+  __device__ __forceinline__ BatchShape() {}
   __device__ __forceinline__ BatchShape(const BatchAttendArgs& a, const BatchSplit& b, int32_t group, int32_t r) {
-    start = min(max(a.starts[r], 0), a.rows);
-    const int32_t n = min(max(a.starts[r + 1], start), a.rows) - start;
+    start = a.starts[r];
+    const int32_t stop = a.starts[r + 1];
     seen = a.paged ? min(max(a.seen[r], 0), a.width << a.page_shift) : 0;
+    start = min(max(start, 0), a.rows);
+    const int32_t n = min(max(stop, start), a.rows) - start;
     rows = n * group;
     if (kFew ? rows > b.few : rows <= b.few) rows = 0;
     tiles = (rows + kTileRows - 1) / kTileRows;
     const int32_t end = seen + n;
     steps = (end + kStep - 1) / kStep;
-    if (a.window < min(end, 1 << 30)) steps = min(steps, (a.window + (kTileRows + group - 2) / group + 2 * kStep - 2) / kStep);
+    if (a.window < min(end, 1 << 30)) steps = min(steps, (a.window + Quotient(kTileRows + group - 2, a.group) + 2 * kStep - 2) / kStep);
     if (rows == 0) steps = 0;
     // The first tile's range ends at its own rows, and without a window those between grow evenly.
-    const int32_t first = min(steps, (seen + min(n, (kTileRows + group - 1) / group) + kStep - 1) / kStep);
+    const int32_t first = min(steps, (seen + min(n, Quotient(kTileRows + group - 1, a.group)) + kStep - 1) / kStep);
     work = (static_cast<int64_t>(tiles) * (a.window < end ? 2 * steps : first + steps) + 1) / 2;
   }
 };
@@ -57,8 +75,8 @@ struct BatchShape {
 template <int kThreads>
 struct BatchScan {
   int64_t steps[kThreads / 64];
-  int32_t sums[kThreads / 64][3];
-  int32_t found[4];
+  int32_t sums[kThreads / 64][4];
+  int32_t found[8];
 };
 
 // The item-th item of a key head's work; false: there are fewer, or it is empty. Uniform over the workgroup. lead: of
@@ -77,48 +95,32 @@ __device__ __forceinline__ bool FindWork(const BatchAttendArgs& a, const BatchSp
   const int32_t group = a.heads / a.kv_heads;
   const bool first_group = lead && item == 0;
   int64_t all = 0;
-  int32_t own_tiles = 0, own_steps = 0;  // of the first kThreads requests, which are looked at once
-  for (int32_t r = tid; r < a.requests; r += kThreads) {
-    const Shape x(a, b, group, r);
-    all += x.work;
-    if (r == tid) {
-      own_tiles = x.tiles;
-      own_steps = x.steps;
-    }
-  }
+  Shape own;  // of the first kThreads requests, which are looked at once
+  if (tid < a.requests) own = Shape(a, b, group, tid);
   constexpr int32_t kMostSteps = 0x3fffffff;
   int32_t size = kMostSteps;
   if (b.ranges > 0) {  // uniform
+    all = own.work;
+    for (int32_t r = tid + kThreads; r < a.requests; r += kThreads) all += Shape(a, b, group, r).work;
     all = WaveButterfly(all, [](int64_t x, int64_t y) { return x + y; });
     if (lane == 0) shared.steps[wave] = all;
     __syncthreads();
     all = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) all += shared.steps[i];
-    size = static_cast<int32_t>(min(int64_t(kMostSteps), max(int64_t(b.min_steps), (all + b.ranges - 1) / b.ranges)));
+    int64_t least = static_cast<int64_t>(static_cast<double>(all) / b.ranges);  // all < 2^53: within 1
+    while (least * b.ranges < all) ++least;
+    size = static_cast<int32_t>(min(int64_t(kMostSteps), max(int64_t(b.min_steps), least)));
   }
   int32_t before[3] = {0, 0, 0};  // items, items of divided tiles, divided tiles
   bool here = false;
   for (int32_t r0 = 0; r0 < a.requests; r0 += kThreads) {
-    int32_t tiles = 0, steps = 0;
-    if (r0 == 0) {
-      tiles = own_tiles;
-      steps = own_steps;
-    } else if (r0 + tid < a.requests) {
-      const Shape x(a, b, group, r0 + tid);
-      tiles = x.tiles;
-      steps = x.steps;
-    }
-    const int32_t per = (steps + size - 1) / size;
-    const int32_t own[3] = {tiles * per, per > 1 ? tiles * per : 0, per > 1 ? tiles : 0};
-    int32_t sum[3] = {own[0], own[1], own[2]};
+    if (r0 > 0) own = r0 + tid < a.requests ? Shape(a, b, group, r0 + tid) : Shape();
+    const int32_t per = own.steps <= size ? min(own.steps, 1) : (own.steps + size - 1) / size;
+    const int32_t mine[3] = {own.tiles * per, per > 1 ? own.tiles * per : 0, per > 1 ? own.tiles : 0};
+    int32_t sum[3];
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1)
-#pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        const int32_t x = __shfl_up(sum[i], off);
-        if (lane >= off) sum[i] += x;
-      }
+    for (int i = 0; i < 3; ++i) sum[i] = WaveSums(mine[i]);
     if (lane == 63) {
 #pragma unroll
       for (int i = 0; i < 3; ++i) shared.sums[wave][i] = sum[i];
@@ -133,12 +135,12 @@ __device__ __forceinline__ bool FindWork(const BatchAttendArgs& a, const BatchSp
         if (v < wave) sum[i] += x;
         total[i] += x;
       }
-    const int32_t from = before[0] + sum[0] - own[0];
-    if (item >= from && item - from < own[0]) {
-      shared.found[0] = r0 + tid;
-      shared.found[1] = item - from;
-      shared.found[2] = before[1] + sum[1] - own[1];
-      shared.found[3] = before[2] + sum[2] - own[2];
+    const int32_t from = before[0] + sum[0] - mine[0];
+    if (item >= from && item - from < mine[0]) {
+      const int32_t found[8] = {r0 + tid, item - from, before[1] + sum[1] - mine[1], before[2] + sum[2] - mine[2],
+                                own.start, own.seen, own.rows, own.steps};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) shared.found[i] = found[i];
     }
 #pragma unroll
     for (int i = 0; i < 3; ++i) before[i] += total[i];
@@ -148,38 +150,37 @@ __device__ __forceinline__ bool FindWork(const BatchAttendArgs& a, const BatchSp
   }
   if (first_group && b.ranges > 0 && tid == 0) b.tiles[0] = before[2];
   if (!here) return false;
-  const int32_t r = __builtin_amdgcn_readfirstlane(shared.found[0]);
-  const int32_t local = __builtin_amdgcn_readfirstlane(shared.found[1]);
-  const Shape x(a, b, group, r);
-  const int32_t per = (x.steps + size - 1) / size;
-  const int32_t at = local / per;
-  const int32_t tile = x.tiles - 1 - at;  // the rows with the most keys first
   const auto uniform = [](int32_t x) { return __builtin_amdgcn_readfirstlane(x); };  // and in scalar registers
-  w->request = r;
-  w->start = uniform(x.start);
-  w->seen = uniform(x.seen);
-  w->rows = uniform(x.rows);
-  w->r0 = uniform(tile * kTileRows);
-  w->p_first = uniform(x.seen + w->r0 / group);
-  w->p_last = uniform(x.seen + (min(w->r0 + kTileRows, x.rows) - 1) / group);
-  w->low = uniform(a.window > w->p_first ? 0 : (w->p_first - a.window + 1) / kStep * kStep);
+  const int32_t local = uniform(shared.found[1]), first_part = uniform(shared.found[2]), first_tile = uniform(shared.found[3]);
+  const int32_t most = uniform(shared.found[7]);
+  w->request = uniform(shared.found[0]);
+  w->start = uniform(shared.found[4]);
+  w->seen = uniform(shared.found[5]);
+  w->rows = uniform(shared.found[6]);
+  const int32_t per = most <= size ? 1 : uniform((most + size - 1) / size);
+  const int32_t at = per == 1 ? local : uniform(local / per);
+  const int32_t tile = (w->rows + kTileRows - 1) / kTileRows - 1 - at;  // the rows with the most keys first
+  w->r0 = tile * kTileRows;
+  w->p_first = w->seen + Quotient(w->r0, a.group);
+  w->p_last = w->seen + Quotient(min(w->r0 + kTileRows, w->rows) - 1, a.group);
+  w->low = a.window > w->p_first ? 0 : (w->p_first - a.window + 1) / kStep * kStep;
   w->high = w->p_last + 1;
   const int32_t steps = (w->high - w->low + kStep - 1) / kStep;
-  w->splits = uniform(min((steps + size - 1) / size, per));
-  w->split = uniform(local - at * per);
+  w->split = local - at * per;
+  w->splits = per == 1 ? 1 : uniform(min((steps + size - 1) / size, per));
   if (w->split >= w->splits) return false;
-  const int32_t each = uniform((steps + w->splits - 1) / w->splits);
+  const int32_t each = w->splits == 1 ? steps : uniform((steps + w->splits - 1) / w->splits);
   w->begin = min(steps, w->split * each);
   w->end = min(steps, w->begin + each);
-  const int32_t first = uniform(shared.found[2] + at * per);
+  const int32_t first = first_part + at * per;
   w->partial = first + w->split;
   if (per > 1 && w->split == 0 && lead && tid == 0) {
-    int32_t* p = b.tiles + static_cast<int64_t>(kTileInts) * (1 + uniform(shared.found[3] + at));
+    int32_t* p = b.tiles + static_cast<int64_t>(kTileInts) * (1 + first_tile + at);
     p[0] = first;
     p[1] = w->splits;
     p[2] = w->start;
     p[3] = w->r0;
-    p[4] = min(kTileRows, x.rows - w->r0);
+    p[4] = min(kTileRows, w->rows - w->r0);
   }
   return true;
 }
@@ -188,7 +189,7 @@ __device__ __forceinline__ bool SeesKey(const BatchAttendArgs& a, int32_t p, int
 
 // Where row rl of the item's tile (rl < rows - r0) lies in the output, in rows of a head.
 __device__ __forceinline__ int64_t BatchOutRow(const BatchAttendArgs& a, int32_t start, int32_t r, int32_t group, int32_t kv) {
-  const int32_t s = r / group;
+  const int32_t s = Quotient(r, a.group);
   return static_cast<int64_t>(start + s) * a.heads + kv * group + (r - s * group);
 }
 
@@ -209,20 +210,25 @@ struct BatchPages {
   }
 };
 
-// kN floats of a query row from dim d on, 0 past the row.
+// kN floats of a query row from dim d on; past the row its last ones, for MaskQuery: no branch between the loads.
 template <int kN>
 __device__ __forceinline__ void LoadBatchQuery(const float* q, int32_t dim, int d, bool vec, float (&x)[kN]) {
   if (vec) {
 #pragma unroll
     for (int i = 0; i < kN / 4; ++i) {
-      const f4 y = d + 4 * i < dim ? *reinterpret_cast<const f4*>(q + d + 4 * i) : f4{0.f, 0.f, 0.f, 0.f};
+      const f4 y = *reinterpret_cast<const f4*>(q + min(d + 4 * i, dim - 4));
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[4 * i + e] = y[e];
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < kN; ++e) x[e] = d + e < dim ? q[d + e] : 0.f;
+    for (int e = 0; e < kN; ++e) x[e] = q[min(d + e, dim - 1)];
   }
+}
+template <int kN>
+__device__ __forceinline__ void MaskQuery(int32_t dim, int d, float (&x)[kN]) {
+#pragma unroll
+  for (int e = 0; e < kN; ++e) x[e] = d + e < dim ? x[e] : 0.f;
 }
 __device__ __forceinline__ bool BatchQueryVec(const BatchAttendArgs& a) {  // uniform
   return a.dim % 4 == 0 && a.q_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0;

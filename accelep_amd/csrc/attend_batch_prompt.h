@@ -69,17 +69,17 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int j = lane & 31;
   const int g = lane >> 5;
-  const int32_t kv = block % a.kv_heads;
+  const int32_t kv = block - Quotient(block, a.by_kv_heads) * a.kv_heads;
   const int32_t group = a.heads / a.kv_heads;
   BatchItem w;
-  if (!FindWork<kBatchThreads, kPromptTileRows, kKeys, false>(a, b, block / a.kv_heads, kv == 0, scan, &w)) return;
+  if (!FindWork<kBatchThreads, kPromptTileRows, kKeys, false>(a, b, Quotient(block, a.by_kv_heads), kv == 0, scan, &w)) return;
   const int32_t w0 = w.r0 + wave * kWaveRows;  // the wave's rows
   const int32_t row = min(w0 + j, w.rows - 1);
-  const int32_t s = row / group;
+  const int32_t s = Quotient(row, a.group);
   const int32_t head = kv * group + (row - s * group);
   const int32_t p_row = w0 + j < w.rows ? w.seen + s : -1;
-  const int32_t pw_first = w.seen + min(w0, w.rows - 1) / group;
-  const int32_t pw_last = w0 < w.rows ? w.seen + (min(w0 + kWaveRows, w.rows) - 1) / group : -1;
+  const int32_t pw_first = w.seen + Quotient(min(w0, w.rows - 1), a.group);
+  const int32_t pw_last = w0 < w.rows ? w.seen + Quotient(min(w0 + kWaveRows, w.rows) - 1, a.group) : -1;
   const bool full_rows = w0 + kWaveRows <= w.rows;
   const BatchPages pages(a, kPaged ? w.request : 0);
   const auto key_of = [&](int32_t step) { return w.low + step * kKeys; };
@@ -241,20 +241,23 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
     uint32_t top = 0;
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) LoadBatchQuery(q, a.dim, 16 * st + 8 * g, vec, x[st]);
+    if (a.dim < DP) {
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) MaskQuery(a.dim, 16 * st + 8 * g, x[st]);
+    }
 #pragma unroll
     for (int st = 0; st < kSteps; ++st)
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[st][e]) & 0x7fffffffu);
     top = max(top, XorLane<32>(top));
-    const bool bad = top >= 0x7f800000u;
-    const float scale = RowScale(top);
+    const float scale = top >= 0x7f800000u ? NAN : RowScale(top);  // no finite row: all of it NaN
     row_back = 1.f / scale;
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
       h2 hi[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        SplitF16Nearest(bad ? NAN : x[st][2 * e] * scale, bad ? NAN : x[st][2 * e + 1] * scale, hi[e], lo[e]);
+        SplitF16Nearest(x[st][2 * e] * scale, x[st][2 * e + 1] * scale, hi[e], lo[e]);
       qh[st] = Join(hi[0], hi[1], hi[2], hi[3]);
       ql[st] = Join(lo[0], lo[1], lo[2], lo[3]);
     }
@@ -449,9 +452,10 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
   // acc[t][r] is O^T[dim 32t + 8 (r / 4) + 4g + r % 4][row j].
   l = l + XorLane<32>(l);
   if (w0 + j >= w.rows) return;
+  // fp32: the sums hold 2^power times what they are, and where they may pass the largest float 2^-64 of that is left.
   const bool far = !kHalf && power < kFarPower;
   const int32_t down = kHalf ? 0 : far ? -power - kFarShift : -power;
-  const float up = far ? kFarUp : 1.f;
+  const float inverse = w.splits > 1 ? 1.f : __fdiv_rn(1.f, l);
   float* dst = a.out + (static_cast<int64_t>(w.start + s) * a.heads + head) * a.dim;
   bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
   if (w.splits > 1) {
@@ -470,10 +474,8 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
       const int d = 32 * t + 8 * r4 + 4 * g;
       f4 o;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        o[e] = kHalf ? acc[t][4 * r4 + e] : ldexpf(acc[t][4 * r4 + e], down);
-        if (w.splits == 1) o[e] = __fdiv_rn(o[e], l) * up;
-      }
+      for (int e = 0; e < 4; ++e) o[e] = (kHalf ? acc[t][4 * r4 + e] : ldexpf(acc[t][4 * r4 + e], down)) * inverse;
+      if (!kHalf && far && w.splits == 1) o *= kFarUp;
       if (vec) {
         if (d < a.dim) *reinterpret_cast<f4*>(dst + d) = o;
       } else {

@@ -89,12 +89,12 @@ __device__ __forceinline__ void StepF32Group(const BatchAttendArgs& a, const Bat
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j = lane & 15;
   const int g = lane >> 4;
-  const int32_t kv = block % a.kv_heads;
+  const int32_t kv = block - Quotient(block, a.by_kv_heads) * a.kv_heads;
   const int32_t group = a.heads / a.kv_heads;
   BatchItem w;
-  if (!FindWork<kBatchThreads, kStepTileRows, kKeys, true>(a, b, block / a.kv_heads, kv == 0, scan, &w)) return;
+  if (!FindWork<kBatchThreads, kStepTileRows, kKeys, true>(a, b, Quotient(block, a.by_kv_heads), kv == 0, scan, &w)) return;
   const int32_t row = min(w.r0 + j, w.rows - 1);
-  const int32_t s = row / group;
+  const int32_t s = Quotient(row, a.group);
   const int32_t p_row = w.r0 + j < w.rows ? w.seen + s : -1;  // a row past the last sees nothing
   const float* kbase = static_cast<const float*>(a.k) + static_cast<int64_t>(kv) * a.dim;
   const float* vbase = static_cast<const float*>(a.v) + static_cast<int64_t>(kv) * a.dim;
@@ -149,6 +149,11 @@ __device__ __forceinline__ void StepF32Group(const BatchAttendArgs& a, const Bat
     load_k(key_of(u), entry);
     load_v(key_of(u), entry);
   }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < kI; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[i][e] = 16 * i + 4 * g + e < a.dim ? q[i][e] : 0.f;
 
   float m = -INFINITY, l = 0.f;  // l: this lane's share of the row's sum
   float shift = 1.f, share = 0.f;  // the weighted sum's power of two, and the largest weight now of a large value
@@ -324,12 +329,12 @@ __device__ __forceinline__ void StepF16Group(const BatchAttendArgs& a, const Bat
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j = lane & 15;
   const int g = lane >> 4;
-  const int32_t kv = block % a.kv_heads;
+  const int32_t kv = block - Quotient(block, a.by_kv_heads) * a.kv_heads;
   const int32_t group = a.heads / a.kv_heads;
   BatchItem w;
-  if (!FindWork<kBatchThreads, kStepTileRows, kKeys, true>(a, b, block / a.kv_heads, kv == 0, scan, &w)) return;
+  if (!FindWork<kBatchThreads, kStepTileRows, kKeys, true>(a, b, Quotient(block, a.by_kv_heads), kv == 0, scan, &w)) return;
   const int32_t row = min(w.r0 + j, w.rows - 1);
-  const int32_t s = row / group;
+  const int32_t s = Quotient(row, a.group);
   const int32_t p_row = w.r0 + j < w.rows ? w.seen + s : -1;  // a row past the last sees nothing
   const _Float16* kbase = static_cast<const _Float16*>(a.k) + static_cast<int64_t>(kv) * a.dim;
   const _Float16* vbase = static_cast<const _Float16*>(a.v) + static_cast<int64_t>(kv) * a.dim;
@@ -389,18 +394,22 @@ __device__ __forceinline__ void StepF16Group(const BatchAttendArgs& a, const Bat
     load_k(key_of(u), entry);
     load_v(key_of(u), entry);
   }
+  __builtin_amdgcn_sched_barrier(0);
   h8 qh[kC][2], ql[kC][2];
   float factor;  // takes the row's scale out of its scores again
   {
     uint32_t top = 0;
+    if (a.dim < DP) {
+#pragma unroll
+      for (int i = 0; i < kC; ++i) MaskQuery(a.dim, 64 * i + 16 * g, x[i]);
+    }
 #pragma unroll
     for (int i = 0; i < kC; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
     top = max(top, XorLane<16>(top));
     top = max(top, XorLane<32>(top));
-    const bool bad = top >= 0x7f800000u;  // no finite row: all of it NaN
-    const float scale = RowScale(top);
+    const float scale = top >= 0x7f800000u ? NAN : RowScale(top);  // no finite row: all of it NaN
     factor = 1.f / scale * a.factor;
 #pragma unroll
     for (int i = 0; i < kC; ++i)
@@ -410,7 +419,7 @@ __device__ __forceinline__ void StepF16Group(const BatchAttendArgs& a, const Bat
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float y0 = x[i][8 * half + 2 * e] * scale, y1 = x[i][8 * half + 2 * e + 1] * scale;
-          SplitF16Nearest(bad ? NAN : y0, bad ? NAN : y1, hi[e], lo[e]);
+          SplitF16Nearest(y0, y1, hi[e], lo[e]);
         }
         qh[i][half] = Join(hi[0], hi[1], hi[2], hi[3]);
         ql[i][half] = Join(lo[0], lo[1], lo[2], lo[3]);

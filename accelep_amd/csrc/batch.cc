@@ -111,6 +111,8 @@ bool CheckAttend(const AccelHipBuffer& q, const AccelHipBatch* batch, const Acce
   a->window = window == 0 || window > kMaxRows ? kNoWindow : static_cast<int32_t>(window);
   a->longest = static_cast<int32_t>(batch->longest == 0 ? batch->rows : std::min(batch->longest, batch->rows));
   a->factor = AttendFactor(dim);
+  a->group = DivisorOf(std::max<int64_t>(heads / kv_heads, 1));
+  a->by_kv_heads = DivisorOf(kv_heads);
   return batch->requests > 0 && *out_bytes > 0;
 }
 

@@ -529,6 +529,18 @@ struct AppendPagedArgs {
   bool f16;
 };
 void LaunchAppendPaged(const AppendPagedArgs& a, hipStream_t stream);
+// A divisor d of numbers below 2^31: x / d is x * mul >> shift, with mul = ceil(2^shift / d) and 2^shift >= 2^31 d, so
+// that the excess of x * mul / 2^shift over x / d stays below 1 / d.
+struct QuickDivisor {
+  uint32_t mul = 1u << 31;
+  int32_t shift = 31;
+};
+inline QuickDivisor DivisorOf(int64_t d) {
+  QuickDivisor q;
+  while ((uint64_t(1) << (q.shift - 31)) < static_cast<uint64_t>(d)) ++q.shift;
+  q.mul = static_cast<uint32_t>(((uint64_t(1) << q.shift) + static_cast<uint64_t>(d) - 1) / static_cast<uint64_t>(d));
+  return q;
+}
 // Attention of a batch. paged: keys and values are pages of a cache, otherwise rows as the queries are.
 struct BatchAttendArgs {
   const float* q;  // rows of heads * dim, q_stride apart
@@ -540,6 +552,7 @@ struct BatchAttendArgs {
   int32_t heads, kv_heads, dim, window, longest;     // window: kNoWindow for none; longest: of the rows, at most
   float factor;  // log2(e) / sqrt(dim): scores in log2 units
   bool f16, paged;
+  QuickDivisor group, by_kv_heads;  // of heads / kv_heads, and of kv_heads
 };
 void LaunchAttendBatch(const BatchAttendArgs& a, hipStream_t stream);
 // rng_inout is a device word holding the xorshift32 state; index_dev offsets `chosen`.
