@@ -69,6 +69,11 @@ struct BatchShape {
     const int32_t first = min(steps, (seen + min(n, Quotient(kTileRows + group - 1, a.group)) + kStep - 1) / kStep);
     work = (static_cast<int64_t>(tiles) * (a.window < end ? 2 * steps : first + steps) + 1) / 2;
   }
+  // The first tiles, whose rows all end within `most` steps.
+  __device__ __forceinline__ int32_t ShortTiles(int32_t group, int32_t most) const {
+    const int64_t rows_below = max(int64_t(0), static_cast<int64_t>(most) * kStep - seen) * group;
+    return static_cast<int32_t>(min(rows_below / kTileRows, int64_t(tiles)));
+  }
 };
 
 // What a wave passes on to the others.
@@ -81,9 +86,11 @@ struct BatchScan {
 
 // The item-th item of a key head's work; false: there are fewer, or it is empty. Uniform over the workgroup. lead: of
 // the first key head, whose workgroups note the divided tiles.
-// Items: a request's tiles are cut into `per` = ceil(steps / size) ranges each, size >= all work / ranges. A request's
-// tiles * steps is at most twice its work, so all items are at most 2 * ranges + all tiles, and those of divided tiles,
-// whose steps / size is above 1, at most twice their steps / size: 4 * ranges. Divided tiles: 2 * ranges.
+// Items: a request's long tiles, those of more than size / 2 steps, are cut into `per` = ceil(steps / size) ranges each,
+// size >= all work / ranges; they come first, all requests' short tiles behind them, each one item, so that what is begun
+// last is short. A request's tiles * steps is at most twice its work, so all items are at most 2 * ranges + all tiles, and
+// those of divided tiles, whose steps / size is above 1, at most twice their steps / size: 4 * ranges. Divided tiles:
+// 2 * ranges.
 template <int kThreads, int kTileRows, int kStep, bool kFew>
 __device__ __forceinline__ bool FindWork(const BatchAttendArgs& a, const BatchSplit& b, int32_t item, bool lead,
                                          BatchScan<kThreads>& shared, BatchItem* w) {
@@ -112,54 +119,70 @@ __device__ __forceinline__ bool FindWork(const BatchAttendArgs& a, const BatchSp
     while (least * b.ranges < all) ++least;
     size = static_cast<int32_t>(min(int64_t(kMostSteps), max(int64_t(b.min_steps), least)));
   }
-  int32_t before[3] = {0, 0, 0};  // items, items of divided tiles, divided tiles
+  int32_t before = 0, parts_before = 0, divided_before = 0;  // items, items of divided tiles, divided tiles
   bool here = false;
-  for (int32_t r0 = 0; r0 < a.requests; r0 += kThreads) {
-    if (r0 > 0) own = r0 + tid < a.requests ? Shape(a, b, group, r0 + tid) : Shape();
-    const int32_t per = own.steps <= size ? min(own.steps, 1) : (own.steps + size - 1) / size;
-    const int32_t mine[3] = {own.tiles * per, per > 1 ? own.tiles * per : 0, per > 1 ? own.tiles : 0};
-    int32_t sum[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) sum[i] = WaveSums(mine[i]);
-    if (lane == 63) {
-#pragma unroll
-      for (int i = 0; i < 3; ++i) shared.sums[wave][i] = sum[i];
-    }
-    __syncthreads();
-    int32_t total[3] = {0, 0, 0};
-#pragma unroll
-    for (int v = 0; v < kWaves; ++v)
-#pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        const int32_t x = shared.sums[v][i];
-        if (v < wave) sum[i] += x;
-        total[i] += x;
+  // Long tiles, then short ones: in one look where the requests are few enough for one, otherwise in a second.
+  const bool at_once = a.requests <= kThreads;
+  for (int pass = 0; pass < 2 && !here; ++pass) {
+    for (int32_t r0 = 0; r0 < a.requests; r0 += kThreads) {
+      if (!at_once) own = r0 + tid < a.requests ? Shape(a, b, group, r0 + tid) : Shape();
+      const int32_t per = own.steps <= size ? 1 : (own.steps + size - 1) / size;
+      const int32_t short_tiles = kFew ? 0 : own.ShortTiles(group, size / 2);
+      const int32_t long_tiles = own.tiles - short_tiles;
+      const int32_t mine = pass == 0 ? long_tiles * per : 0, mine_short = at_once || pass == 1 ? short_tiles : 0;
+      const int32_t items = WaveSums(mine), parts = WaveSums(per > 1 ? mine : 0), divided = WaveSums(per > 1 ? long_tiles : 0);
+      const int32_t shorts = kFew ? 0 : WaveSums(mine_short);
+      if (lane == 63) {
+        shared.sums[wave][0] = items;
+        shared.sums[wave][1] = parts;
+        shared.sums[wave][2] = divided;
+        shared.sums[wave][3] = shorts;
       }
-    const int32_t from = before[0] + sum[0] - mine[0];
-    if (item >= from && item - from < mine[0]) {
-      const int32_t found[8] = {r0 + tid, item - from, before[1] + sum[1] - mine[1], before[2] + sum[2] - mine[2],
-                                own.start, own.seen, own.rows, own.steps};
+      __syncthreads();
+      int32_t from = before + items - mine, part = parts_before + parts, tile = divided_before + divided;
+      int32_t from_short = shorts - mine_short, short_sum = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) shared.found[i] = found[i];
+      for (int v = 0; v < kWaves; ++v) {
+        const int32_t x = shared.sums[v][0], y = shared.sums[v][1], z = shared.sums[v][2], t = shared.sums[v][3];
+        if (v < wave) {
+          from += x;
+          part += y;
+          tile += z;
+          from_short += t;
+        }
+        before += x;
+        parts_before += y;
+        divided_before += z;
+        short_sum += t;
+      }
+      from_short += before;  // behind all long ones
+      before += short_sum;
+      const bool in_long = item >= from && item - from < mine, in_short = item >= from_short && item - from_short < mine_short;
+      if (in_long || in_short) {
+        const int32_t found[8] = {r0 + tid, item - (in_long ? from : from_short), part - mine, tile - long_tiles, own.start,
+                                  own.seen, own.rows, in_long ? per : -short_tiles};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) shared.found[i] = found[i];
+      }
+      __syncthreads();
+      here = item < before;
+      if (here && !(first_group && pass == 0 && b.ranges > 0)) break;  // the first workgroup counts on
     }
-#pragma unroll
-    for (int i = 0; i < 3; ++i) before[i] += total[i];
-    __syncthreads();
-    here = item < before[0];
-    if (here && !(first_group && b.ranges > 0)) break;  // the first workgroup counts on
+    if (first_group && pass == 0 && b.ranges > 0 && tid == 0) b.tiles[0] = divided_before;
+    if (kFew || at_once) break;
   }
-  if (first_group && b.ranges > 0 && tid == 0) b.tiles[0] = before[2];
   if (!here) return false;
   const auto uniform = [](int32_t x) { return __builtin_amdgcn_readfirstlane(x); };  // and in scalar registers
   const int32_t local = uniform(shared.found[1]), first_part = uniform(shared.found[2]), first_tile = uniform(shared.found[3]);
-  const int32_t most = uniform(shared.found[7]);
+  const int32_t kind = uniform(shared.found[7]);  // long tiles: ranges of each; short ones: minus their count
   w->request = uniform(shared.found[0]);
   w->start = uniform(shared.found[4]);
   w->seen = uniform(shared.found[5]);
   w->rows = uniform(shared.found[6]);
-  const int32_t per = most <= size ? 1 : uniform((most + size - 1) / size);
+  const int32_t per = max(kind, 1);
   const int32_t at = per == 1 ? local : uniform(local / per);
-  const int32_t tile = (w->rows + kTileRows - 1) / kTileRows - 1 - at;  // the rows with the most keys first
+  const int32_t tiles = kind > 0 ? (w->rows + kTileRows - 1) / kTileRows : -kind;
+  const int32_t tile = tiles - 1 - at;  // the rows with the most keys first
   w->r0 = tile * kTileRows;
   w->p_first = w->seen + Quotient(w->r0, a.group);
   w->p_last = w->seen + Quotient(min(w->r0 + kTileRows, w->rows) - 1, a.group);

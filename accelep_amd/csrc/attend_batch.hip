@@ -200,11 +200,11 @@ void LaunchAttendBatch(const BatchAttendArgs& a, hipStream_t stream) {
   Share step{}, prompt{};
   if (steps) {
     const int64_t tiles = std::min<int64_t>(a.requests, a.rows) + (steps_only ? all_rows / kStepTileRows : 0);
-    step = ShareOf(a, kStepTileRows, StepKeys(a.f16), tiles, 4 * cus, 8);
+    step = ShareOf(a, kStepTileRows, StepKeys(a.f16), tiles, 3 * cus, 8);
   }
   if (!steps_only) {
     const int64_t tiles = all_rows / kPromptTileRows + std::min<int64_t>(a.requests, all_rows / (few + 1));
-    prompt = ShareOf(a, kPromptTileRows, PromptKeys(a.f16), tiles, 2 * cus, 4);
+    prompt = ShareOf(a, kPromptTileRows, PromptKeys(a.f16), tiles, cus, 4);
   }
   // Where there is no memory for the parts the ranges stay whole.
   std::unique_lock<std::mutex> held;
