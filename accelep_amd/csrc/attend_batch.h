@@ -216,6 +216,32 @@ __device__ __forceinline__ int64_t BatchOutRow(const BatchAttendArgs& a, int32_t
   return static_cast<int64_t>(start + s) * a.heads + kv * group + (r - s * group);
 }
 
+// x * s = hi + lo for two values, both parts rounded to nearest: 22 bits where lo is a normal number, and within 2^-25
+// where it is not. Four instructions: fp32 in, products and differences exact, each half of a pair on its own.
+__device__ __forceinline__ void SplitScaled(float x, float y, float s, h2& hi, h2& lo) {
+  uint32_t h, l;
+  asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(h) : "v"(x), "v"(s));
+  asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(h) : "v"(y), "v"(s));
+  asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(l) : "v"(x), "v"(s), "v"(h));
+  asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(l) : "v"(y), "v"(s), "v"(h));
+  hi = __builtin_bit_cast(h2, h);
+  lo = __builtin_bit_cast(h2, l);
+}
+// x = hi + lo for two weights, hi cut towards zero and lo to nearest: three instructions.
+__device__ __forceinline__ void SplitWeights(float x, float y, h2& hi, h2& lo) {
+  hi = PackRtz(x, y);
+  const uint32_t h = __builtin_bit_cast(uint32_t, hi);
+  uint32_t l;
+  asm("v_fma_mixlo_f16 %0, %1, 1.0, -%2 op_sel_hi:[0,0,1]" : "=v"(l) : "v"(x), "v"(h));
+  asm("v_fma_mixhi_f16 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(l) : "v"(y), "v"(h));
+  lo = __builtin_bit_cast(h2, l);
+}
+// The larger of |x| and what was largest so far, half by half; a NaN stays one.
+__device__ __forceinline__ h2 LargestHalves(h2 x, h2 so_far) {
+  asm("v_pk_maximum3_f16 %0, %1, %1, %0 neg_lo:[0,1,0] neg_hi:[0,1,0]" : "+v"(so_far) : "v"(x));
+  return so_far;
+}
+
 // The page of the 16 tokens from t on, and whether there is one.
 struct BatchPages {
   const int32_t* entries;

@@ -11,8 +11,8 @@
 //  * O^T += V^T P^T: those scores are the lane's own k-slots of P^T if slot e of 16 keys is key
 //    (e % 4) + 8 (e / 4) + 4g, and the value operand is read transposed from the row-major tile
 //    (ds_read_b64_tr_b16 gives a lane four keys of one dim).
-// An fp32 row enters as its parts times a power of two: 2^9 for rows whose largest magnitude lies in [2^-6, 2^6)
-// (or that are zero), which keeps 22 bits of all of them, otherwise one from the row's own largest magnitude, whose
+// An fp32 row enters as its parts times a power of two: 2^9 for rows whose largest magnitude lies in [2^-6, 2^6),
+// which keeps 22 bits of all of them, otherwise one from the row's own largest magnitude, whose
 // inverse meets its scores or weights. A row that is not finite, or has no page, has NaN there and zeros for values.
 #pragma once
 
@@ -26,7 +26,7 @@ static_assert(kPromptTileRows == kPromptWaves * kWaveRows, "a wave has 32 rows")
 constexpr float kCommonScale = 0x1p9f;
 constexpr int32_t kCommonPower = 9;
 constexpr float kBackFirst = 0x1p60f;
-constexpr uint32_t kCommonLow = 121u << 23, kCommonHigh = 133u << 23;  // bits of 2^-6 and 2^6
+constexpr uint32_t kCommonLow = 0x4800, kCommonHigh = 0x7800;  // f16's bits of 2^-6 and 2^6 times that
 constexpr int32_t kUnits = 14;  // weights of up to 2^14 meet values' scales times 2^-14
 typedef short s4 __attribute__((ext_vector_type(4)));
 
@@ -139,48 +139,47 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
     }
   };
   // fp32: writes a thread's pieces of one plane; tile row `key` begins at dst + key * stride, its second part
-  // `part` halves later.
-  const auto put_plane = [&](uint4 (&x)[kChunks], _Float16* dst, int stride, int part, float& row_back, int slot) {
-    // The row's largest magnitude: of the bits as signed numbers for its positive values, as unsigned
-    // ones for its negative.
-    int32_t pos = 0;
-    uint32_t neg = 0;
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      pos = max(max(pos, max(static_cast<int32_t>(x[i].x), static_cast<int32_t>(x[i].y))),
-                max(static_cast<int32_t>(x[i].z), static_cast<int32_t>(x[i].w)));
-      neg = max(max(neg, max(x[i].x, x[i].y)), max(x[i].z, x[i].w));
-    }
-    uint32_t top = max(static_cast<uint32_t>(pos), neg & 0x7fffffffu);
-    top = max(top, XorLane<1>(top));
-    top = max(top, XorLane<2>(top));
-    top = max(top, XorLane<4>(top));
-    if (kPaged && !pages.Is(entry[0])) top = 0x7f800000u;  // uniform
-    float scale = kCommonScale, back = 1.f / kCommonScale;
-    const bool common = top == 0 || (top >= kCommonLow && top < kCommonHigh);
-    if (!__all(common)) {
-      odd[slot] = 1;
-      scale = RowScale(top);
-      back = 1.f / scale;
-      if (top >= 0x7f800000u) {
-        back = NAN;
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i) x[i] = make_uint4(0, 0, 0, 0);
-      }
-    }
-    row_back = back;
+  // `part` halves later. All rows are written at the common scale, and again where a row of the wave's is not common.
+  const auto put_plane = [&](const uint4 (&x)[kChunks], _Float16* dst, int stride, int part, float& row_back, int slot) {
     h8* p = reinterpret_cast<h8*>(dst + (tid / 8) * stride + 8 * (tid % 8));
+    const auto write = [&](float scale, bool zero) {
+      h2 most = h2{0, 0};
 #pragma unroll
-    for (int i = 0; i < kChunks; i += 2) {
-      const uint4 a0 = x[i], a1 = x[i + 1];
-      h2 hi[4], lo[4];
-      SplitF16(__uint_as_float(a0.x) * scale, __uint_as_float(a0.y) * scale, hi[0], lo[0]);
-      SplitF16(__uint_as_float(a0.z) * scale, __uint_as_float(a0.w) * scale, hi[1], lo[1]);
-      SplitF16(__uint_as_float(a1.x) * scale, __uint_as_float(a1.y) * scale, hi[2], lo[2]);
-      SplitF16(__uint_as_float(a1.z) * scale, __uint_as_float(a1.w) * scale, hi[3], lo[3]);
-      if (DP < kStaged && 8 * (tid % 8 + 4 * i) >= DP) break;
-      p[4 * i] = Join(hi[0], hi[1], hi[2], hi[3]);
-      p[4 * i + part / 8] = Join(lo[0], lo[1], lo[2], lo[3]);
+      for (int i = 0; i < kChunks; i += 2) {
+        const uint32_t v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, x[i + 1].x, x[i + 1].y, x[i + 1].z, x[i + 1].w};
+        h2 hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          SplitScaled(zero ? 0.f : __uint_as_float(v[2 * e]), zero ? 0.f : __uint_as_float(v[2 * e + 1]), scale, hi[e], lo[e]);
+          most = LargestHalves(hi[e], most);
+        }
+        if (DP < kStaged && 8 * (tid % 8 + 4 * i) >= DP) break;
+        p[4 * i] = Join(hi[0], hi[1], hi[2], hi[3]);
+        p[4 * i + part / 8] = Join(lo[0], lo[1], lo[2], lo[3]);
+      }
+      return __builtin_bit_cast(uint32_t, most);
+    };
+    uint32_t most = write(kCommonScale, false);
+    most = max(most & 0xffffu, most >> 16);
+    most = max(most, XorLane<1>(most));
+    most = max(most, XorLane<2>(most));
+    most = max(most, XorLane<4>(most));
+    row_back = 1.f / kCommonScale;
+    const bool common = most - kCommonLow < kCommonHigh - kCommonLow && (!kPaged || pages.Is(entry[0]));
+    if (!__all(common)) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i)
+        top = max(max(top, max(x[i].x & 0x7fffffffu, x[i].y & 0x7fffffffu)), max(x[i].z & 0x7fffffffu, x[i].w & 0x7fffffffu));
+      top = max(top, XorLane<1>(top));
+      top = max(top, XorLane<2>(top));
+      top = max(top, XorLane<4>(top));
+      if (kPaged && !pages.Is(entry[0])) top = 0x7f800000u;  // uniform
+      const bool finite = top < 0x7f800000u;
+      const float scale = RowScale(finite ? top : 0);
+      odd[slot] = 1;
+      row_back = finite ? 1.f / scale : NAN;
+      write(scale, !finite);
     }
   };
   const auto put = [&](int buf, int slot) {
@@ -418,7 +417,7 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
         for (int k16 = 0; k16 < 2; ++k16) {
           h2 hi[4], lo[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) SplitF16(st[h][8 * k16 + 2 * e], st[h][8 * k16 + 2 * e + 1], hi[e], lo[e]);
+          for (int e = 0; e < 4; ++e) SplitWeights(st[h][8 * k16 + 2 * e], st[h][8 * k16 + 2 * e + 1], hi[e], lo[e]);
           const h8 ph = Join(hi[0], hi[1], hi[2], hi[3]), pl = Join(lo[0], lo[1], lo[2], lo[3]);
           const auto read = [&](int t, int part) {
             const _Float16* p = vrow + part * kKeys * kVStride + (32 * h + 16 * k16) * kVStride + 32 * t;

@@ -526,7 +526,7 @@ __device__ __forceinline__ void StepF16Group(const BatchAttendArgs& a, const Bat
     }
     h2 ph[4], pl[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) SplitF16(p[2 * e], p[2 * e + 1], ph[e], pl[e]);
+    for (int e = 0; e < 4; ++e) SplitWeights(p[2 * e], p[2 * e + 1], ph[e], pl[e]);
     const h8 p_hi = Join(ph[0], ph[1], ph[2], ph[3]), p_lo = Join(pl[0], pl[1], pl[2], pl[3]);
 #pragma unroll
     for (int i = 0; i < kVWords; ++i) {
