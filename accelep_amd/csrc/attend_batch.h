@@ -51,10 +51,12 @@ template <int kTileRows, int kStep, bool kFew>
 struct BatchShape {
   int32_t start = 0, seen = 0, rows = 0, tiles = 0, steps = 0;  // steps: of one tile's range, at most
   int64_t work = 0;  // of all tiles' ranges, half of tiles * steps at least
+  bool descends = false;  // the next request begins before this one
   __device__ __forceinline__ BatchShape() {}
   __device__ __forceinline__ BatchShape(const BatchAttendArgs& a, const BatchSplit& b, int32_t group, int32_t r) {
     start = a.starts[r];
     const int32_t stop = a.starts[r + 1];
+    descends = stop < start;
     seen = a.paged ? min(max(a.seen[r], 0), a.width << a.page_shift) : 0;
     start = min(max(start, 0), a.rows);
     const int32_t n = min(max(stop, start), a.rows) - start;
@@ -71,7 +73,7 @@ struct BatchShape {
   }
   // The first tiles, whose rows all end within `most` steps.
   __device__ __forceinline__ int32_t ShortTiles(int32_t group, int32_t most) const {
-    const int64_t rows_below = max(int64_t(0), static_cast<int64_t>(most) * kStep - seen) * group;
+    const int64_t rows_below = min(max(int64_t(0), static_cast<int64_t>(most) * kStep - seen), int64_t(rows)) * group;
     return static_cast<int32_t>(min(rows_below / kTileRows, int64_t(tiles)));
   }
 };
@@ -90,7 +92,7 @@ struct BatchScan {
 // size >= all work / ranges; they come first, all requests' short tiles behind them, each one item, so that what is begun
 // last is short. A request's tiles * steps is at most twice its work, so all items are at most 2 * ranges + all tiles, and
 // those of divided tiles, whose steps / size is above 1, at most twice their steps / size: 4 * ranges. Divided tiles:
-// 2 * ranges.
+// 2 * ranges. That holds while no row is of two requests, so starts that descend leave no item.
 template <int kThreads, int kTileRows, int kStep, bool kFew>
 __device__ __forceinline__ bool FindWork(const BatchAttendArgs& a, const BatchSplit& b, int32_t item, bool lead,
                                          BatchScan<kThreads>& shared, BatchItem* w) {
@@ -108,13 +110,28 @@ __device__ __forceinline__ bool FindWork(const BatchAttendArgs& a, const BatchSp
   int32_t size = kMostSteps;
   if (b.ranges > 0) {  // uniform
     all = own.work;
-    for (int32_t r = tid + kThreads; r < a.requests; r += kThreads) all += Shape(a, b, group, r).work;
+    bool descends = own.descends;
+    for (int32_t r = tid + kThreads; r < a.requests; r += kThreads) {
+      const Shape x(a, b, group, r);
+      all += x.work;
+      descends = descends || x.descends;
+    }
     all = WaveButterfly(all, [](int64_t x, int64_t y) { return x + y; });
-    if (lane == 0) shared.steps[wave] = all;
+    descends = __any(descends);
+    if (lane == 0) shared.steps[wave] = descends ? -1 : all;
     __syncthreads();
     all = 0;
+    descends = false;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) all += shared.steps[i];
+    for (int i = 0; i < kWaves; ++i) {
+      const int64_t x = shared.steps[i];
+      descends = descends || x < 0;
+      all += x;
+    }
+    if (descends) {  // uniform
+      if (first_group && tid == 0) b.tiles[0] = 0;
+      return false;
+    }
     int64_t least = static_cast<int64_t>(static_cast<double>(all) / b.ranges);  // all < 2^53: within 1
     while (least * b.ranges < all) ++least;
     size = static_cast<int32_t>(min(int64_t(kMostSteps), max(int64_t(b.min_steps), least)));

@@ -141,8 +141,8 @@ Share ShareOf(const BatchAttendArgs& a, int32_t tile_rows, int32_t keys, int64_t
   const int64_t most_keys = std::min<int64_t>(a.paged ? (int64_t(a.width) << a.page_shift) + a.rows : a.rows,
                                               int64_t(a.window) + tile_rows + 2 * keys);
   const int64_t most_steps = (most_keys + keys - 1) / keys;
-  if (most_steps <= min_steps) return s;
-  s.ranges = std::max<int64_t>(1, groups / a.kv_heads);
+  if (most_steps <= min_steps || groups < 2 * a.kv_heads) return s;  // one range would be all there is
+  s.ranges = groups / a.kv_heads;
   s.items = std::min<int64_t>(4 * s.ranges, tiles * ((most_steps + min_steps - 1) / min_steps));
   s.divided = std::min<int64_t>(2 * s.ranges, tiles);
   const size_t parts = static_cast<size_t>(s.items) * a.kv_heads * tile_rows;

@@ -329,8 +329,9 @@ typedef struct AccelHipCachePaged {
 } AccelHipCachePaged;
 /* One step of a batch. The new tokens of all requests are rows that lie one behind the other: those of
  * request r are starts[r] .. starts[r + 1] - 1, its first token is its token seen[r]. table[r] are the pages
- * of its tokens in order. rows is what there is room for; rows past starts[requests] are padding. longest is
- * the most new rows of one request where the host knows it, otherwise 0: it chooses kernels, not results. */
+ * of its tokens in order. rows is what there is room for; rows past starts[requests] are padding. Where starts
+ * descend, the output's rows (no others) hold anything. longest is the most new rows of one request where the
+ * host knows it, otherwise 0: it chooses kernels, not results. */
 typedef struct AccelHipBatch {
   AccelHipBuffer seen;   /* int32 [requests] */
   AccelHipBuffer starts; /* int32 [requests + 1] */
@@ -350,7 +351,8 @@ typedef struct AccelHipPagePool {
  * `lengths` and the pool's state themselves. A request whose new pages are not all there, nor those of the requests
  * before it, or do not fit its table row, takes none: its rows have slot -1, its missing entries become -1,
  * its length stays, and it is counted in state_after[1]. Who needs no new page is always served. Other
- * outputs may overlap neither one another nor the inputs. */
+ * outputs may overlap neither one another nor the inputs. More than 2048 requests or 4096 rows take a workspace,
+ * which a call before a capture has to have grown. */
 ACCEL_HIP_API int accel_hip_batch_tables(AccelHipBuffer counts, AccelHipBuffer lengths, const AccelHipPagePool* pool,
                                          const AccelHipBatch* batch, AccelHipBuffer slots, AccelHipBuffer positions,
                                          AccelHipBuffer lengths_after, AccelHipBuffer state_after);
