@@ -27,6 +27,8 @@ constexpr float kCommonScale = 0x1p9f;
 constexpr int32_t kCommonPower = 9;
 constexpr float kBackFirst = 0x1p60f;
 constexpr uint32_t kCommonLow = 0x4800, kCommonHigh = 0x7800;  // f16's bits of 2^-6 and 2^6 times that
+// What a barrier of the scheduler's lets pass: vector and scalar arithmetic, LDS; no product and no load.
+constexpr int kNotLoads = 0x2 | 0x4 | 0x80;
 constexpr int32_t kUnits = 14;  // weights of up to 2^14 meet values' scales times 2^-14
 typedef short s4 __attribute__((ext_vector_type(4)));
 
@@ -54,7 +56,7 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
   constexpr int kSub = kKeys / 32;
   constexpr int kSteps = DP / 16;
   constexpr int kDims = DP / 32;
-  constexpr int kStaged = DP == 96 ? 128 : DP;  // dims that the threads of a key row are dealt
+  constexpr int kStaged = DP == 96 && kHalf ? 128 : DP;  // dims that the threads of a key row are dealt
   constexpr int kRowLanes = kHalf ? kStaged / 8 : 8;  // threads that stage a key row, neighbours
   constexpr int kStagedRows = kBatchThreads / kRowLanes;  // rows staged at once
   constexpr int kChunks = kHalf ? kKeys / kStagedRows : kStaged / 32;  // 16-byte pieces of a plane a thread stages
@@ -83,6 +85,13 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
   const bool full_rows = w0 + kWaveRows <= w.rows;
   const BatchPages pages(a, kPaged ? w.request : 0);
   const auto key_of = [&](int32_t step) { return w.low + step * kKeys; };
+  // Where a tile's row holds which dims: 4 from a place that is a multiple of 4 on. Eight threads load 128 bytes of an
+  // fp32 row at a time, and each writes what it has of two such loads as 16 bytes: places 8l .. 8l + 7 of 64 are dims
+  // 4l .. 4l + 3 and 32 + 4l .. Of 96, the last 32 are in order.
+  const auto dim_of = [](int place) {
+    if (kHalf || (DP == 96 && place >= 64)) return place;
+    return (place & ~63) + (place >> 2 & 1) * 32 + (place >> 3 & 7) * 4;
+  };
 
   // ---- staging: a thread's pieces of the next tile, from memory to registers and on to LDS ----
   uint4 kreg[kChunks], vreg[kChunks];
@@ -94,68 +103,81 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
         entry_next[i] = pages.Entry(t0 + (wave * 64 / kRowLanes + i * kStagedRows) / 16 * 16);
     }
   };
-  const auto fetch = [&](int32_t t0) {
+  // The tile at t0: its pages, then its pieces, one by one.
+  const float* fetched[2];
+  int32_t t_fetch = 0;
+  const auto fetch_at = [&](int32_t t0) {
     if constexpr (kPaged) {
 #pragma unroll
       for (int i = 0; i < kPages; ++i) entry[i] = __builtin_amdgcn_readfirstlane(entry_next[i]);
     }
-    if constexpr (kHalf) {
-      const int d = 8 * (tid % kRowLanes);
-#pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int64_t at = (pages.Slot(entry[i], t0 + tid / kRowLanes + i * kStagedRows)) * a.kv_stride + static_cast<int64_t>(kv) * a.dim;
-        const auto piece = [&](const void* plane) {
-          const _Float16* p = static_cast<const _Float16*>(plane) + at;
-          if (kLoad == 16) return *reinterpret_cast<const uint4*>(p + min(d, a.dim - 8));
-          const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-          const auto two = [&](int e) {
-            return h[min(d + e, a.dim - 1)] | static_cast<uint32_t>(h[min(d + e + 1, a.dim - 1)]) << 16;
-          };
-          return make_uint4(two(0), two(2), two(4), two(6));
-        };
-        kreg[i] = piece(a.k);
-        vreg[i] = piece(a.v);
-      }
-    } else {
+    t_fetch = t0;
+    if constexpr (!kHalf) {
       // A row past a prompt's last reads its last one, a piece past a head's dims its last: both are not used.
       const int32_t t = t0 + tid / kRowLanes;
       const int64_t row_at = kPaged ? pages.Slot(entry[0], t) : static_cast<int64_t>(w.start) + min(t, w.high - 1);
       const int64_t at = row_at * a.kv_stride + static_cast<int64_t>(kv) * a.dim;
-      const auto plane = [&](const void* base, uint4 (&x)[kChunks]) {
-        const float* p = static_cast<const float*>(base) + at;
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-          const int d = 8 * (tid % 8 + 8 * (i / 2)) + 4 * (i % 2);
-          if (kLoad == 16) {
-            x[i] = *reinterpret_cast<const uint4*>(p + min(d, a.dim - 4));
-          } else {
-            const auto one = [&](int e) { return __float_as_uint(p[min(d + e, a.dim - 1)]); };
-            x[i] = make_uint4(one(0), one(1), one(2), one(3));
-          }
-        }
-      };
-      plane(a.k, kreg);
-      plane(a.v, vreg);
+      fetched[0] = static_cast<const float*>(a.k) + at;
+      fetched[1] = static_cast<const float*>(a.v) + at;
     }
+  };
+  const auto fetch_piece = [&](int i) {
+    if constexpr (kHalf) {
+      const int d = 8 * (tid % kRowLanes);
+      const int64_t at = pages.Slot(entry[i], t_fetch + tid / kRowLanes + i * kStagedRows) * a.kv_stride + static_cast<int64_t>(kv) * a.dim;
+      const auto piece = [&](const void* plane) {
+        const _Float16* p = static_cast<const _Float16*>(plane) + at;
+        if (kLoad == 16) return *reinterpret_cast<const uint4*>(p + min(d, a.dim - 8));
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+        const auto two = [&](int e) {
+          return h[min(d + e, a.dim - 1)] | static_cast<uint32_t>(h[min(d + e + 1, a.dim - 1)]) << 16;
+        };
+        return make_uint4(two(0), two(2), two(4), two(6));
+      };
+      kreg[i] = piece(a.k);
+      vreg[i] = piece(a.v);
+    } else {
+      const int d = 32 * i + 4 * (tid % 8);
+      const auto piece = [&](const float* p) {
+        if (kLoad == 16) return *reinterpret_cast<const uint4*>(p + min(d, a.dim - 4));
+        const auto one = [&](int e) { return __float_as_uint(p[min(d + e, a.dim - 1)]); };
+        return make_uint4(one(0), one(1), one(2), one(3));
+      };
+      kreg[i] = piece(fetched[0]);
+      vreg[i] = piece(fetched[1]);
+    }
+  };
+  const auto fetch = [&]() {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) fetch_piece(i);
   };
   // fp32: writes a thread's pieces of one plane; tile row `key` begins at dst + key * stride, its second part
   // `part` halves later. All rows are written at the common scale, and again where a row of the wave's is not common.
   const auto put_plane = [&](const uint4 (&x)[kChunks], _Float16* dst, int stride, int part, float& row_back, int slot) {
-    h8* p = reinterpret_cast<h8*>(dst + (tid / 8) * stride + 8 * (tid % 8));
+    _Float16* p = dst + (tid / 8) * stride;
     const auto write = [&](float scale, bool zero) {
       h2 most = h2{0, 0};
 #pragma unroll
       for (int i = 0; i < kChunks; i += 2) {
-        const uint32_t v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, x[i + 1].x, x[i + 1].y, x[i + 1].z, x[i + 1].w};
         h2 hi[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          SplitScaled(zero ? 0.f : __uint_as_float(v[2 * e]), zero ? 0.f : __uint_as_float(v[2 * e + 1]), scale, hi[e], lo[e]);
-          most = LargestHalves(hi[e], most);
+        for (int n = 0; n < 2; ++n) {
+          if (i + n == kChunks) break;
+          const uint32_t v[4] = {x[i + n].x, x[i + n].y, x[i + n].z, x[i + n].w};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            SplitScaled(zero ? 0.f : __uint_as_float(v[2 * e]), zero ? 0.f : __uint_as_float(v[2 * e + 1]), scale, hi[2 * n + e],
+                        lo[2 * n + e]);
+            most = LargestHalves(hi[2 * n + e], most);
+          }
         }
-        if (DP < kStaged && 8 * (tid % 8 + 4 * i) >= DP) break;
-        p[4 * i] = Join(hi[0], hi[1], hi[2], hi[3]);
-        p[4 * i + part / 8] = Join(lo[0], lo[1], lo[2], lo[3]);
+        if (i + 1 < kChunks) {
+          *reinterpret_cast<h8*>(p + 32 * i + 8 * (tid % 8)) = Join(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<h8*>(p + 32 * i + 8 * (tid % 8) + part) = Join(lo[0], lo[1], lo[2], lo[3]);
+        } else {
+          *reinterpret_cast<h4*>(p + 32 * i + 4 * (tid % 8)) = __builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3);
+          *reinterpret_cast<h4*>(p + 32 * i + 4 * (tid % 8) + part) = __builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3);
+        }
       }
       return __builtin_bit_cast(uint32_t, most);
     };
@@ -226,8 +248,9 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
   };
   if (w.begin < w.end) {
     find_pages(key_of(w.begin));
-    fetch(key_of(w.begin));
-    if (w.begin + 1 < w.end) find_pages(key_of(w.begin + 1));
+    fetch_at(key_of(w.begin));
+    fetch();
+    find_pages(key_of(min(w.begin + 1, w.end - 1)));
   }
 
   // ---- the rows' queries ----
@@ -236,18 +259,22 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
   {
     const float* q = a.q + (w.start + s) * a.q_stride + static_cast<int64_t>(head) * a.dim;
     const bool vec = BatchQueryVec(a);
-    float x[kSteps][8];
+    float x[kSteps][2][4];
     uint32_t top = 0;
 #pragma unroll
-    for (int st = 0; st < kSteps; ++st) LoadBatchQuery(q, a.dim, 16 * st + 8 * g, vec, x[st]);
+    for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) LoadBatchQuery(q, a.dim, dim_of(16 * st + 8 * g + 4 * n), vec, x[st][n]);
     if (a.dim < DP) {
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st) MaskQuery(a.dim, 16 * st + 8 * g, x[st]);
+      for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) MaskQuery(a.dim, dim_of(16 * st + 8 * g + 4 * n), x[st][n]);
     }
 #pragma unroll
     for (int st = 0; st < kSteps; ++st)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[st][e]) & 0x7fffffffu);
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[st][e >> 2][e & 3]) & 0x7fffffffu);
     top = max(top, XorLane<32>(top));
     const float scale = top >= 0x7f800000u ? NAN : RowScale(top);  // no finite row: all of it NaN
     row_back = 1.f / scale;
@@ -256,13 +283,14 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
       h2 hi[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        SplitF16Nearest(x[st][2 * e] * scale, x[st][2 * e + 1] * scale, hi[e], lo[e]);
+        SplitF16Nearest(x[st][e >> 1][2 * (e & 1)] * scale, x[st][e >> 1][2 * (e & 1) + 1] * scale, hi[e], lo[e]);
       qh[st] = Join(hi[0], hi[1], hi[2], hi[3]);
       ql[st] = Join(lo[0], lo[1], lo[2], lo[3]);
     }
   }
 
-  float m = -INFINITY, l = 0.f, top = 0.f;
+  float m = -INFINITY, base = 0.f, l = 0.f, hi = -INFINITY, top = 0.f;  // base: m, or 0 where there is none
+  bool far = false, mixed = false;  // one of the wave's rows has far scores; a tile was not of common scale
   int32_t power = kCommonPower;  // fp32: the sums hold weight * value * 2^power
   f16v acc[kDims];
 #pragma unroll
@@ -278,38 +306,43 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
     const int32_t t0 = key_of(u);
     __syncthreads();
     if (tid == 0) odd[(u + 2 - w.begin) % 3] = 0;  // next written behind the next barrier
-    if (u + 1 < w.end) {
-      fetch(key_of(u + 1));
-      if (u + 2 < w.end) find_pages(key_of(u + 2));
-    }
-    __builtin_amdgcn_sched_barrier(0);
+    // Behind the last tile it is fetched again, so that nothing here branches.
+    fetch_at(key_of(min(u + 1, w.end - 1)));
+    find_pages(key_of(min(u + 2, w.end - 1)));
     const int32_t last = t0 + kKeys - 1;
     const bool none = t0 > pw_last || last <= pw_first - a.window;
-    if (!none) {  // uniform over the wave
-      const bool whole = full_rows && last <= pw_first && t0 > pw_last - a.window;
-      f16v st[kSub];
+    const bool whole = full_rows && last <= pw_first && t0 > pw_last - a.window;
+    // A wave whose rows see none of the tile makes these products too: its loads go out among them.
+    f16v st[kSub];
 #pragma unroll
-      for (int h = 0; h < kSub; ++h)
+    for (int h = 0; h < kSub; ++h)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) st[h][r] = 0.f;
-      __builtin_amdgcn_s_setprio(1);
+      for (int r = 0; r < 16; ++r) st[h][r] = 0.f;
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int step = 0; step < kSteps; ++step) {
-        // Neighbouring instructions add to different sums.
-        h8 k8[kSub];
+    for (int step = 0; step < kSteps; ++step) {
+      // Neighbouring instructions add to different sums.
+      h8 k8[kSub];
 #pragma unroll
-        for (int h = 0; h < kSub; ++h) {
-          k8[h] = *reinterpret_cast<const h8*>(&kt[buf][0][32 * h + j][16 * step + 8 * g]);
-          st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[h], qh[step], st[h], 0, 0, 0);
-        }
-#pragma unroll
-        for (int h = 0; h < kSub; ++h) st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[h], ql[step], st[h], 0, 0, 0);
-        if constexpr (!kHalf) {
-          const h8 k8l = *reinterpret_cast<const h8*>(&kt[buf][kParts - 1][j][16 * step + 8 * g]);
-          st[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8l, qh[step], st[0], 0, 0, 0);
-        }
+      for (int h = 0; h < kSub; ++h) {
+        k8[h] = *reinterpret_cast<const h8*>(&kt[buf][0][32 * h + j][16 * step + 8 * g]);
+        st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[h], qh[step], st[h], 0, 0, 0);
       }
-      __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+      for (int h = 0; h < kSub; ++h) st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[h], ql[step], st[h], 0, 0, 0);
+      if constexpr (!kHalf) {
+        const h8 k8l = *reinterpret_cast<const h8*>(&kt[buf][kParts - 1][j][16 * step + 8 * g]);
+        st[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8l, qh[step], st[0], 0, 0, 0);
+      }
+      // The next tile's loads go out between the products, none of which waits for the memory pipe then.
+      constexpr int kEach = (kChunks + kSteps - 1) / kSteps;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (step * kEach + i < kChunks) fetch_piece(step * kEach + i);
+      __builtin_amdgcn_sched_barrier(kNotLoads);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if (!none) {  // uniform over the wave
       const bool plain = odd[(u - w.begin) % 3] == 0;  // uniform
       float c = a.factor;
       if (kHalf || plain) {
@@ -348,12 +381,19 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[h][r]);
       mx = fmaxf(mx, XorLane<32>(mx)) * c;
       // The reference moves only when a score passes it far enough, so the sums are seldom scaled.
-      const float m_old = m;
-      if (mx > m + (kHeadroom + kSlack)) m = mx - kHeadroom;
-      const float base = m == -INFINITY ? 0.f : m;
-      const float corr = __builtin_amdgcn_exp2f(m_old - base);
+      const bool moves = mx > m + (kHeadroom + kSlack);
+      bool scale = __any(moves);  // uniform, as are far and mixed
+      float again = 1.f;
+      if (scale) {
+        if (moves) {
+          again = __builtin_amdgcn_exp2f(m - (mx - kHeadroom));
+          base = m = mx - kHeadroom;
+          l *= again;
+        }
+        far = __any(fabsf(base) >= kFarScore);
+      }
       float sum = 0.f, below = base;
-      if (__any(fabsf(base) >= kFarScore)) {
+      if (far) {
 #pragma unroll
         for (int h = 0; h < kSub; ++h)
 #pragma unroll
@@ -368,14 +408,17 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
           st[h][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[h][r], c, -below));
           sum += st[h][r];
         }
-      l = l * corr + sum;
-      float again = corr;
-      if constexpr (!kHalf) {
+      l += sum;
+      const float before = hi;  // the largest score of the tiles before, while all are of common scale
+      if constexpr (!kHalf) hi = fmaxf(hi, mx);
+      if (!kHalf && (mixed || !plain)) {
         // Values of common scale meet the weights as they are; others, and weights that are held otherwise since, times
         // the values' scales and a power of two that follows the largest of them.
         constexpr float kDown = 1.f / (1 << kUnits);
+        top = mixed ? top * again : __builtin_amdgcn_exp2f(before - base) * (kDown / kCommonScale);
+        mixed = true;
         if (plain) {
-          top = fmaxf(top * corr, __builtin_amdgcn_exp2f(mx - base) * (kDown / kCommonScale));
+          top = fmaxf(top, __builtin_amdgcn_exp2f(mx - base) * (kDown / kCommonScale));
         } else {
           float tile_top = 0.f;
 #pragma unroll
@@ -389,11 +432,12 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
                 tile_top = fmaxf(tile_top, fabsf(st[h][4 * r4 + e]));
               }
             }
-          top = fmaxf(top * corr, fmaxf(tile_top, XorLane<32>(tile_top)));
+          top = fmaxf(top, fmaxf(tile_top, XorLane<32>(tile_top)));
         }
         const int32_t power_old = power;
         power = WeightPower(top, power + kUnits) - kUnits;
-        again = ldexpf(corr, power - power_old);
+        again = ldexpf(again, power - power_old);
+        scale = true;
         if (!plain || __any(power != kCommonPower)) {
           const int32_t by = plain ? power - kCommonPower : power + kUnits;
 #pragma unroll
@@ -402,7 +446,7 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
             for (int r = 0; r < 16; ++r) st[h][r] = ldexpf(st[h][r], by);
         }
       }
-      if (__any(again != 1.f)) {
+      if (scale) {
 #pragma unroll
         for (int t = 0; t < kDims; ++t)
 #pragma unroll
@@ -448,12 +492,12 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
     if (u + 1 < w.end) put(buf ^ 1, (u + 1 - w.begin) % 3);
   }
 
-  // acc[t][r] is O^T[dim 32t + 8 (r / 4) + 4g + r % 4][row j].
+  // acc[t][r] is O^T[place 32t + 8 (r / 4) + 4g + r % 4][row j].
   l = l + XorLane<32>(l);
   if (w0 + j >= w.rows) return;
   // fp32: the sums hold 2^power times what they are, and where they may pass the largest float 2^-64 of that is left.
-  const bool far = !kHalf && power < kFarPower;
-  const int32_t down = kHalf ? 0 : far ? -power - kFarShift : -power;
+  const bool held = !kHalf && power < kFarPower;
+  const int32_t down = kHalf ? 0 : held ? -power - kFarShift : -power;
   const float inverse = w.splits > 1 ? 1.f : __fdiv_rn(1.f, l);
   float* dst = a.out + (static_cast<int64_t>(w.start + s) * a.heads + head) * a.dim;
   bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
@@ -463,18 +507,18 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
     vec = true;
     if (g == 0) {
       b.partial.ml[2 * at] = m;
-      b.partial.ml[2 * at + 1] = far ? -l : l;
+      b.partial.ml[2 * at + 1] = held ? -l : l;
     }
   }
 #pragma unroll
   for (int t = 0; t < kDims; ++t)
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
-      const int d = 32 * t + 8 * r4 + 4 * g;
+      const int d = dim_of(32 * t + 8 * r4 + 4 * g);
       f4 o;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = (kHalf ? acc[t][4 * r4 + e] : ldexpf(acc[t][4 * r4 + e], down)) * inverse;
-      if (!kHalf && far && w.splits == 1) o *= kFarUp;
+      if (!kHalf && held && w.splits == 1) o *= kFarUp;
       if (vec) {
         if (d < a.dim) *reinterpret_cast<f4*>(dst + d) = o;
       } else {
