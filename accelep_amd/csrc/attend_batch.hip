@@ -8,34 +8,41 @@ namespace {
 constexpr int kJoinRows = 4;  // of a workgroup and round
 constexpr int kJoinEach = 4;  // ranges in flight at once
 
-// A workgroup's threads are (row, key range, 16-byte piece). Workgroup (tile and key head, y) takes rows 4y .. 4y + 3
-// of each 4 * gridDim.y of a divided tile; prompt_tiles: tiles and key heads of the prompt's share, which come first.
-__global__ __launch_bounds__(kBatchThreads) void BatchJoinKernel(BatchLaunch args, uint32_t prompt_tiles, bool vec) {
+// A workgroup's threads are (row, key range, 16-byte piece). Its items are 4 rows of a divided tile and key head each,
+// taken in turn: how many tiles are divided is known on the device alone, mostly few of those that there is room for.
+__global__ __launch_bounds__(kBatchThreads) void BatchJoinKernel(BatchLaunch args, bool vec) {
   __shared__ __align__(16) f4 part_o[kBatchThreads];
   __shared__ float part_m[kBatchThreads];
   __shared__ float part_l[kBatchThreads];
   const BatchAttendArgs& a = args.a;
-  const bool prompt = blockIdx.x < prompt_tiles;
-  const BatchSplit& b = prompt ? args.prompt : args.step;
-  const int32_t tile_rows = prompt ? kPromptTileRows : kStepTileRows;
-  const int32_t block = static_cast<int32_t>(blockIdx.x - (prompt ? 0 : prompt_tiles));
-  const int32_t kv = block % a.kv_heads;
-  const int32_t which = block / a.kv_heads;
-  if (which >= b.tiles[0]) return;
-  const int32_t* tile = b.tiles + static_cast<int64_t>(kTileInts) * (1 + which);
-  const int32_t first = tile[0], splits = tile[1], start = tile[2], r0 = tile[3], rows = tile[4];
-  if (splits == 1) return;
+  const int32_t prompt_blocks = args.prompt.ranges > 0 ? args.prompt.tiles[0] * a.kv_heads : 0;
+  const int32_t step_blocks = args.step.ranges > 0 ? args.step.tiles[0] * a.kv_heads : 0;
+  const int32_t prompt_items = prompt_blocks * (kPromptTileRows / kJoinRows);
+  const int32_t step_items = step_blocks * (kStepTileRows / kJoinRows);
   const int32_t group = a.heads / a.kv_heads;
   const int dims = PartialDims(a.dim);
   const int pieces = dims / 4;
-  const int lanes = min(splits, kBatchThreads / (kJoinRows * pieces));
-  const int per_row = pieces * lanes;
-  const int local = static_cast<int>(threadIdx.x) / per_row;
-  const int rest = static_cast<int>(threadIdx.x) - local * per_row;
-  const int of = rest / pieces;
-  const int piece = rest - of * pieces;
-  for (int32_t base_row = kJoinRows * static_cast<int32_t>(blockIdx.y); base_row < rows;
-       base_row += kJoinRows * static_cast<int32_t>(gridDim.y)) {
+  for (int32_t item = static_cast<int32_t>(blockIdx.x); item < prompt_items + step_items;
+       item += static_cast<int32_t>(gridDim.x)) {
+    const bool prompt = item < prompt_items;
+    const BatchSplit& b = prompt ? args.prompt : args.step;
+    const int32_t tile_rows = prompt ? kPromptTileRows : kStepTileRows;
+    const int32_t local_item = prompt ? item : item - prompt_items;
+    const int32_t blocks = prompt ? prompt_blocks : step_blocks;
+    const int32_t row_group = local_item / blocks;  // all tiles' first rows first: many tiles have no others
+    const int32_t block = local_item - row_group * blocks;
+    const int32_t which = Quotient(block, a.by_kv_heads);
+    const int32_t kv = block - which * a.kv_heads;
+    const int32_t* tile = b.tiles + static_cast<int64_t>(kTileInts) * (1 + which);
+    const int32_t first = tile[0], splits = tile[1], start = tile[2], r0 = tile[3], rows = tile[4];
+    const int32_t base_row = kJoinRows * row_group;
+    if (splits == 1 || base_row >= rows) continue;  // uniform
+    const int lanes = min(splits, kBatchThreads / (kJoinRows * pieces));
+    const int per_row = pieces * lanes;
+    const int local = static_cast<int>(threadIdx.x) / per_row;
+    const int rest = static_cast<int>(threadIdx.x) - local * per_row;
+    const int of = rest / pieces;
+    const int piece = rest - of * pieces;
     const int32_t rl = base_row + local;
     const bool active = local < kJoinRows && rl < rows;
     const int64_t at0 = (static_cast<int64_t>(kv) * b.items + first) * tile_rows + rl;  // the next range's: tile_rows on
@@ -122,6 +129,10 @@ __global__ __launch_bounds__(kBatchThreads) void BatchJoinKernel(BatchLaunch arg
   }
 }
 
+// Workgroups of the join: enough to fill the CUs' threads. 24 short prompts with 2, 4, 8 and 16 a CU: 23.3, 21.0, 19.7 and
+// 20.0 us, chunks in a window 87.0, 84.8, 84.8 and 84.7; with one for each tile that there is room for 20.2 and 87.5.
+constexpr int64_t kJoinGroupsPerCu = 8;
+
 // One share of a call: the tiles of requests with few rows, or of those with many.
 struct Share {
   int32_t tile_rows;
@@ -167,17 +178,14 @@ BatchSplit SplitOf(const Share& s, int32_t few, char* scratch) {
 
 constexpr const char* kTooLarge = "Attention is too large";
 
-void LaunchJoin(const BatchLaunch& args, const Share& step, const Share& prompt, hipStream_t stream) {
+void LaunchJoin(const BatchLaunch& args, const Share& step, const Share& prompt, int64_t cus, hipStream_t stream) {
   const BatchAttendArgs& a = args.a;
-  const int64_t step_tiles = args.step.ranges > 0 ? step.divided * a.kv_heads : 0;
-  const int64_t prompt_tiles = args.prompt.ranges > 0 ? prompt.divided * a.kv_heads : 0;
-  if (step_tiles + prompt_tiles == 0) return;
+  const int64_t items = (args.step.ranges > 0 ? step.divided * kStepTileRows : 0) +
+                        (args.prompt.ranges > 0 ? prompt.divided * kPromptTileRows : 0);
+  if (items == 0) return;
   const bool vec = a.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
-  const int64_t rows = std::min<int64_t>(prompt_tiles > 0 ? kPromptTileRows : kStepTileRows,
-                                         int64_t(a.longest) * (a.heads / a.kv_heads));
-  const int64_t row_groups = (rows + kJoinRows - 1) / kJoinRows;
-  const dim3 grid(GridOf(step_tiles + prompt_tiles, kBatchThreads * row_groups, kTooLarge), static_cast<uint32_t>(row_groups));
-  hipLaunchKernelGGL(BatchJoinKernel, grid, dim3(kBatchThreads), 0, stream, args, static_cast<uint32_t>(prompt_tiles), vec);
+  const dim3 grid(static_cast<uint32_t>(std::min(items / kJoinRows * a.kv_heads, kJoinGroupsPerCu * cus)));
+  hipLaunchKernelGGL(BatchJoinKernel, grid, dim3(kBatchThreads), 0, stream, args, vec);
   Check(hipGetLastError(), "BatchJoinKernel launch");
 }
 
@@ -192,7 +200,10 @@ void LaunchAttendBatch(const BatchAttendArgs& a, hipStream_t stream) {
                    reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
   // Requests of up to 16 rows of a key head are the step tiles', larger ones the prompt tiles'. Where no request
   // has more, the first have all (also one that is longer than `longest` says); packed prompts, whose short ones
-  // have few keys too, are the second's.
+  // have few keys too, are the second's. 32 requests over 4000 tokens of 8 heads of 128, in step tiles and in prompt
+  // tiles: 4 or 16 rows 107 - 111 and 178 us in f16, 191 and 291 in fp32; 32 rows 143 and 150, 258 and 265; 64 rows
+  // 222 and 159, 454 and 283. At 32 rows the first gain 3 to 5 %, which is not worth a third rule. 24 packed prompts of 5
+  // .. 300 tokens: 28 and 21.
   constexpr int32_t kAll = 0x7fffffff;
   const bool steps_only = a.longest * group <= kStepTileRows;
   const bool steps = steps_only || (a.paged && group <= kStepTileRows);
@@ -200,10 +211,16 @@ void LaunchAttendBatch(const BatchAttendArgs& a, hipStream_t stream) {
   Share step{}, prompt{};
   if (steps) {
     const int64_t tiles = std::min<int64_t>(a.requests, a.rows) + (steps_only ? all_rows / kStepTileRows : 0);
+    // A step tile's range costs little to begin and join. With 2, 3 and 4 ranges a CU: 32 requests of up to 16384 tokens
+    // 142, 130 and 135 us, 125 of up to 2048 102, 97 and 97. At least 8 steps each, two a wave: 4 requests of a small
+    // model 12.1 us, with 4 11.8 and with 16 14.0.
     step = ShareOf(a, kStepTileRows, StepKeys(a.f16), tiles, 3 * cus, 8);
   }
   if (!steps_only) {
     const int64_t tiles = all_rows / kPromptTileRows + std::min<int64_t>(a.requests, all_rows / (few + 1));
+    // A prompt tile's part is 64 KB to write and to read again, so it is cut less: as if a CU had one. With 1, 1.5, 2 and
+    // 3 ranges a CU: chunks in a window 88, 110, 98 and 115 us; a mixed batch 339, 343, 365 and 411; heads of 80 126, 133,
+    // 145 and 140; long prompts 717, 718, 719 and 727. At least 4 steps each: 24 short prompts 20.2 us, with 8 22.8.
     prompt = ShareOf(a, kPromptTileRows, PromptKeys(a.f16), tiles, cus, 4);
   }
   // Where there is no memory for the parts the ranges stay whole.
@@ -228,7 +245,7 @@ void LaunchAttendBatch(const BatchAttendArgs& a, hipStream_t stream) {
   if (steps_only) LaunchBatchStep(args, vec, stream);
   else if (a.paged) LaunchBatchMixed(args, vec, stream);
   else LaunchBatchPrompt(args, vec, stream);
-  LaunchJoin(args, step, prompt, stream);
+  LaunchJoin(args, step, prompt, cus, stream);
 }
 
 }  // namespace accel_hip

@@ -1,6 +1,6 @@
 // C-ABI entry points for many requests served from one cache in pages: the tables of a step, pages taken
 // back, rows into pages, attention over pages and over packed prompts. The checks of arguments; the
-// kernels are in batch_tables.hip, cache_paged.hip and attend_batch*.hip. What lies in device memory (lengths,
+// kernels are in batch_tables.hip, cache_paged.hip and attend_batch*.{h,hip}. What lies in device memory (lengths,
 // tables, slots) is checked by the kernels that read it. No reference counterpart; checks and statuses follow
 // AppendCache and Attention in capi.cc.
 #include <algorithm>

@@ -5,6 +5,10 @@
 // behind the new pages before it: one scan of both over the requests, by one workgroup. A new page is
 // begun by exactly one new row, the one at a multiple of the page, so each row finds its own page without the
 // others: an old entry of the table, or an entry of the stack, which it also writes into the table.
+//
+// Bound: latency. 64 single tokens 5.1 us, of which a launch and a chain of lengths, two scans and a row's search, page
+// and stores; 1000 requests with 21000 rows 9.3 us in two launches, of which 5.6 are the scan. Their bytes would
+// take 0.1 us.
 #include <algorithm>
 
 #include "attend_split.h"
@@ -233,7 +237,8 @@ __global__ __launch_bounds__(kThreads) void ReleasePagesKernel(ReleasePagesArgs 
   if (threadIdx.x == 0) a.state[0] = static_cast<int32_t>(min(left + carry, int64_t(a.pages)));
 }
 
-// Rows from which on a second launch with many workgroups is worth its start.
+// Rows from which on a second launch with many workgroups is worth its start: 64 requests with 2048 rows take 8.0 us in
+// one and 9.7 in two launches, with 4096 9.6 and 9.9, with 8192 12.8 and 10.3.
 constexpr int32_t kOneGroupRows = 4096;
 
 }  // namespace

