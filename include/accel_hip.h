@@ -359,7 +359,8 @@ ACCEL_HIP_API int accel_hip_batch_tables(AccelHipBuffer counts, AccelHipBuffer l
 /* Cuts requests short: a request with keep[r] (below 0: 0) less than lengths[r] keeps that many tokens (0: it has
  * ended; drafts that were rejected go the same way). The pages past them, in the order of the requests and
  * of their tokens, go onto the pool's stack, their table entries become -1 and lengths[r] becomes keep[r].
- * Entries that are no page are left out. batch gives requests, width and the table; pool's state[1] stays. */
+ * Entries that are no page are left out; a page that two requests share goes on once for each, so it is taken
+ * out of one's table first. batch gives requests, width and the table; pool's state[1] stays. */
 ACCEL_HIP_API int accel_hip_release_pages(AccelHipBuffer keep, AccelHipBuffer lengths, const AccelHipPagePool* pool,
                                           const AccelHipBatch* batch);
 /* Rows of k and v (fp32, kv_heads * head_dim a row, row_stride apart) into their slots (int32 [rows]),
