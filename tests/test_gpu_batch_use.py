@@ -149,6 +149,40 @@ def test_starts_that_descend(kind):
     np.testing.assert_array_equal(x.call(), good)
 
 
+@pytest.mark.parametrize("name", "kv")
+@pytest.mark.parametrize("tokens", [[0], [70], [290], [0, 290], [33, 34, 130, 131, 200]])
+@pytest.mark.parametrize("power", [-30, -12, 12, 30])
+def test_few_rows_of_another_magnitude(name, tokens, power):
+    """Tiles of rows of ordinary size before, between and behind tiles that hold one of another, in prompts' tiles."""
+    rng = np.random.default_rng(power + 100 + tokens[-1])
+
+    def make(which, r, total):
+        x = rng.standard_normal((total, 2, 64))
+        if which == name:
+            x[tokens] *= 2.0 ** (power if name == "v" else min(power, 4))
+        return x
+
+    x = Paged(rng, [260], [60], 16, 8, 2, 64, "f32", make=make)
+    at, want, bound = x.want()
+    # What a weight or value loses of its 22 bits, at most 2^-24 of the largest value that a row sees, for each key.
+    big = max(np.abs(v.astype(np.float64)).max() for v in x.v)
+    assert_within(x.call()[at], want, bound + 2.0 ** -24 * 320 * big * 2.0 ** -3)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("order", [1, -1])
+def test_scores_that_grow_or_fall_along_the_keys(kind, order):
+    """The largest score of a row moves with nearly every tile, or is the first tile's."""
+    rng = np.random.default_rng(43)
+
+    def make(which, r, total):
+        x = rng.standard_normal((total, 2, 64))
+        return x * (np.linspace(0.05, 12, total)[::order, None, None] if which == "k" else 1)
+
+    x = Paged(rng, [300, 700], [50, 1], 16, 8, 2, 64, kind, make=make)
+    compare(x, x.call())
+
+
 # ---- threads and graphs --------------------------------------------------------------------------
 
 def attention_job(rng, kind, seen, new, window=0):
