@@ -15,6 +15,7 @@ namespace accel_hip {
 
 constexpr int kStepWaves = kBatchThreads / 64;
 constexpr uint32_t kLargeBits = (127 + 96) << 23;  // 2^96
+constexpr float kHeldWeight = 0x1p-40f;
 
 // The results of a workgroup's waves meet in LDS; l and o are held as in AttendPartial.
 template <int DP>
@@ -81,7 +82,9 @@ struct alignas(16) BatchParts {
 // A key or value row that is not finite would reach rows that do not see it, as 0 * NaN: a step that
 // holds one (a test of the bits, uniform) has its values taken as zeros and its weights as NaN, and so has a step
 // without a page. The same test finds values from 2^96 on, whose sum over the keys may pass the largest float: a row
-// that gives one of them a weight holds its sum times 2^-64 until that weight is next to nothing beside later ones.
+// that gives one of them a weight from 2^-40 on holds its sum times 2^-64 until that weight is next to nothing beside
+// later ones. Such a value is itself taken times 2^-64, and its weight, times 2^64 where the row's sum is not held, keeps
+// its bits however small it is: 2^-80 of 2^126 outweighs all ordinary values.
 template <int DP, int kLoad, bool kPaged>
 __device__ __forceinline__ void StepF32Group(const BatchAttendArgs& a, const BatchSplit& b, int32_t block,
                                              BatchParts<DP>& parts, BatchScan<kBatchThreads>& scan) {
@@ -235,19 +238,26 @@ __device__ __forceinline__ void StepF32Group(const BatchAttendArgs& a, const Bat
     m = m_new;
     float again = corr;
     share *= corr;
-    if (shift != 1.f && share < 0x1p-40f) {  // little is left of the large values
+    if (shift != 1.f && share < kHeldWeight) {  // little is left of the large values
       again *= kFarUp;
       shift = 1.f;
     }
     if (__any(large != 0)) {
       bool weighs = false;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) weighs = weighs || ((large >> e & 1) != 0 && p[e] > 0.f);
+      for (int e = 0; e < 4; ++e) weighs = weighs || ((large >> e & 1) != 0 && p[e] >= kHeldWeight);
       const uint64_t lanes = __ballot(weighs);
       if (((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) >> j & 1) != 0) {
         share = 1.f;
         again *= shift == 1.f ? kFarDown : 1.f;
         shift = kFarDown;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if ((large >> e & 1) == 0) continue;
+        p[e] *= kFarUp;
+#pragma unroll
+        for (int c = 0; c < kC; ++c) vx[e][c] *= kFarDown;
       }
     }
     if (__any(again != 1.f)) {

@@ -373,7 +373,8 @@ ACCEL_HIP_API int accel_hip_append_paged(AccelHipBuffer k, AccelHipBuffer v, con
  * with t > p - window. q's rows are row_stride floats apart, out is dense and may not overlap q, the cache
  * or the batch; padding rows of it stay as they were. Rounding: with an f16 cache, and with many rows
  * (over fp32), queries, softmax weights and fp32 keys and values enter the products with 22 bits (of their row's
- * largest value, the weights of the largest), otherwise with all; sums are fp32. A row whose query is not finite,
+ * largest value, the weights of the largest), otherwise with all, where a weight below 2^-126 of the largest may count
+ * as 0; sums are fp32 (of a row that gives a value from 2^96 on a weight, times 2^-64). A row whose query is not finite,
  * that sees a key or value that is not, a score past the largest float, or a token without a page (an entry of
  * the table that is none, a token past the table's width), is NaN; a value that no row sees has no say.
  * Inside a capture whose workspace was not grown before (by the same call, once), key ranges are not divided
