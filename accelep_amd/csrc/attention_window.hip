@@ -10,6 +10,7 @@ namespace {
 constexpr int kRows = 16;
 constexpr int kKeys = 16;  // of a wave's step
 constexpr uint32_t kLargeBits = (127 + 96) << 23;  // 2^96
+constexpr float kHeldWeight = 0x1p-40f;
 
 // One argument, not five: less of the host's work for a launch (a step over a window of 4096: 16.5 -> 16.1 us).
 struct StepArgs {
@@ -33,7 +34,9 @@ struct StepArgs {
 // A key or value row that is not finite would reach rows that do not see it, as 0 * NaN: a step that
 // holds one (a test of the bits, uniform) has its values taken as zeros and its weights as NaN. The same test
 // finds values from 2^96 on, whose sum over the keys may pass the largest float: a row that gives one of them a
-// weight holds its sum times 2^-64 until that weight is next to nothing beside later ones.
+// weight from 2^-40 on holds its sum times 2^-64 until that weight is next to nothing beside later ones. Such a value
+// is itself taken times 2^-64, and its weight, times 2^64 where the row's sum is not held, keeps its bits however
+// small it is: 2^-80 of 2^126 outweighs all ordinary values.
 template <int DP, int kLoad>
 __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
     StepArgs args) {
@@ -183,19 +186,26 @@ __global__ __launch_bounds__(64 * StepWaves(DP)) void AttendF32StepKernel(
     m = m_new;
     float again = corr;
     share *= corr;
-    if (shift != 1.f && share < 0x1p-40f) {  // little is left of the large values
+    if (shift != 1.f && share < kHeldWeight) {  // little is left of the large values
       again *= kFarUp;
       shift = 1.f;
     }
     if (__any(large != 0)) {
       bool weighs = false;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) weighs = weighs || ((large >> e & 1) != 0 && p[e] > 0.f);
+      for (int e = 0; e < 4; ++e) weighs = weighs || ((large >> e & 1) != 0 && p[e] >= kHeldWeight);
       const uint64_t lanes = __ballot(weighs);
       if (((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) >> j & 1) != 0) {
         share = 1.f;
         again *= shift == 1.f ? kFarDown : 1.f;
         shift = kFarDown;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if ((large >> e & 1) == 0) continue;
+        p[e] *= kFarUp;
+#pragma unroll
+        for (int c = 0; c < kC; ++c) vx[e][c] *= kFarDown;
       }
     }
     if (__any(again != 1.f)) {

@@ -308,8 +308,9 @@ ACCEL_HIP_API int accel_hip_attention_q8(AccelHipBuffer q, const AccelHipCacheQ8
  * row sees count for nothing, NaN included. q's rows are row_stride apart, out is dense and may not
  * overlap q, k or v. Sizes, captures and queries as above. Rounding: with many rows (more than 16 of a
  * key head, over a long range) queries, keys and values enter the products with 22 bits of their row's
- * largest value and weights with 22 bits of the largest; otherwise in fp32. A key or value that is not
- * finite makes the rows that see it NaN, and so does a score past the largest float. */
+ * largest value and weights with 22 bits of the largest; otherwise in fp32, where a weight below 2^-126 of the
+ * largest may count as 0, and the sums of a row that gives a value from 2^96 on a weight are held times 2^-64. A key
+ * or value that is not finite makes the rows that see it NaN, and so does a score past the largest float. */
 ACCEL_HIP_API int accel_hip_attention_window(AccelHipBuffer q, AccelHipBuffer k, AccelHipBuffer v, AccelHipBuffer out,
                                              int64_t seq, int64_t position, int64_t heads, int64_t kv_heads,
                                              int64_t head_dim, int64_t row_stride, int64_t window, int64_t sinks);
