@@ -41,7 +41,9 @@ constexpr float kBackFirst = 0x1p60f;
 constexpr uint32_t kCommonLow = 0x4800, kCommonHigh = 0x7800;  // f16's bits of 2^-6 and 2^6 times that
 // What a barrier of the scheduler's lets pass: vector and scalar arithmetic, LDS; no product and no load.
 constexpr int kNotLoads = 0x2 | 0x4 | 0x80;
-constexpr int32_t kUnits = 14;  // weights of up to 2^14 meet values' scales times 2^-14
+// Weights of up to 2^14 meet values' scales, 2^-127 .. 2^114, times 2^-1: all of these products are floats, and the
+// largest of a row, whose weight is 2^6 at least, is 2^-122 or more, so that what it loses below 2^-126 is within 2^-27.
+constexpr int32_t kUnits = 1;
 typedef short s4 __attribute__((ext_vector_type(4)));
 
 template <int DP, bool kHalf>
