@@ -12,7 +12,7 @@
 //    (e % 4) + 8 (e / 4) + 4g, and the value operand is read transposed from the row-major tile
 //    (ds_read_b64_tr_b16 gives a lane four keys of one dim).
 // An fp32 row enters as its parts times a power of two: 2^9 for rows whose largest magnitude lies in [2^-6, 2^6),
-// which keeps 22 bits of all of them, otherwise one from the row's own largest magnitude, whose
+// which keeps 22 bits of all of them, otherwise one from the row's own largest magnitude (of a row of zeros 2^127), whose
 // inverse meets its scores or weights. A row that is not finite, or has no page, has NaN there and zeros for values.
 //
 // Bound: the matrix cores, at the clock that they leave. Prompts of 474 .. 3410 tokens, 32 heads on 8 of 128, take
@@ -212,7 +212,7 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
       top = max(top, XorLane<4>(top));
       if (kPaged && !pages.Is(entry[0])) top = 0x7f800000u;  // uniform
       const bool finite = top < 0x7f800000u;
-      const float scale = RowScale(finite ? top : 0);
+      const float scale = RowScale(finite ? max(top, 1u) : 0);  // zeros: as of the smallest values, so that they weigh nothing
       odd[slot] = 1;
       row_back = finite ? 1.f / scale : NAN;
       write(scale, !finite);

@@ -127,3 +127,22 @@ def test_values_of_many_magnitudes(low, high, seen, new):
     x = Paged(rng, seen, new, 16, 4, 2, 64, "f32", make=lambda name, r, total: rng.uniform(-1, 1, (total, 2, 64)) * (
         3 if name == "k" else np.exp2(rng.integers(low, high + 1, (total, 1, 1)))))
     compare_many(x)
+
+
+@pytest.mark.parametrize("power", [-116, -60, -30, -12, -8, 0, 30])
+@pytest.mark.parametrize("zeros", [[0], [5, 6, 40], list(range(32)), list(range(64, 99))])
+@pytest.mark.parametrize("score", [0, 12])
+def test_rows_of_zeros_beside_small_values(power, zeros, score):
+    """A value row of zeros adds nothing to a row's sum, so the others keep their bits, also where it has the largest weight."""
+    rng = np.random.default_rng(len(zeros) + score)
+
+    def make(name, r, total):
+        if name == "k":
+            return keys_below(rng, total, zeros, [score] * len(zeros))
+        v = rng.standard_normal((total, 2, 64)) * 2.0 ** power
+        v[zeros] = 0
+        return v
+
+    x = Paged(rng, [100], [70], 16, 4, 2, 64, "f32", make=make)
+    queries(x)
+    compare_many(x)
