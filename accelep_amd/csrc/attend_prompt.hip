@@ -11,9 +11,10 @@
 //    (e % 4) + 8 (e / 4) + 4g, and the value operand is read transposed from the row-major tile
 //    (ds_read_b64_tr_b16 gives a lane four keys of one dim).
 // An fp32 row enters as its parts times a power of two, whose inverse takes the place of a block's scale:
-// 2^9 for rows whose largest magnitude lies in [2^-6, 2^6) (or that are zero), which keeps 22 bits of all
-// of them, and a tile of such rows has one scale; otherwise one from the row's own largest magnitude. A
-// row that is not finite has a NaN for a scale and zeros for values.
+// 2^9 for rows whose largest magnitude lies in [2^-6, 2^6) (or keys that are zero), which keeps 22 bits of all
+// of them, and a tile of such rows has one scale; otherwise one from the row's own largest magnitude (of values
+// that are zero 2^127, so that they take no bits from others). A row that is not finite has a NaN for a scale
+// and zeros for values.
 //
 // Bound: the matrix cores at the clock that they leave themselves (1.7-1.9 GHz under this load), with the
 // softmax and the split of its weights between their phases. 2048 rows from position 4097 on, 32 heads on
@@ -140,8 +141,9 @@ __global__ __launch_bounds__(kThreads, WavesPerSimd(DP, kLoad)) void AttendPromp
     }
   };
   // Writes a thread's pieces of one plane; tile row `key` begins at dst + key * stride, its second part
-  // `part` halves later.
-  const auto put_plane = [&](const uint4 (&x)[kChunks], _Float16* dst, int stride, int part, float& row_back, int slot) {
+  // `part` halves later. least: 0, or 1 for values, the bits of what a row of zeros counts as.
+  const auto put_plane = [&](const uint4 (&x)[kChunks], _Float16* dst, int stride, int part, float& row_back, int slot,
+                             uint32_t least) {
     if (kF32) {
       // The row's largest magnitude: of the bits as signed numbers for its positive values, as unsigned
       // ones for its negative.
@@ -156,7 +158,7 @@ __global__ __launch_bounds__(kThreads, WavesPerSimd(DP, kLoad)) void AttendPromp
       uint32_t top = max(static_cast<uint32_t>(pos), neg & 0x7fffffffu);
       top = max(top, XorLane<1>(top));
       top = max(top, XorLane<2>(top));
-      top = max(top, XorLane<4>(top));
+      top = max(max(top, XorLane<4>(top)), least);
       float scale = kCommonScale, back = 1.f / kCommonScale;
       const bool common = top == 0 || (top >= kCommonLow && top < kCommonHigh);
       if (!__all(common)) {
@@ -205,8 +207,8 @@ __global__ __launch_bounds__(kThreads, WavesPerSimd(DP, kLoad)) void AttendPromp
   };
   const auto put = [&](int buf, int slot) {
     float k_back = 1.f, v_back = 1.f;
-    put_plane(kreg, &kt[buf][0][0][0], kKStride, kKeys * kKStride, k_back, slot);
-    put_plane(vreg, &vt[buf][0][0][0], kVStride, kKeys * kVStride, v_back, slot);
+    put_plane(kreg, &kt[buf][0][0][0], kKStride, kKeys * kKStride, k_back, slot, 0);
+    put_plane(vreg, &vt[buf][0][0][0], kVStride, kKeys * kVStride, v_back, slot, 1);
     if (kF32) {
       move_nan(k_back, v_back);
       if (tid % 8 == 0) {
