@@ -79,7 +79,7 @@ class Batch(C.Structure):
     """AccelHipBatch."""
 
     _fields_ = [("seen", Buffer), ("starts", Buffer), ("table", Buffer), ("requests", C.c_int64), ("rows", C.c_int64),
-                ("width", C.c_int64), ("longest", C.c_int64)]
+                ("width", C.c_int64), ("longest", C.c_int64), ("slots", Buffer)]
 
 
 class PagePool(C.Structure):

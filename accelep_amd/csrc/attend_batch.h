@@ -300,6 +300,12 @@ __device__ __forceinline__ bool BatchQueryVec(const BatchAttendArgs& a) {  // un
   return a.dim % 4 == 0 && a.q_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
 }
 
+// Whether row i of the batch was put into the cache. A row that was not is answered as one whose query is not finite: its
+// request may have been refused a page, and what lies where its key would be may be of another.
+__device__ __forceinline__ bool BatchRowStored(const BatchAttendArgs& a, int32_t i) {
+  return a.slots == nullptr || static_cast<uint32_t>(a.slots[i]) < static_cast<uint32_t>(a.pages) << a.page_shift;
+}
+
 constexpr int kBatchThreads = 256;
 constexpr int kStepTileRows = 16, kPromptTileRows = 128;
 constexpr int StepKeys(bool f16) { return f16 ? 32 : 16; }

@@ -273,6 +273,7 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
   {
     const float* q = a.q + (w.start + s) * a.q_stride + static_cast<int64_t>(head) * a.dim;
     const bool vec = BatchQueryVec(a);
+    const bool stored = !kPaged || BatchRowStored(a, w.start + s);
     float x[kSteps][2][4];
     uint32_t top = 0;
 #pragma unroll
@@ -290,7 +291,7 @@ __device__ __forceinline__ void PromptGroup(const BatchAttendArgs& a, const Batc
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[st][e >> 2][e & 3]) & 0x7fffffffu);
     top = max(top, XorLane<32>(top));
-    const float scale = top >= 0x7f800000u ? NAN : RowScale(top);  // no finite row: all of it NaN
+    const float scale = top >= 0x7f800000u || !stored ? NAN : RowScale(top);  // no finite row: all of it NaN
     row_back = 1.f / scale;
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {

@@ -150,6 +150,7 @@ __device__ __forceinline__ void StepF32Group(const BatchAttendArgs& a, const Bat
       q[i] = f4{x[0], x[1], x[2], x[3]};
     }
   }
+  const bool stored = !kPaged || BatchRowStored(a, w.start + s);
   if (u < w.end) {
     entry = __builtin_amdgcn_readfirstlane(entry);
     load_k(key_of(u), entry);
@@ -160,6 +161,7 @@ __device__ __forceinline__ void StepF32Group(const BatchAttendArgs& a, const Bat
   for (int i = 0; i < kI; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) q[i][e] = 16 * i + 4 * g + e < a.dim ? q[i][e] : 0.f;
+  if (!stored) q[0][0] = NAN;
 
   float m = -INFINITY, l = 0.f;  // l: this lane's share of the row's sum
   float shift = 1.f, share = 0.f;  // the weighted sum's power of two, and the largest weight now of a large value
@@ -402,6 +404,7 @@ __device__ __forceinline__ void StepF16Group(const BatchAttendArgs& a, const Bat
 #pragma unroll
     for (int i = 0; i < kC; ++i) LoadBatchQuery(q, a.dim, 64 * i + 16 * g, vec, x[i]);
   }
+  const bool stored = BatchRowStored(a, w.start + s);
   if (u < w.end) {
     uniform(entry, entry);
     load_k(key_of(u), entry);
@@ -422,7 +425,7 @@ __device__ __forceinline__ void StepF16Group(const BatchAttendArgs& a, const Bat
       for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
     top = max(top, XorLane<16>(top));
     top = max(top, XorLane<32>(top));
-    const float scale = top >= 0x7f800000u ? NAN : RowScale(top);  // no finite row: all of it NaN
+    const float scale = top >= 0x7f800000u || !stored ? NAN : RowScale(top);  // no finite row: all of it NaN
     factor = 1.f / scale * a.factor;
 #pragma unroll
     for (int i = 0; i < kC; ++i)

@@ -243,14 +243,16 @@ ACCEL_HIP_API int accel_hip_attention_paged(AccelHipBuffer q, const AccelHipCach
     size_t table_bytes = 0, q_bytes = 0, out_bytes = 0;
     CheckBatch(batch, a.page_shift, true, &table_bytes);
     const size_t seen_bytes = CheckedIntBytes(batch->requests);
+    const size_t slot_bytes = batch->slots.data == nullptr ? 0 : CheckedIntBytes(batch->rows);
     RequireInts(batch->seen, seen_bytes, "the batch's seen tokens are out of range");
     RequireInts(batch->table, table_bytes, "the batch's table is out of range");
+    RequireInts(batch->slots, slot_bytes, "the batch's slots are out of range");
     const bool any = CheckAttend(q, batch, out, heads, cache->kv_heads, cache->head_dim, row_stride, window, &q_bytes,
                                  &out_bytes, &a);
     const Part outputs[] = {{&out, out_bytes}};
     const Part inputs[] = {{&q, q_bytes}, {&cache->k, plane}, {&cache->v, plane}, {&batch->starts, StartsBytes(batch)},
-                           {&batch->seen, seen_bytes}, {&batch->table, table_bytes}};
-    RequireApart(outputs, 1, inputs, 6, "Attention output overlaps what is read");
+                           {&batch->seen, seen_bytes}, {&batch->table, table_bytes}, {&batch->slots, slot_bytes}};
+    RequireApart(outputs, 1, inputs, 7, "Attention output overlaps what is read");
     if (!any) return;
     NoteDeviceWrite(out.data, out_bytes);
     a.k = cache->k.data;
@@ -262,6 +264,7 @@ ACCEL_HIP_API int accel_hip_attention_paged(AccelHipBuffer q, const AccelHipCach
     a.pages = static_cast<int32_t>(cache->pages);
     a.f16 = cache->type == ACCEL_HIP_CACHE_F16;
     a.paged = true;
+    a.slots = slot_bytes == 0 ? nullptr : static_cast<const int32_t*>(batch->slots.data);
     LaunchAttendBatch(a, Ctx().stream);
   });
 }

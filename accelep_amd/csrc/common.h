@@ -553,6 +553,7 @@ struct BatchAttendArgs {
   float factor;  // log2(e) / sqrt(dim): scores in log2 units
   bool f16, paged;
   QuickDivisor group, by_kv_heads;  // of heads / kv_heads, and of kv_heads
+  const int32_t* slots;  // the rows', or null: all of them are in the cache
 };
 void LaunchAttendBatch(const BatchAttendArgs& a, hipStream_t stream);
 // rng_inout is a device word holding the xorshift32 state; index_dev offsets `chosen`.

@@ -332,12 +332,15 @@ typedef struct AccelHipCachePaged {
  * request r are starts[r] .. starts[r + 1] - 1, its first token is its token seen[r]. table[r] are the pages
  * of its tokens in order. rows is what there is room for; rows past starts[requests] are padding. Where starts
  * descend, the output's rows (no others) hold anything. longest is the most new rows of one request where the
- * host knows it, otherwise 0: it chooses kernels, not results. */
+ * host knows it, otherwise 0: it chooses kernels, not results. slots, where it has data, are the rows' slots as
+ * accel_hip_batch_tables wrote them and accel_hip_append_paged took them: a row without one is not in the cache,
+ * and accel_hip_attention_paged gives it NaN. The other calls do not read it. */
 typedef struct AccelHipBatch {
   AccelHipBuffer seen;   /* int32 [requests] */
   AccelHipBuffer starts; /* int32 [requests + 1] */
   AccelHipBuffer table;  /* int32 [requests, width] */
   int64_t requests, rows, width, longest;
+  AccelHipBuffer slots;  /* int32 [rows], or none */
 } AccelHipBatch;
 /* The pages that no request owns: the first state[0] entries of `stack`, the last of them taken first. */
 typedef struct AccelHipPagePool {
@@ -351,7 +354,10 @@ typedef struct AccelHipPagePool {
  * position and its slot (padding: 0 and -1); lengths_after (lengths + counts) and state_after, which may be
  * `lengths` and the pool's state themselves. A request whose new pages are not all there, nor those of the requests
  * before it, or do not fit its table row, takes none: its rows have slot -1, its missing entries become -1,
- * its length stays, and it is counted in state_after[1]. Who needs no new page is always served. Other
+ * its length stays, and it is counted in state_after[1]. Its first new tokens may belong on a page that it has: they
+ * are not written there, so what the page held before, another request's tokens perhaps, is still there, and only the
+ * batch's slots keep attention from it; without them all its rows of the output mean nothing. Who needs no new page
+ * is always served. Other
  * outputs may overlap neither one another nor the inputs. More than 2048 requests or 4096 rows take a workspace,
  * which a call before a capture has to have grown. */
 ACCEL_HIP_API int accel_hip_batch_tables(AccelHipBuffer counts, AccelHipBuffer lengths, const AccelHipPagePool* pool,
@@ -377,7 +383,8 @@ ACCEL_HIP_API int accel_hip_append_paged(AccelHipBuffer k, AccelHipBuffer v, con
  * largest value, the weights of the largest), otherwise with all, where a weight below 2^-126 of the largest may count
  * as 0; sums are fp32 (of a row that gives a value from 2^96 on a weight, times 2^-64). A row whose query is not finite,
  * that sees a key or value that is not, a score past the largest float, or a token without a page (an entry of
- * the table that is none, a token past the table's width), is NaN; a value that no row sees has no say.
+ * the table that is none, a token past the table's width), or whose slot (where the batch has slots) is outside the
+ * cache, is NaN; a value that no row sees has no say.
  * Inside a capture whose workspace was not grown before (by the same call, once), key ranges are not divided
  * over workgroups. */
 ACCEL_HIP_API int accel_hip_attention_paged(AccelHipBuffer q, const AccelHipCachePaged* cache, const AccelHipBatch* batch,

@@ -154,4 +154,25 @@ def test_an_f16_cache_takes_half_the_bytes():
                 "overlap" if call == "append" else "window")
 
 
+def test_the_slots_of_a_batch():
+    """Where a batch has them, attention over pages checks them like its other parts; the other calls do not look."""
+    at, size = PLACES["slots"]
+    for slots, text in ((buf(size - 1, at * GIB), "slots are out of range"), (buf(size, at * GIB + 2), "slots are out of range"),
+                        (buf(size, PLACES["out"][0] * GIB), "overlap"), (buf(size, PLACES["out"][0] * GIB + 4 - size), "overlap"),
+                        (buf(size, PLACES["out"][0] * GIB + PLACES["out"][1] - 4), "overlap")):
+        c = Call()
+        c.batch.slots = slots
+        refused(c.paged(), text)
+        c = Call(window=-1)  # refused for that, behind the checks of the batch
+        c.batch.slots = slots
+        refused(c.packed(), "window")
+    c = Call(window=-1)
+    c.batch.slots = buf(size, at * GIB)
+    refused(c.paged(), "window")
+    c = Call(page=8)
+    c.batch.slots = buf(1, at * GIB + 1)
+    refused(c.tables(), "power of two")
+    refused(c.release(), "power of two")
+
+
 assert INVALID == 1
