@@ -16,16 +16,23 @@
 // inverse meets its scores or weights. A row that is not finite, or has no page, has NaN there and zeros for values.
 //
 // Bound: the matrix cores, at the clock that they leave. Prompts of 474 .. 3410 tokens, 32 heads on 8 of 128, take
-// 704 - 717 us, 287 - 292 TFLOP/s counted once and three f16 products each; these products alone, from registers, 475. The cores
+// 693 - 732 us, 281 - 297 TFLOP/s counted once and three f16 products each; these products alone, from registers and over
+// random values, 372, at a large library product's rate 468. The cores
 // are busy 41 % of the cycles, at 1.9 GHz. A workgroup by itself took 4100 cycles a tile of 32 keys: 1536 of products,
 // 510 of softmax, 700 to send the loads in a burst, 800 to split rows and weights; a second one on the CU fills part
 // of that. So
-//  * two workgroups a CU (244 registers at head dim 128), rather than tiles of 256 rows, which spill;
+//  * two workgroups a CU (at head dim 128 245 registers for packed prompts, 251 over fp32 pages and 255 over f16 ones),
+//    rather than tiles of 256 rows, which spill;
 //  * loads go out between the score products, and what only tiles of odd scales or moving references need is behind
 //    uniform branches (144 -> 126 us for 3 prompts of 16 heads of 80). Splitting rows between the value products
 //    as well would spill 72 registers at 128;
 //  * no other part is the bound by itself: of 735 us before these steps, without softmax 592, without the split and
 //    its stores 649, without the loads 692; with 15 % fewer vector instructions in all 735.
+// Head dims of 129 .. 256 are worked on as 256, in one workgroup a CU, and do not fit its 512 registers: 38 are spilled for
+// packed prompts, 45 over fp32 pages, 62 over f16 ones. 5 prompts of 426 .. 1819 tokens, 16 heads on 4: 524 us at 256 and 519
+// at 192 (165 at 128); chunks of 200 .. 500 over up to 4000 tokens 169 and 164 in fp32 (62), 120 and 116 in f16 (48).
+// Rows off the 16-byte grid are loaded an element at a time, from head dim 65 on in one workgroup a CU too, at 256 with 94 to
+// 338 registers spilled: the same chunks over f16 with heads of 100 take 88 us, of 96 43.
 #pragma once
 
 #include "attend_batch_step.h"

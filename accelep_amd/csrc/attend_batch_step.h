@@ -5,8 +5,11 @@
 // barriers in the loop; a step's keys lie in one or two pages, whose table entries are read a step ahead.
 // Lane (j, g) = (lane % 16, lane / 16). Bound: the bytes of the keys and values. 32 requests of 512 .. 16384 tokens in f16
 // (32 heads on 8 of 128): 130 us, 4.7 TB/s, with the join; a large copy reaches 5.16. 125 requests of 16 .. 2048 in fp32:
-// 97 us, 4.4 TB/s. 4 requests of a small model: 12 us, of which 8.3 this kernel (lengths, query, one page entry, keys,
-// softmax and values wait for one another) and 3.6 the join.
+// 97 - 105 us, 4.1 - 4.4 TB/s. 4 requests of a small model: 12 us, of which 8.3 this kernel (lengths, query, one page entry,
+// keys, softmax and values wait for one another) and 3.6 the join. Rows off the 16-byte grid (f16 head dims that are no
+// multiple of 8, memory that is not aligned) are loaded an element at a time, from head dim 65 on in one workgroup a CU: the
+// 32 requests with heads of 100 take 522 us, of 96 111; in fp32, where 100 is on the grid, 205 and 195. Head dim 256, 16 heads
+// on 4, the same bytes as 32 on 8 of 128: 146 us in f16, 258 in fp32, where 128 takes 130 and 222.
 #pragma once
 
 #include "attend_batch.h"

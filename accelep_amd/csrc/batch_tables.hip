@@ -180,6 +180,10 @@ __global__ __launch_bounds__(kThreads) void BatchRowsKernel(BatchTablesArgs a, c
 
 // A wave a request, twice: its pages are counted, the counts summed over the requests, and the pages put where the
 // sums say. Between, the chunk's counts are in LDS.
+// Bound: latency. Each of the 16 waves goes from request to request, and waits for its lengths and for 64 entries at a
+// time. Requests of 500 .. 4000 tokens, pages of 64: 1000 of which none is cut 29 us, ten of them 30, all by up to
+// 4 tokens 38, all of them ended 102 (pages of 16: 187); 64 requests over pages of 16 4.7, by up to 4 tokens 6.5, all
+// ended 16. The bytes of the largest would take 0.1 us.
 __global__ __launch_bounds__(kThreads) void ReleasePagesKernel(ReleasePagesArgs a) {
   __shared__ Sums of_wave[kWaves];
   __shared__ int32_t count[kThreads];
