@@ -1,7 +1,7 @@
 // Batches over pages with requests of few new rows and of many. Both kinds of tiles are workgroups of one launch: those
 // of many rows come first and keep the matrix cores busy, those of few fill the CUs' memory time and the end. Both
 // run two workgroups a CU. 30 single tokens beside chunks of 1071 and 1196 over 1000 .. 9000 tokens in f16 (32 heads on 8
-// of 128): 328 - 342 us, with the join; in two launches one behind the other 477, when one took 374. Bound: the chunks' products (195 us at a large product's
+// of 128): 328 - 347 us, with the join; in two launches one behind the other 477, when one took 374. Bound: the chunks' products (195 us at a large product's
 // rate) and their softmax.
 #include "attend_batch_prompt.h"
 

@@ -16,7 +16,7 @@
 // inverse meets its scores or weights. A row that is not finite, or has no page, has NaN there and zeros for values.
 //
 // Bound: the matrix cores, at the clock that they leave. Prompts of 474 .. 3410 tokens, 32 heads on 8 of 128, take
-// 693 - 732 us, 281 - 297 TFLOP/s counted once and three f16 products each; these products alone, from registers and over
+// 693 - 753 us, 274 - 297 TFLOP/s counted once and three f16 products each; these products alone, from registers and over
 // random values, 372, at a large library product's rate 468. The cores
 // are busy 41 % of the cycles, at 1.9 GHz. A workgroup by itself took 4100 cycles a tile of 32 keys: 1536 of products,
 // 510 of softmax, 700 to send the loads in a burst, 800 to split rows and weights; a second one on the CU fills part
